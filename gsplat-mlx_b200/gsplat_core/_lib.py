@@ -85,6 +85,16 @@ class RasterParams(ct.Structure):
                 ("tile_order", _vp), ("tile_cost", _vp)]
 
 
+class DropoutParams(ct.Structure):
+    _fields_ = [("rows", _i64), ("width", _i64), ("seed", ct.c_uint64), ("step", ct.c_uint64),
+                ("p", ct.c_double), ("dtype", _i32), ("by_row", _i32)]
+
+
+class GroupedParams(ct.Structure):
+    _fields_ = [("rows", _i64), ("n", _i64), ("groups", _i32), ("in_features", _i32),
+                ("out_features", _i32), ("dtype", _i32), ("activation", _i32), ("use_row_ids", _i32)]
+
+
 _P = ct.POINTER
 
 # (name, restype, argtypes); every exported symbol of include/gsplat_b200.h.
@@ -141,6 +151,11 @@ SIGNATURES = {
     "gs_densify_accumulate": (ct.c_int, [_P(DensifyParams)] + [_vp] * 6),
     "gs_densify_masks": (ct.c_int, [_P(DensifyMaskParams)] + [_vp] * 10),
     "gs_spz_attributes": (ct.c_int, [_P(SpzParams)] + [_vp] * 13),
+    "gs_dropout": (ct.c_int, [_P(DropoutParams)] + [_vp] * 4),
+    "gs_group_offsets": (ct.c_int, [_i64, _vp, _i32, _vp, _vp]),
+    "gs_grouped_linear_fwd": (ct.c_int, [_P(GroupedParams)] + [_vp] * 7),
+    "gs_grouped_linear_bwd_workspace_size": (_sz, [_P(GroupedParams)]),
+    "gs_grouped_linear_bwd": (ct.c_int, [_P(GroupedParams)] + [_vp] * 10 + [_sz, _vp]),
     "gs_rasterize_fwd": (ct.c_int, [_P(RasterParams)] + [_vp] * 12),
     "gs_rasterize_bwd": (ct.c_int, [_P(RasterParams)] + [_vp] * 19),
 }

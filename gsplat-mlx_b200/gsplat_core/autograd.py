@@ -15,6 +15,9 @@ Primitives' ``vjp`` methods, as ``torch.autograd.Function`` s.
   (gsplat_rasterize.cpp:749-795): absgrad off, gradients for means2d,
   conics, colors, opacities and backgrounds (when given).
 
+* ``grouped_linear`` and ``dropout`` -- a learned layer per camera and the
+  counter-based dropout (no counterpart in the reference).
+
 Every forward and backward runs the native kernels through the drop-in
 functions of ``_gsplat_core``; integer outputs (radii, last_ids) are
 non-differentiable.
@@ -24,6 +27,8 @@ from __future__ import annotations
 import torch
 
 from . import _gsplat_core as G
+from .dropout import dropout_backward, dropout_forward
+from .grouped import grouped_linear_backward, grouped_linear_forward
 
 
 def _empty_like_none(x):
@@ -194,3 +199,52 @@ def rasterize_to_pixels_3dgs(means2d, conics, colors, opacities, tile_offsets, f
     return _RasterizeToPixels3DGS.apply(means2d, conics, colors, opacities, backgrounds, masks,
                                         tile_offsets, flatten_ids, int(width), int(height),
                                         int(tile_size))
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weights, offsets, biases, row_ids, activation):
+        y = grouped_linear_forward({"x": x, "weights": weights, "offsets": offsets,
+                                    "biases": biases, "row_ids": row_ids}, activation)
+        ctx.save_for_backward(x, weights, offsets, biases, row_ids,
+                              y if activation != "none" else None)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    def backward(ctx, v_y):
+        x, weights, offsets, biases, row_ids, y = ctx.saved_tensors
+        names = {"v_x": 0, "v_weights": 1, "v_biases": 3}
+        g = grouped_linear_backward({"x": x, "weights": weights, "offsets": offsets,
+                                     "biases": biases, "row_ids": row_ids}, y, v_y,
+                                    ctx.activation,
+                                    [k for k, i in names.items() if ctx.needs_input_grad[i]])
+        return g.get("v_x"), g.get("v_weights"), None, g.get("v_biases"), None, None
+
+
+def grouped_linear(x, weights, offsets, biases=None, row_ids=None, activation="none"):
+    """Differentiable grouped_linear_forward: gradients for x, weights and
+    biases."""
+    return _GroupedLinear.apply(x, weights, offsets, biases, row_ids, str(activation))
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, step, rows):
+        # a step tensor is saved, so that changing it before the backward
+        # raises instead of drawing another mask
+        ctx.save_for_backward(step if isinstance(step, torch.Tensor) else None)
+        ctx.cfg = (p, seed, None if isinstance(step, torch.Tensor) else step, rows)
+        return dropout_forward(x, p, seed, step, rows)
+
+    @staticmethod
+    def backward(ctx, v_y):
+        p, seed, step, rows = ctx.cfg
+        step = ctx.saved_tensors[0] if step is None else step
+        return dropout_backward(v_y, p, seed, step, rows), None, None, None, None
+
+
+def dropout(x, p, seed, step=0, rows=False):
+    """Differentiable dropout_forward: the mask is drawn again in the
+    backward, not stored."""
+    return _Dropout.apply(x, p, seed, step, rows)

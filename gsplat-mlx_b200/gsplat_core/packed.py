@@ -13,15 +13,22 @@ The rows are exactly the dense outputs' visible entries; the sorted lists
 are the dense lists with element ids replaced by row ids, so renders and
 gradients equal the dense path's.  ``unpack_rows`` scatters per-row
 gradients back to the dense [I, N, ...] layout of the projection backward.
+
+Colours learned per camera: ``camera_colors_forward`` turns the Gaussians'
+features [N, K] into the rows' colours (or 1-64 feature channels) with each
+row's own camera's weights, ``camera_colors_backward`` is its reverse mode
+(gsplat_core.grouped, on the rows' image bounds packed["image_offsets"]).
 """
 from __future__ import annotations
 
 import ctypes as ct
+import math
 
 import torch
 
 from . import _lib
 from ._lib import IsectParams, RasterParams, check
+from .grouped import group_offsets, grouped_linear_backward, grouped_linear_forward
 
 
 def _p(t):
@@ -36,7 +43,8 @@ def pack_projection(proj):
     """Packed rows of a dense projection output (radii [..., N, 2], means2d,
     depths, conics, compensations [..., N] or [0]): {"image_ids",
     "gaussian_ids", "radii", "means2d", "depths", "conics", "compensations"
-    (or None)} with nnz rows, image = flattened leading index."""
+    (or None)} with nnz rows, image = flattened leading index, and
+    "image_offsets" [I + 1]: image i's rows are offsets[i] .. offsets[i+1] - 1."""
     radii = proj["radii"].contiguous()
     N = radii.shape[-2]
     n = radii.numel() // 2
@@ -63,7 +71,29 @@ def pack_projection(proj):
            "means2d": f32(nnz, 2), "depths": f32(nnz), "conics": f32(nnz, 3),
            "compensations": f32(nnz) if comps is not None else None}
     call(nnz, out)
+    out["image_offsets"] = group_offsets(out["image_ids"], math.prod(radii.shape[:-2]))
     return out
+
+
+def _camera_inputs(features, weights, biases, packed):
+    return {"x": features, "weights": weights, "biases": biases,
+            "offsets": packed["image_offsets"], "row_ids": packed["gaussian_ids"]}
+
+
+def camera_colors_forward(features, weights, biases, packed, activation="sigmoid"):
+    """[nnz, M] colours of the packed rows from the Gaussians' features
+    [N, K] and per-camera weights [I, M, K] and biases [I, M] (or None)."""
+    return grouped_linear_forward(_camera_inputs(features, weights, biases, packed), activation)
+
+
+def camera_colors_backward(features, weights, biases, packed, colors, v_colors,
+                           activation="sigmoid"):
+    """{"v_features", "v_weights", "v_biases" (with biases)} from the
+    forward's colours and their gradient."""
+    g = grouped_linear_backward(_camera_inputs(features, weights, biases, packed), colors,
+                                v_colors, activation)
+    g["v_features"] = g.pop("v_x")
+    return g
 
 
 def intersect_tile_packed_forward(packed, I, tile_size, tile_width, tile_height):

@@ -639,6 +639,79 @@ int gs_spz_attributes(const gs_spz_params* p, const float* means,
                       float* scales, float* rotations, float* alphas,
                       float* colors, float* sh, gs_stream_t stream);
 
+/* ------------------------------------------------------------------ */
+/* Learned colours per camera: grouped products, dropout.  No          */
+/* counterpart in the reference.                                       */
+/* ------------------------------------------------------------------ */
+enum gs_dtype { GS_F32 = 0, GS_BF16 = 1, GS_F16 = 2 };
+
+typedef struct {
+  int64_t rows, width; /* x is [rows, width]                                */
+  uint64_t seed;       /* the generator's key                               */
+  uint64_t step;       /* the draw: another step is another mask            */
+  double p;            /* probability of a drop, in [0, 1]                  */
+  int32_t dtype;       /* gs_dtype of x and y                               */
+  int32_t by_row;      /* 1: a row is kept or dropped as a whole (width
+                          below 2^24); 0: every value by itself             */
+} gs_dropout_params;
+
+/* y = x / (1 - p) where the mask keeps and 0 where it drops (a select: what
+ * a dropped place holds, NaN too, does not matter).  The mask is a function
+ * of (seed, step, index) and is not stored: the backward is the same call
+ * on v_y.  Index i (the row, or the value's row-major place) is dropped when
+ * word i % 4 of Philox4x32-7 (Salmon et al. 2011) with key = seed (low word
+ * first) and counter = (i / 4 low, i / 4 high, step low, step high) is below
+ * p 2^32 rounded to nearest even.  step_device, if given, is an int64 in
+ * device memory that is added to step when the kernel runs, so that a
+ * captured graph draws another mask at each replay.  y may be x. */
+int gs_dropout(const gs_dropout_params* p, const void* x, const int64_t* step_device,
+               void* y, gs_stream_t stream);
+
+/* offsets[g] = how many of the n sorted ids are below g, g = 0..groups: the
+ * ragged group bounds of rows sorted by group (packed rows by image). */
+int gs_group_offsets(int64_t n, const int32_t* sorted_ids, int32_t groups,
+                     int32_t* offsets, gs_stream_t stream);
+
+enum gs_activation { GS_ACT_NONE = 0, GS_ACT_RELU = 1, GS_ACT_SIGMOID = 2 };
+
+typedef struct {
+  int64_t rows;         /* R, below 2^31                                    */
+  int64_t n;            /* rows of x: R without row_ids; below 2^31         */
+  int32_t groups;       /* G                                                */
+  int32_t in_features;  /* K                                                */
+  int32_t out_features; /* M                                                */
+  int32_t dtype;        /* gs_dtype of x, weights, biases, y and gradients  */
+  int32_t activation;   /* gs_activation                                    */
+  int32_t use_row_ids;  /* 1: row_ids is given; 0: id(r) = r                */
+} gs_grouped_params;
+
+/* y[r] = act(weights[g] x[id(r)] + biases[g]) for offsets[g] <= r <
+ * offsets[g + 1]: x [n,K], weights [G,M,K], biases [G,M] or NULL, offsets
+ * [G+1] int32 ascending, row_ids [R] int32 (with use_row_ids), y [R,M].
+ * Sums are in fp32 and rounded once.  Rows outside every group are written
+ * as zeros; an id outside [0, n) reads a row of zeros.  Offsets that do not
+ * ascend give unspecified values and no access out of bounds. */
+int gs_grouped_linear_fwd(const gs_grouped_params* p, const void* x,
+                          const int32_t* row_ids, const int32_t* offsets,
+                          const void* weights, const void* biases, void* y,
+                          gs_stream_t stream);
+
+size_t gs_grouped_linear_bwd_workspace_size(const gs_grouped_params* p);
+
+/* Its reverse mode from y (the forward's; may be NULL for GS_ACT_NONE) and
+ * v_y [R,M].  With v_z = v_y act'(y): v_x [n,K] = the sum over the rows that
+ * read it of v_z[r] weights[g] (zeros where none does), v_weights [G,M,K] =
+ * the sum over g's rows of v_z[r]^T x[id(r)], v_biases [G,M] = the sum of
+ * v_z[r]; each may be NULL (not wanted).  v_weights and v_biases are summed
+ * in a fixed order; v_x is too, except that with row_ids the rows of one id
+ * are added atomically in fp32. */
+int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
+                          const int32_t* row_ids, const int32_t* offsets,
+                          const void* weights, const void* y, const void* v_y,
+                          void* v_x, void* v_weights, void* v_biases,
+                          void* workspace, size_t workspace_bytes,
+                          gs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
