@@ -10,6 +10,8 @@ from __future__ import annotations
 import ctypes as ct
 import os
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GSPLAT_B200_LIB", os.path.join(_HERE, "libgsplat_b200.so"))
 
@@ -179,6 +181,16 @@ def load(path: str = LIB_PATH) -> ct.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def on_device_of(t, call):
+    """call(stream) with t's device as the current one and the raw handle of
+    its current torch stream."""
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        return call(torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(torch._C._cuda_getCurrentRawStream(index))
 
 
 class GsplatError(RuntimeError):

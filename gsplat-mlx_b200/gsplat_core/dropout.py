@@ -19,7 +19,7 @@ import ctypes as ct
 import torch
 
 from . import _lib
-from ._lib import DropoutParams, check
+from ._lib import DropoutParams, check, on_device_of
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _U64 = (1 << 64) - 1
@@ -58,10 +58,10 @@ def dropout_forward(x, p, seed, step=0, rows=False, out=None):
     y = torch.empty_like(x) if out is None else out
     prm = DropoutParams(n, width, int(seed) & _U64, int(step) & _U64, p, _DTYPES[x.dtype],
                         int(bool(rows)))
-    with torch.cuda.device(x.device):
-        check(_lib.load().gs_dropout(
-            ct.byref(prm), x.data_ptr(), None if step_dev is None else step_dev.data_ptr(),
-            y.data_ptr(), torch.cuda.current_stream().cuda_stream), "dropout")
+    lib = _lib.load()
+    check(on_device_of(x, lambda stream: lib.gs_dropout(
+        ct.byref(prm), x.data_ptr(), None if step_dev is None else step_dev.data_ptr(),
+        y.data_ptr(), stream)), "dropout")
     return y
 
 

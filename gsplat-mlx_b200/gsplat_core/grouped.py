@@ -21,7 +21,7 @@ import ctypes as ct
 import torch
 
 from . import _lib
-from ._lib import GroupedParams, check
+from ._lib import GroupedParams, check, on_device_of
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2}
@@ -29,10 +29,6 @@ _ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2}
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
-
-
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
 
 
 def group_offsets(ids, groups):
@@ -47,9 +43,9 @@ def group_offsets(ids, groups):
         raise RuntimeError("group_offsets: ids must be a CUDA tensor (there is no CPU fallback).")
     ids = ids.contiguous()
     off = torch.empty((int(groups) + 1,), dtype=torch.int32, device=ids.device)
-    with torch.cuda.device(ids.device):
-        check(_lib.load().gs_group_offsets(ids.numel(), _ptr(ids), int(groups), _ptr(off),
-                                           _stream()), "group_offsets")
+    lib = _lib.load()
+    check(on_device_of(ids, lambda stream: lib.gs_group_offsets(
+        ids.numel(), _ptr(ids), int(groups), _ptr(off), stream)), "group_offsets")
     return off
 
 
@@ -107,10 +103,10 @@ def grouped_linear_forward(inputs, activation="none"):
     p, (x, w, off, b, ids) = _validated(inputs, activation)
     _on_cuda(x)
     y = torch.empty((p.rows, p.out_features), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        check(_lib.load().gs_grouped_linear_fwd(ct.byref(p), _ptr(x), _ptr(ids), _ptr(off),
-                                                _ptr(w), _ptr(b), _ptr(y), _stream()),
-              "grouped_linear_forward")
+    lib = _lib.load()
+    check(on_device_of(x, lambda stream: lib.gs_grouped_linear_fwd(
+        ct.byref(p), _ptr(x), _ptr(ids), _ptr(off), _ptr(w), _ptr(b), _ptr(y), stream)),
+        "grouped_linear_forward")
     return y
 
 
@@ -143,11 +139,14 @@ def grouped_linear_backward(inputs, y, v_y, activation="none",
     if "v_biases" in wanted and b is not None:
         out["v_biases"] = torch.empty_like(b)
     lib = _lib.load()
-    with torch.cuda.device(x.device):
+
+    def call(stream):
         need = lib.gs_grouped_linear_bwd_workspace_size(ct.byref(p))
         ws = torch.empty((need,), dtype=torch.uint8, device=x.device)
-        check(lib.gs_grouped_linear_bwd(
+        return lib.gs_grouped_linear_bwd(
             ct.byref(p), _ptr(x), _ptr(ids), _ptr(off), _ptr(w), _ptr(y), _ptr(v_y),
             _ptr(out.get("v_x")), _ptr(out.get("v_weights")), _ptr(out.get("v_biases")),
-            _ptr(ws), need, _stream()), "grouped_linear_backward")
+            _ptr(ws), need, stream)
+
+    check(on_device_of(x, call), "grouped_linear_backward")
     return out
