@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace gsb {
 namespace {
@@ -57,54 +58,730 @@ __device__ __forceinline__ float through(float v, float y) {
   return v;
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) fwd_kernel(Shape s, const T* __restrict__ x,
-                                                  const int32_t* __restrict__ ids,
-                                                  const int32_t* __restrict__ off,
-                                                  const T* __restrict__ w,
-                                                  const T* __restrict__ b, T* __restrict__ y) {
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < s.R * s.M;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / s.M;
-    const int m = (int)(i - r * s.M);
-    const int g = group_of(off, s.G, r);
-    if (g < 0 || g >= s.G) {
-      y[i] = from_f<T>(0.0f);
-      continue;
-    }
-    const int64_t at = ids ? ids[r] : r;
-    float acc = 0.0f;
-    if (at >= 0 && at < s.n)
-      for (int k = 0; k < s.K; ++k)
-        acc = fmaf(to_f(x[at * s.K + k]), to_f(w[((int64_t)g * s.M + m) * s.K + k]), acc);
-    if (b) acc += to_f(b[(int64_t)g * s.M + m]);
-    y[i] = from_f<T>(activate<ACT>(acc));
-  }
+// ------------------------------------------------------------ tensor-core tiles
+//
+// Operands in 16 bits go to the tensor core as they are.  An fp32 value goes
+// as two tf32 parts, x = hi + lo; the products hi hi are summed in one
+// accumulator and hi lo + lo hi in a second (the neglected lo lo is 2^-22 of
+// the product), which are added in fp32 when the sum is read: about the
+// accuracy of fp32 multiply-adds.  Where the first is not finite it is the
+// result: the second cannot be trusted with infinities (inf * 0).  v_z of the
+// sigmoid in 16 bits goes as two parts in the same manner, so that it is not
+// rounded to 16 bits on its way.
+__device__ unsigned int g_wait_gave_up;
+constexpr uint32_t kWaitLimit = 1u << 16;  // polls of the hardware's own bounded wait
+
+template <typename T> struct Mma;
+template <> struct Mma<float> {
+  static constexpr bool TF32 = true;
+  static constexpr uint32_t format = tc::kTF32;
+};
+template <> struct Mma<__nv_bfloat16> {
+  static constexpr bool TF32 = false;
+  static constexpr uint32_t format = tc::kBF16;
+};
+template <> struct Mma<__half> {
+  static constexpr bool TF32 = false;
+  static constexpr uint32_t format = tc::kF16;
+};
+
+constexpr int kThreads = 256;
+constexpr int kTile = 128;               // rows of a tile: the lanes of an accumulator
+constexpr int kPanel = kTile * 128;      // bytes of 128 operand rows, 128 bytes deep
+
+// The values of one 16-byte chunk.
+template <typename T>
+union Chunk {
+  static constexpr int E = 16 / sizeof(T);
+  uint4 q;
+  T v[E];
+  __device__ Chunk() {}
+};
+
+// Where chunk c of operand row r lies in its panel.
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
 }
 
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) bwd_x_kernel(Shape s, const int32_t* __restrict__ ids,
-                                                    const int32_t* __restrict__ off,
-                                                    const T* __restrict__ w,
-                                                    const T* __restrict__ y,
-                                                    const T* __restrict__ vy,
-                                                    float* __restrict__ sum, T* __restrict__ vx) {
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < s.R * s.K;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / s.K;
-    const int k = (int)(i - r * s.K);
-    const int g = group_of(off, s.G, r);
-    float acc = 0.0f;
-    if (g >= 0 && g < s.G)
-      for (int m = 0; m < s.M; ++m) {
-        const float v = through<ACT>(to_f(vy[r * s.M + m]), ACT ? to_f(y[r * s.M + m]) : 0.0f);
-        acc = fmaf(v, to_f(w[((int64_t)g * s.M + m) * s.K + k]), acc);
+// Writes f[0..E) as one operand chunk: one part, or two at a panel's distance.
+template <typename T, bool SPLIT>
+__device__ __forceinline__ void put_chunk(char* at, uint32_t lo_offset, const float* f) {
+  Chunk<T> hi, lo;
+#pragma unroll
+  for (int e = 0; e < Chunk<T>::E; ++e) {
+    if (sizeof(T) == 4) {
+      float a, b;
+      tc::split_tf32(f[e], a, b);
+      hi.v[e] = from_f<T>(a);
+      lo.v[e] = from_f<T>(b);
+    } else {
+      hi.v[e] = from_f<T>(f[e]);
+      if (SPLIT) {
+        const float back = to_f(hi.v[e]);
+        lo.v[e] = from_f<T>(fabsf(back) < INFINITY ? f[e] - back : 0.0f);
       }
-    if (!ids) {
-      vx[i] = from_f<T>(acc);
-    } else if (g >= 0 && g < s.G) {
-      const int64_t at = ids[r];
-      if (at >= 0 && at < s.n) atomicAdd(sum + at * s.K + k, acc);
+    }
+  }
+  *reinterpret_cast<uint4*>(at) = hi.q;
+  if (SPLIT || sizeof(T) == 4) *reinterpret_cast<uint4*>(at + lo_offset) = lo.q;
+}
+
+// E values from p: one access, or one by one where p is not aligned or fewer
+// than E are there.  What is not there is zero.
+template <typename T, bool WIDE>
+__device__ __forceinline__ uint4 get_chunk(const T* __restrict__ p, int there) {
+  Chunk<T> c;
+  if (WIDE) {
+    c.q = there > 0 ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < Chunk<T>::E; ++e) c.v[e] = e < there ? p[e] : from_f<T>(0.0f);
+  }
+  return c.q;
+}
+
+// Consecutive rows of one group, at most `most` of them, up to `end`.
+struct Run {
+  int64_t row;
+  int n;      // 0: no rows are left
+  int g;      // -1 or G: outside every group
+  int64_t group_end;
+};
+
+__device__ __forceinline__ Run run_from(const int32_t* __restrict__ off, int G, int64_t row,
+                                        int64_t end, int most, Run prev) {
+  Run t;
+  t.row = row;
+  t.g = prev.g;
+  t.group_end = prev.group_end;
+  if (row >= end) {
+    t.n = 0;
+    return t;
+  }
+  if (row >= t.group_end) {
+    t.g = group_of(off, G, row);
+    const int64_t stop = t.g < 0 ? __ldg(off) : t.g < G ? __ldg(off + t.g + 1) : end;
+    t.group_end = min(stop, end);
+  }
+  t.n = (int)min((int64_t)most, t.group_end - row);
+  return t;
+}
+
+// The tiles of kTile rows are dealt to `parts` CTAs in order: CTA b has the
+// tiles [T b / parts, T (b + 1) / parts).
+__host__ __device__ __forceinline__ int64_t first_tile(int64_t tiles, int parts, int b) {
+  return tiles * b / parts;
+}
+
+struct RowsArgs {
+  Shape s;                 // R, n, G and K, M as the caller gave them
+  const void* a;           // rows that are multiplied: x, or v_y
+  const void* y;           // backward through an activation
+  const int32_t* ids;
+  const int32_t* off;
+  const void* w;
+  const void* bias;
+  void* out;
+  int depth, width;        // K, M; the backward's M, K
+  int nt;                  // columns of a CTA's tile: a multiple of 32
+  int panels;              // of `depth`
+  int resident;            // all weight panels of the tile stay in shared memory
+  int wide_w, wide_out;    // 16-byte accesses are aligned
+};
+
+enum { kForward, kBackward, kScatter };
+
+template <typename T, bool SPLIT>
+struct RowsLayout {
+  static constexpr int kTerms = SPLIT || sizeof(T) == 4 ? 2 : 1;  // parts of a row value
+  static constexpr int kWTerms = sizeof(T) == 4 ? 2 : 1;          // of a weight
+  // also the warps' staging of results: 8 x 32 rows x 32 columns
+  static constexpr int kA = kTerms * kPanel > 32768 ? kTerms * kPanel : 32768;
+  static int weight_panels(const RowsArgs& p) { return p.resident ? p.panels : 1; }
+  static int smem(const RowsArgs& p) {
+    return 1024 + kA + weight_panels(p) * kWTerms * p.nt * 128;
+  }
+  static int columns(int nt) {
+    int c = 32;
+    while (c < nt * kTerms) c *= 2;
+    return c;
+  }
+};
+
+// out[row] = f(rows a, weights of the row's group): the forward, and v_x.
+//
+// A CTA streams its consecutive 128-row tiles; the rows' 16-byte chunks go
+// through registers (16 KB a CTA in flight, the next panel's while this one
+// is multiplied and stored) into swizzled panels, which lets the gather, the
+// activation's reverse mode, the split into parts and the zeros behind K
+// happen on the way; one thread issues the MMAs.  The group's weights are
+// staged once per group, and stay.
+template <typename T, int ACT, int MODE, bool WIDE, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 2) rows_mma_kernel(RowsArgs p, int columns) {
+  using L = RowsLayout<T, SPLIT>;
+  constexpr int E = Chunk<T>::E;
+  constexpr int DP = 128 / sizeof(T);   // depth of a panel
+  constexpr int STEP = 32 / sizeof(T);  // depth of an MMA
+  constexpr bool BACK = MODE != kForward;
+  extern __shared__ char smem_raw[];
+  __shared__ uint64_t s_bar;
+  __shared__ uint32_t s_tmem;
+  __shared__ int32_t s_ids[4][kTile];
+  __shared__ float s_bias[kTile];
+  char* const s_a = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
+  char* const s_w = s_a + L::kA;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int n0 = blockIdx.y * p.nt;
+  const int cols = min(p.nt, p.width - n0);
+  const int wbytes = p.nt * 128;  // of a weight panel's part
+  const T* const a = static_cast<const T*>(p.a);
+  const T* const y = static_cast<const T*>(p.y);
+  const T* const w = static_cast<const T*>(p.w);
+  const T* const bias = static_cast<const T*>(p.bias);
+
+  if (warp == 0) tc::alloc(&s_tmem, columns);
+  if (tid == 0) tc::bar_init(tc::smem_addr(&s_bar), 1);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = s_tmem, bar = tc::smem_addr(&s_bar);
+  const uint32_t idesc = tc::instr_desc(Mma<T>::format, (cols + 15) / 16 * 16);
+  uint32_t phase = 0, limit = kWaitLimit;
+  auto wait_mma = [&]() {
+    if (!tc::bar_wait(bar, phase, limit)) {
+      limit = 0;  // results are void: no later wait holds the kernel up
+      g_wait_gave_up = 1;
+    }
+    phase ^= 1;
+    tc::fence_after_sync();
+  };
+
+  const int64_t tiles = (p.s.R + kTile - 1) / kTile;
+  const int64_t end = min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
+  Run none;
+  none.row = 0, none.n = 0, none.g = -1, none.group_end = 0;
+  Run cur = run_from(p.off, p.s.G, first_tile(tiles, gridDim.x, blockIdx.x) * kTile, end, kTile, none);
+  Run nxt = run_from(p.off, p.s.G, cur.row + cur.n, end, kTile, cur);
+
+  auto id_of = [&](const Run& t, int i) {
+    return p.ids && i < t.n ? __ldg(p.ids + t.row + i) : -1;
+  };
+  uint4 ra[4], ry[BACK && ACT ? 4 : 1];
+  // this thread's four chunks of panel j of tile t (number k of this CTA's)
+  auto load_panel = [&](const Run& t, int k, int j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (tid >> 3) + 32 * i, d = j * DP + (tid & 7) * E;
+      int64_t at = t.row + row;
+      bool ok = row < t.n && t.g >= 0 && t.g < p.s.G;
+      if (!BACK && p.ids) {
+        at = s_ids[k & 3][row];
+        ok = ok && at >= 0 && at < p.s.n;
+      }
+      const int there = ok ? p.depth - d : 0;
+      const int64_t from = ok ? at * p.depth + d : 0;
+      ra[i] = get_chunk<T, WIDE>(a + from, there);
+      if (BACK && ACT) ry[BACK && ACT ? i : 0] = get_chunk<T, WIDE>(y + from, there);
+    }
+  };
+  // weight panels [j0, j1) of group g: rows n (columns of the result) x depth
+  auto stage_weights = [&](int g, int j0, int j1) {
+    const T* const wg = w + (int64_t)g * p.s.M * p.s.K;
+    const int units = (j1 - j0) * 8 * cols;
+    for (int u = tid; u < units; u += kThreads) {
+      int n, c, j;
+      Chunk<T> q;
+      if (!BACK) {  // chunks of a weight row
+        c = u & 7, n = (u >> 3) % cols, j = (u >> 3) / cols;
+        const int d = (j0 + j) * DP + c * E;
+        const T* const from = wg + (int64_t)(n0 + n) * p.depth + d;
+        if (p.wide_w)
+          q.q = get_chunk<T, true>(d < p.depth ? from : wg, p.depth - d);
+        else
+          q.q = get_chunk<T, false>(from, p.depth - d);
+      } else {      // down a weight column; neighbours are neighbouring threads'
+        n = u % cols, c = (u / cols) & 7, j = u / cols / 8;
+        const int d = (j0 + j) * DP + c * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          q.v[e] = d + e < p.depth ? wg[(int64_t)(d + e) * p.width + n0 + n] : from_f<T>(0.0f);
+      }
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = to_f(q.v[e]);
+      put_chunk<T, false>(s_w + j * L::kWTerms * wbytes + chunk_at(n, c), wbytes, f);
+    }
+  };
+
+  if (tid < kTile) s_ids[0][tid] = id_of(cur, tid);
+  int next_id = tid < kTile ? id_of(nxt, tid) : -1;
+  __syncthreads();
+  load_panel(cur, 0, 0);
+  int staged = -2;
+
+  for (int k = 0; cur.n > 0; ++k) {
+    const bool live = cur.g >= 0 && cur.g < p.s.G;
+    if (live && cur.g != staged) {  // every MMA of the group before is done
+      if (p.resident) stage_weights(cur.g, 0, p.panels);
+      if (tid < kTile)
+        s_bias[tid] = !BACK && bias && tid < cols ? to_f(bias[(int64_t)cur.g * p.s.M + n0 + tid]) : 0.0f;
+      staged = cur.g;
+    }
+    Run after = nxt;
+    for (int j = 0; j < p.panels; ++j) {
+      if (live) {
+        if (j > 0) wait_mma();  // the panel's memory is free again
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          char* const to = s_a + chunk_at((tid >> 3) + 32 * i, tid & 7);
+          Chunk<T> q;
+          q.q = ra[i];
+          if (sizeof(T) == 2 && !SPLIT && !(BACK && ACT)) {
+            *reinterpret_cast<uint4*>(to) = q.q;
+            continue;
+          }
+          float f[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[e] = to_f(q.v[e]);
+          if (BACK && ACT) {
+            Chunk<T> o;
+            o.q = ry[BACK && ACT ? i : 0];
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[e] = through<ACT>(f[e], to_f(o.v[e]));
+          }
+          put_chunk<T, SPLIT>(to, kPanel, f);
+        }
+        if (!p.resident) stage_weights(cur.g, j, j + 1);
+      }
+      if (j == 0 && tid < kTile) s_ids[(k + 1) & 3][tid] = next_id;
+      tc::fence_smem();
+      tc::fence_before_sync();
+      __syncthreads();
+      if (live && tid == 0) {
+        tc::fence_after_sync();
+        const int steps = (min(DP, p.depth - j * DP) + STEP - 1) / STEP;
+        const uint64_t da = tc::smem_desc(tc::smem_addr(s_a));
+        const uint64_t dw = tc::smem_desc(tc::smem_addr(s_w + (p.resident ? j : 0) * L::kWTerms * wbytes));
+        const uint64_t lo_a = kPanel >> 4, lo_w = wbytes >> 4;
+        for (int i = 0; i < steps; ++i) {
+          const uint64_t at = 2 * i;  // 32 bytes
+          const bool more = j > 0 || i > 0;
+          if (L::kTerms == 2) {
+            tc::mma<Mma<T>::TF32>(tmem + p.nt, da + lo_a + at, dw + at, idesc, more);
+            if (L::kWTerms == 2)
+              tc::mma<Mma<T>::TF32>(tmem + p.nt, da + at, dw + lo_w + at, idesc, true);
+          }
+          tc::mma<Mma<T>::TF32>(tmem, da + at, dw + at, idesc, more);
+        }
+        tc::commit(bar);
+      }
+      // the next panel's rows are on their way while this one is multiplied
+      if (j + 1 < p.panels) {
+        load_panel(cur, k, j + 1);
+      } else if (nxt.n > 0) {
+        load_panel(nxt, k + 1, 0);
+        after = run_from(p.off, p.s.G, nxt.row + nxt.n, end, kTile, nxt);
+        if (tid < kTile) next_id = id_of(after, tid);
+      } else {
+        after.n = 0;
+      }
+    }
+    if (live) wait_mma();
+
+    // 32 rows x 32 columns at a time: out of the accumulator, through the
+    // warp's own part of the operand memory, and in whole rows to `out`
+    constexpr int OB = MODE == kScatter ? 4 : sizeof(T);  // bytes of a result
+    constexpr int OE = 16 / OB;
+    constexpr int CH = 32 / OE;                           // chunks of 32 columns
+    char* const stage = s_a + warp * (32 * 32 * OB);
+    auto stage_at = [&](int r, int c) {
+      return stage + r * (32 * OB) + ((c ^ (CH == 8 ? r & 7 : (r >> 1) & 3)) << 4);
+    };
+    const int row0 = (warp & 3) * 32;
+    const int rows = min(32, cur.n - row0);
+    for (int c0 = (warp >> 2) * 32; c0 < cols; c0 += 64) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[16];
+        if (live) {
+          const uint32_t from = tmem + ((uint32_t)row0 << 16) + c0 + h * 16;
+          tc::load16(from, v);
+          if (L::kTerms == 2) {
+            float u[16];
+            tc::load16(from + p.nt, u);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (!live) v[i] = 0.0f;
+          else if (!BACK) v[i] = activate<ACT>(v[i] + s_bias[c0 + h * 16 + i]);
+        }
+#pragma unroll
+        for (int c = 0; c < CH / 2; ++c) {
+          char* const to = stage_at(lane, h * (CH / 2) + c);
+          if constexpr (OB == 4) {
+            *reinterpret_cast<float4*>(to) =
+                make_float4(v[c * OE], v[c * OE + 1], v[c * OE + 2], v[c * OE + 3]);
+          } else {
+            Chunk<T> q;
+#pragma unroll
+            for (int e = 0; e < OE; ++e) q.v[e] = from_f<T>(v[c * OE + e]);
+            *reinterpret_cast<uint4*>(to) = q.q;
+          }
+        }
+      }
+      __syncwarp();
+      const int width = min(32, cols - c0);  // columns here
+      if (MODE == kScatter) {
+        float* const sum = static_cast<float*>(p.out);
+        if (live) {
+          const int c = lane & 7;
+          for (int r = lane >> 3; r < rows; r += 4) {
+            const int32_t at = s_ids[k & 3][row0 + r];
+            if (at < 0 || at >= p.s.n || c * 4 >= width) continue;
+            float* const to = sum + (int64_t)at * p.width + n0 + c0 + c * 4;
+            const float4 q = *reinterpret_cast<const float4*>(stage_at(r, c));
+            if (p.wide_out) {
+              asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
+                           ::"l"(to), "f"(q.x), "f"(q.y), "f"(q.z), "f"(q.w) : "memory");
+            } else {
+              atomicAdd(to, q.x);
+              if (c * 4 + 1 < width) atomicAdd(to + 1, q.y);
+              if (c * 4 + 2 < width) atomicAdd(to + 2, q.z);
+              if (c * 4 + 3 < width) atomicAdd(to + 3, q.w);
+            }
+          }
+        }
+      } else {
+        T* const out = static_cast<T*>(p.out) + (cur.row + row0) * p.width + n0 + c0;
+        if (p.wide_out) {
+          const int c = lane & (CH - 1);
+          if (c * OE < width)
+            for (int r = lane / CH; r < rows; r += 32 / CH)
+              *reinterpret_cast<uint4*>(out + (int64_t)r * p.width + c * OE) =
+                  *reinterpret_cast<const uint4*>(stage_at(r, c));
+        } else if (p.width <= 32) {  // whole rows: one run of memory
+          const int total = rows * width;
+          for (int i = lane; i < total; i += 32) {
+            const int r = i / width, c = i - r * width;
+            out[i] = reinterpret_cast<const T*>(stage_at(r, c / OE))[c % OE];
+          }
+        } else if (lane < width) {
+          for (int r = 0; r < rows; ++r)
+            out[(int64_t)r * p.width + lane] =
+                reinterpret_cast<const T*>(stage_at(r, lane / OE))[lane % OE];
+        }
+      }
+      __syncwarp();
+    }
+    tc::fence_before_sync();
+    __syncthreads();  // the operand memory and the accumulators are free
+    cur = nxt;
+    nxt = after;
+  }
+  if (warp == 0) tc::dealloc(tmem, columns);
+}
+
+// ---------------------------------------------------------- v_weights, v_biases
+struct WeightArgs {
+  Shape s;
+  const void* x;
+  const void* y;
+  const void* vy;
+  const int32_t* ids;
+  const int32_t* off;
+  float* part;       // [parts + G][M * K + M]
+  int kt, mt;        // tiles of K (128) and M (NT)
+  int wide_x, wide_y;
+  int biases;
+};
+
+// v_W[g] (as K lanes x M columns) = sum over g's rows of x[r]^T v_z[r].
+//
+// The rows are the depth here, so both operands are staged transposed: a
+// thread takes a few rows' chunks of the same columns (4 x 4 fp32, 8 x 8 in
+// 16 bits) and writes their columns as chunks.  A CTA sums the rows of its
+// consecutive tiles; what it has at the end of a group goes to its own place
+// in `part` (CTA b and group g: place b + g; both only ever grow), and the
+// places of a group are added in order by another kernel, so the sums have a
+// fixed order.  In fp32 the accumulators are moved to registers every
+// kFlush panels: the tensor core cuts a sum to fp32 rather than rounding it,
+// which a few thousand additions would make visible.
+constexpr int kFlush = 8;
+
+template <typename T, int ACT, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
+    weights_mma_kernel(WeightArgs p, int columns) {
+  constexpr int E = Chunk<T>::E;
+  constexpr int DP = 128 / sizeof(T);
+  constexpr int STEP = 32 / sizeof(T);
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int XTERMS = F32 ? 2 : 1, VTERMS = F32 || SPLIT ? 2 : 1;
+  constexpr int VPANEL = NT * 128;
+  extern __shared__ char smem_raw[];
+  __shared__ uint64_t s_bar;
+  __shared__ uint32_t s_tmem;
+  __shared__ int32_t s_ids[4][DP];
+  char* const s_x = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
+  char* const s_v = s_x + XTERMS * kPanel;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int k0 = (blockIdx.y % p.kt) * 128, m0 = (blockIdx.y / p.kt) * NT;
+  const int kn = min(128, p.s.K - k0), mn = min(NT, p.s.M - m0);
+  const T* const x = static_cast<const T*>(p.x);
+  const T* const y = static_cast<const T*>(p.y);
+  const T* const vy = static_cast<const T*>(p.vy);
+
+  if (warp == 0) tc::alloc(&s_tmem, columns);
+  if (tid == 0) tc::bar_init(tc::smem_addr(&s_bar), 1);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = s_tmem, bar = tc::smem_addr(&s_bar);
+  const uint32_t idesc = tc::instr_desc(Mma<T>::format, (mn + 15) / 16 * 16);
+  uint32_t phase = 0, limit = kWaitLimit;
+  auto wait_mma = [&]() {
+    if (!tc::bar_wait(bar, phase, limit)) {
+      limit = 0;
+      g_wait_gave_up = 1;
+    }
+    phase ^= 1;
+    tc::fence_after_sync();
+  };
+
+  // This thread's blocks of E rows x E columns: eight neighbouring threads
+  // have the panel's eight row blocks of the same columns, so that their
+  // writes of a column go to eight different chunks of one operand row.
+  const int x_units = 8 * ((kn + E - 1) / E), v_units = 8 * ((mn + E - 1) / E);
+  const int vu = (tid + kThreads - x_units % kThreads) % kThreads;
+  const bool has_x = tid < x_units, has_v = vu < v_units;
+  const int rb = (tid & 7) * E;                 // first row of either block
+  const int xc = (tid >> 3) * E, vc = (vu >> 3) * E;
+  // in 16 bits a thread has a block of x or one of v_y: they share registers
+  uint4 rx[E], rv_own[F32 ? E : 1], ry[ACT ? E : 1];
+  auto rv = [&](int i) -> uint4& {
+    if constexpr (F32) return rv_own[i];
+    else return rx[i];
+  };
+  float bsum[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) bsum[e] = 0.0f;
+
+  const int64_t tiles = (p.s.R + kTile - 1) / kTile;
+  const int64_t end = min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
+  auto next_run = [&](Run t) {  // skips rows outside every group
+    Run n = run_from(p.off, p.s.G, t.row + t.n, end, DP, t);
+    while (n.n > 0 && (n.g < 0 || n.g >= p.s.G))
+      n = run_from(p.off, p.s.G, n.group_end, end, DP, n);
+    return n;
+  };
+  Run none;
+  none.row = first_tile(tiles, gridDim.x, blockIdx.x) * kTile, none.n = 0, none.g = -1;
+  none.group_end = 0;
+  Run cur = next_run(none);
+  Run nxt = next_run(cur);
+  auto id_of = [&](const Run& t, int i) {
+    return p.ids && i < t.n ? __ldg(p.ids + t.row + i) : -1;
+  };
+  auto load_run = [&](const Run& t, int k) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const bool in = rb + i < t.n;
+      if (has_x) {
+        int64_t at = t.row + rb + i;
+        bool ok = in;
+        if (p.ids) {
+          at = s_ids[k & 3][rb + i];
+          ok = at >= 0 && at < p.s.n;
+        }
+        const T* const from = x + (ok ? at * p.s.K + k0 + xc : 0);
+        const int there = ok ? kn - xc : 0;
+        rx[i] = p.wide_x ? get_chunk<T, true>(from, there) : get_chunk<T, false>(from, there);
+      }
+      if (has_v) {
+        const int64_t from = in ? (t.row + rb + i) * p.s.M + m0 + vc : 0;
+        const int there = in ? mn - vc : 0;
+        rv(i) = p.wide_y ? get_chunk<T, true>(vy + from, there) : get_chunk<T, false>(vy + from, there);
+        if (ACT)
+          ry[ACT ? i : 0] = p.wide_y ? get_chunk<T, true>(y + from, there)
+                                     : get_chunk<T, false>(y + from, there);
+      }
+    }
+  };
+
+  constexpr int HALF = NT / 2;  // columns of a warp's half of the accumulators
+  float acc[F32 ? HALF : 1];
+  bool held = false;            // acc has a part of the sum
+  // adds the accumulators to acc (fp32 only)
+  auto flush = [&]() {
+    if constexpr (F32) {
+#pragma unroll
+      for (int c = 0; c < HALF; c += 16) {
+        float v[16], u[16];
+        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * HALF + c;
+        tc::load16(from, v);
+        tc::load16(from + NT, u);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+          acc[c + i] = held ? acc[c + i] + v[i] : v[i];
+        }
+      }
+      held = true;
+    }
+  };
+
+  if (tid < DP) s_ids[0][tid] = id_of(cur, tid);
+  int next_id = tid < DP ? id_of(nxt, tid) : -1;
+  __syncthreads();
+  if (cur.n > 0) load_run(cur, 0);
+  int pending = 0;              // panels in the accumulators
+
+  for (int k = 0; cur.n > 0; ++k) {
+    if (pending > 0) wait_mma();  // the panels' memory is free again
+    if (F32 && pending == kFlush) {
+      flush();
+      pending = 0;
+    }
+    if (has_x) {
+#pragma unroll
+      for (int c = 0; c < E; ++c) {
+        float f[E];
+        Chunk<T> raw;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          Chunk<T> q;
+          q.q = rx[i];
+          f[i] = to_f(q.v[c]);
+          raw.v[i] = q.v[c];
+        }
+        char* const to = s_x + chunk_at(xc + c, tid & 7);
+        if (F32) put_chunk<T, false>(to, kPanel, f);
+        else *reinterpret_cast<uint4*>(to) = raw.q;
+      }
+    }
+    if (has_v) {
+#pragma unroll
+      for (int c = 0; c < E; ++c) {
+        float f[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          Chunk<T> q, o;
+          q.q = rv(i);
+          if (ACT) o.q = ry[ACT ? i : 0];
+          f[i] = through<ACT>(to_f(q.v[c]), ACT ? to_f(o.v[c]) : 0.0f);
+          bsum[c] += f[i];
+        }
+        put_chunk<T, SPLIT>(s_v + chunk_at(vc + c, tid & 7), VPANEL, f);
+      }
+    }
+    if (tid < DP) s_ids[(k + 1) & 3][tid] = next_id;
+    tc::fence_smem();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (tid == 0) {
+      tc::fence_after_sync();
+      const uint64_t dx = tc::smem_desc(tc::smem_addr(s_x)), dv = tc::smem_desc(tc::smem_addr(s_v));
+      const int steps = (cur.n + STEP - 1) / STEP;
+      for (int i = 0; i < steps; ++i) {
+        const uint64_t at = 2 * i;
+        const bool more = pending > 0 || i > 0;
+        if (VTERMS == 2) {
+          tc::mma<Mma<T>::TF32>(tmem + NT, dx + at, dv + (VPANEL >> 4) + at, idesc, more);
+          if (XTERMS == 2)
+            tc::mma<Mma<T>::TF32>(tmem + NT, dx + (kPanel >> 4) + at, dv + at, idesc, true);
+        }
+        tc::mma<Mma<T>::TF32>(tmem, dx + at, dv + at, idesc, more);
+      }
+      tc::commit(bar);
+    }
+    ++pending;
+    Run after = nxt;
+    if (nxt.n > 0) {
+      load_run(nxt, k + 1);
+      after = next_run(nxt);
+      if (tid < DP) next_id = id_of(after, tid);
+    }
+    if (nxt.n == 0 || nxt.g != cur.g) {  // the group ends here: its sums to their place
+      wait_mma();
+      float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)p.s.M * (p.s.K + 1));
+      const int kk = (warp & 3) * 32 + lane;
+      if (F32) flush();
+#pragma unroll
+      for (int c = 0; c < HALF; c += 16) {
+        float v[16];
+        if (!F32) {
+          const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * HALF + c;
+          tc::load16(from, v);
+          if (SPLIT) {
+            float u[16];
+            tc::load16(from + NT, u);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = (warp >> 2) * HALF + c + i;
+          if (kk < kn && m < mn)
+            to[(int64_t)(m0 + m) * p.s.K + k0 + kk] = F32 ? acc[F32 ? c + i : 0] : v[i];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float b = bsum[e];
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
+        if (has_v && p.biases && k0 == 0 && (tid & 7) == 0 && vc + e < mn)
+          to[(int64_t)p.s.M * p.s.K + m0 + vc + e] = b;
+        bsum[e] = 0.0f;
+      }
+      pending = 0;
+      held = false;
+      tc::fence_before_sync();
+      __syncthreads();
+    }
+    cur = nxt;
+    nxt = after;
+  }
+  if (warp == 0) tc::dealloc(tmem, columns);
+}
+
+// v_W and v_b of a group: the places of the CTAs that had rows of it, in
+// order.  Eight warps take an eighth of the places each, for 32 values.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(Shape s, int parts,
+                                                   const int32_t* __restrict__ off,
+                                                   const float* __restrict__ part,
+                                                   T* __restrict__ vw, T* __restrict__ vb) {
+  __shared__ float s_sum[8][32];
+  const int g = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t mk = (int64_t)s.M * s.K, each = mk + s.M;
+  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t r0 = max((int64_t)__ldg(off + g), (int64_t)0);
+  const int64_t r1 = min((int64_t)__ldg(off + g + 1), s.R);
+  float sum = 0.0f;
+  if (r0 < r1 && i < each) {
+    const int64_t tiles = (s.R + kTile - 1) / kTile;
+    auto part_of = [&](int64_t r) { return (int)(((r / kTile + 1) * parts - 1) / tiles); };
+    const int b0 = part_of(r0), n = part_of(r1 - 1) - b0 + 1;
+    const int from = n * warp / 8, to = n * (warp + 1) / 8;
+    const float* p = part + (int64_t)(b0 + g + from) * each + i;
+#pragma unroll 8
+    for (int b = from; b < to; ++b, p += each) sum += __ldg(p);
+  }
+  s_sum[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && i < each) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) sum += s_sum[w][lane];
+    if (i < mk) {
+      if (vw) vw[g * mk + i] = from_f<T>(sum);
+    } else if (vb) {
+      vb[(int64_t)g * s.M + (i - mk)] = from_f<T>(sum);
     }
   }
 }
@@ -115,38 +792,6 @@ __global__ void __launch_bounds__(256) round_kernel(int64_t n, const float* __re
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n;
        i += (int64_t)gridDim.x * blockDim.x)
     b[i] = from_f<T>(a[i]);
-}
-
-template <typename T, int ACT>
-__global__ void __launch_bounds__(256) bwd_w_kernel(Shape s, const T* __restrict__ x,
-                                                    const int32_t* __restrict__ ids,
-                                                    const int32_t* __restrict__ off,
-                                                    const T* __restrict__ y,
-                                                    const T* __restrict__ vy, T* __restrict__ vw,
-                                                    T* __restrict__ vb) {
-  const int64_t each = (int64_t)s.M * (s.K + 1);
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < s.G * each;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int g = (int)(i / each);
-    const int m = (int)((i - g * each) / (s.K + 1));
-    const int k = (int)((i - g * each) % (s.K + 1));
-    const int64_t r0 = max((int64_t)off[g], (int64_t)0), r1 = min((int64_t)off[g + 1], s.R);
-    float acc = 0.0f;
-    for (int64_t r = r0; r < r1; ++r) {
-      const float v = through<ACT>(to_f(vy[r * s.M + m]), ACT ? to_f(y[r * s.M + m]) : 0.0f);
-      if (k == s.K) {
-        acc += v;
-        continue;
-      }
-      const int64_t at = ids ? ids[r] : r;
-      if (at >= 0 && at < s.n) acc = fmaf(v, to_f(x[at * s.K + k]), acc);
-    }
-    if (k < s.K) {
-      if (vw) vw[((int64_t)g * s.M + m) * s.K + k] = from_f<T>(acc);
-    } else if (vb) {
-      vb[(int64_t)g * s.M + m] = from_f<T>(acc);
-    }
-  }
 }
 
 __global__ void __launch_bounds__(256) offsets_kernel(int64_t n, const int32_t* __restrict__ ids,
@@ -161,35 +806,159 @@ __global__ void __launch_bounds__(256) offsets_kernel(int64_t n, const int32_t* 
   }
 }
 
-template <typename T, int ACT>
-int run_fwd(const Shape& s, const void* x, const int32_t* ids, const int32_t* off, const void* w,
-            const void* b, void* y, cudaStream_t st) {
-  fwd_kernel<T, ACT><<<grid_for(s.R * s.M, 256), 256, 0, st>>>(
-      s, static_cast<const T*>(x), ids, off, static_cast<const T*>(w), static_cast<const T*>(b),
-      static_cast<T*>(y));
-  return launch_status("grouped_linear_fwd");
+// ------------------------------------------------------------------- host side
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr int kSmemMost = 227 * 1024 - 4096;  // dynamic, beside the static arrays
+
+// Lets a kernel use kSmemMost bytes on the current device; asked once for
+// each kernel (the instantiation is the kernel's own) and device.
+template <auto kernel>
+int allow_smem() {
+  static bool done[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return launch_status("grouped_linear");
+  if (!done[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost) !=
+        cudaSuccess)
+      return launch_status("grouped_linear");
+    done[dev] = true;
+  }
+  return GS_OK;
+}
+
+// CTAs of 256 threads that an SM holds, by shared memory and accumulator
+// columns (a CTA that found none free would wait for another to end).
+int per_sm(int smem, int columns, int by_registers) {
+  int n = 227 * 1024 / (smem + 4096);
+  n = n < 512 / columns ? n : 512 / columns;
+  n = n < by_registers ? n : by_registers;
+  return n < 1 ? 1 : n;
+}
+
+template <typename T, int ACT, int MODE, bool WIDE, bool SPLIT>
+int launch_rows(RowsArgs p, cudaStream_t st) {
+  using L = RowsLayout<T, SPLIT>;
+  constexpr auto kernel = rows_mma_kernel<T, ACT, MODE, WIDE, SPLIT>;
+  if (int rc = allow_smem<kernel>()) return rc;
+  p.panels = (int)ceil_div(p.depth, 128 / (int)sizeof(T));
+  // The widest tile whose weights stay in shared memory: half the width
+  // reads the rows twice, which costs less than staging the weights again
+  // for every tile.
+  p.nt = p.width >= 128 ? 128 : (int)ceil_div(p.width, 32) * 32;
+  p.resident = 1;
+  while (L::smem(p) > kSmemMost && p.nt > 32) p.nt = (p.nt / 2 + 31) / 32 * 32;
+  if (L::smem(p) > kSmemMost) {
+    p.resident = 0;
+    p.nt = p.width >= 128 ? 128 : (int)ceil_div(p.width, 32) * 32;
+  }
+  const int smem = L::smem(p), columns = L::columns(p.nt);
+  const int64_t ny = ceil_div(p.width, p.nt);
+  if (ny > 65535) return invalid("grouped_linear: too many features");
+  const int64_t tiles = ceil_div(p.s.R, kTile);
+  int64_t nx = (int64_t)sm_count() * per_sm(smem, columns, 2) / ny;
+  nx = nx < 1 ? 1 : nx > tiles ? tiles : nx;
+  kernel<<<dim3((unsigned)nx, (unsigned)ny), kThreads, smem, st>>>(p, columns);
+  return launch_status("grouped_linear");
+}
+
+template <typename T, int ACT, int MODE, bool SPLIT>
+int launch_rows(const RowsArgs& p, cudaStream_t st) {
+  const bool wide = p.depth * sizeof(T) % 16 == 0 && on16(p.a) && (!p.y || on16(p.y));
+  return wide ? launch_rows<T, ACT, MODE, true, SPLIT>(p, st)
+              : launch_rows<T, ACT, MODE, false, SPLIT>(p, st);
 }
 
 template <typename T, int ACT>
-int run_bwd(const Shape& s, bool shared, const void* x, const int32_t* ids, const int32_t* off, const void* w,
-            const void* y, const void* vy, void* vx, void* vw, void* vb, void* ws,
-            cudaStream_t st) {
+int run_fwd(const Shape& s, const void* x, const int32_t* ids, const int32_t* off, const void* w,
+            const void* b, void* y, cudaStream_t st) {
+  RowsArgs p{};
+  p.s = s;
+  p.a = x, p.ids = ids, p.off = off, p.w = w, p.bias = b, p.out = y;
+  p.depth = s.K, p.width = s.M;
+  p.wide_w = s.K * sizeof(T) % 16 == 0 && on16(w);
+  p.wide_out = s.M * sizeof(T) % 16 == 0 && on16(y);
+  return launch_rows<T, ACT, kForward, false>(p, st);
+}
+
+// The backward's launches and its scratch: parts of the weight sums, then
+// the fp32 sums of shared rows for the 16-bit types.
+struct Plan {
+  int nt, kt, mt, parts;
+  size_t part_floats, sum_floats;
+};
+
+Plan plan_of(const gs_grouped_params* p) {
+  Plan q;
+  q.nt = p->out_features > 64 ? 128 : 64;
+  q.kt = (int)ceil_div(p->in_features, 128);
+  q.mt = (int)ceil_div(p->out_features, q.nt);
+  const int64_t tiles = ceil_div(p->rows, kTile);
+  int64_t n = (int64_t)sm_count() * (p->dtype == GS_F32 ? 1 : 2) / ((int64_t)q.kt * q.mt);
+  n = n < 1 ? 1 : n > tiles ? tiles : n;
+  q.parts = (int)n;
+  q.part_floats = ((size_t)q.parts + p->groups) * p->out_features * ((size_t)p->in_features + 1);
+  q.sum_floats = p->use_row_ids && p->dtype != GS_F32 ? (size_t)p->n * p->in_features : 0;
+  q.part_floats = (q.part_floats + 63) / 64 * 64;  // the sums start on 256 bytes
+  return q;
+}
+
+template <typename T, int ACT, int NT, bool SPLIT>
+int launch_weights(const WeightArgs& p, const Plan& q, cudaStream_t st) {
+  constexpr auto kernel = weights_mma_kernel<T, ACT, NT, SPLIT>;
+  if (int rc = allow_smem<kernel>()) return rc;
+  const int xt = sizeof(T) == 4 ? 2 : 1, vt = sizeof(T) == 4 || SPLIT ? 2 : 1;
+  const int smem = 1024 + xt * kPanel + vt * NT * 128, columns = NT * vt;
+  if ((int64_t)q.kt * q.mt > 65535) return invalid("grouped_linear: too many features");
+  kernel<<<dim3((unsigned)q.parts, (unsigned)(q.kt * q.mt)), kThreads, smem, st>>>(p, columns);
+  return launch_status("grouped_linear_bwd");
+}
+
+template <typename T, int ACT>
+int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const int32_t* ids,
+            const int32_t* off, const void* w, const void* y, const void* vy, void* vx, void* vw,
+            void* vb, float* ws, cudaStream_t st) {
+  constexpr bool kSplit = sizeof(T) == 2 && ACT == GS_ACT_SIGMOID;
+  const Plan q = plan_of(prm);
+  if (ACT == GS_ACT_NONE) y = nullptr;
   if (vx) {
-    float* sum = sizeof(T) == 4 ? static_cast<float*>(vx) : static_cast<float*>(ws);
+    const bool shared = prm->use_row_ids != 0;
+    float* sum = sizeof(T) == 4 ? static_cast<float*>(vx) : ws + q.part_floats;
     if (shared && cudaMemsetAsync(sum, 0, sizeof(float) * s.n * s.K, st) != cudaSuccess)
       return launch_status("grouped_linear_bwd");
-    if (s.R > 0)
-      bwd_x_kernel<T, ACT><<<grid_for(s.R * s.K, 256), 256, 0, st>>>(
-          s, ids, off, static_cast<const T*>(w), static_cast<const T*>(y),
-          static_cast<const T*>(vy), sum, static_cast<T*>(vx));
+    if (s.R > 0) {
+      RowsArgs p{};
+      p.s = s;
+      p.a = vy, p.y = y, p.ids = ids, p.off = off, p.w = w, p.out = shared ? sum : vx;
+      p.depth = s.M, p.width = s.K;
+      const size_t each = shared ? 4 : sizeof(T);
+      p.wide_out = s.K * each % 16 == 0 && on16(p.out);
+      const int rc = shared ? launch_rows<T, ACT, kScatter, kSplit>(p, st)
+                            : launch_rows<T, ACT, kBackward, kSplit>(p, st);
+      if (rc) return rc;
+    }
     if (shared && sizeof(T) == 2 && s.n > 0)
       round_kernel<T><<<grid_for(s.n * s.K, 256), 256, 0, st>>>(s.n * s.K, sum,
                                                                 static_cast<T*>(vx));
   }
-  if (vw || vb)
-    bwd_w_kernel<T, ACT><<<grid_for((int64_t)s.G * s.M * (s.K + 1), 256), 256, 0, st>>>(
-        s, static_cast<const T*>(x), ids, off, static_cast<const T*>(y),
-        static_cast<const T*>(vy), static_cast<T*>(vw), static_cast<T*>(vb));
+  if (vw || vb) {
+    if (s.R > 0) {
+      WeightArgs p{};
+      p.s = s;
+      p.x = x, p.y = y, p.vy = vy, p.ids = ids, p.off = off, p.part = ws;
+      p.kt = q.kt, p.mt = q.mt, p.biases = vb != nullptr;
+      p.wide_x = s.K * sizeof(T) % 16 == 0 && on16(x);
+      p.wide_y = s.M * sizeof(T) % 16 == 0 && on16(vy) && (!y || on16(y));
+      const int rc = q.nt == 64 ? launch_weights<T, ACT, 64, kSplit>(p, q, st)
+                                : launch_weights<T, ACT, 128, kSplit>(p, q, st);
+      if (rc) return rc;
+    }
+    const int64_t each = (int64_t)s.M * (s.K + 1);
+    if (s.G > 65535) return invalid("grouped_linear: more than 65535 groups");
+    join_kernel<T><<<dim3((unsigned)ceil_div(each, 32), (unsigned)s.G), 256, 0, st>>>(
+        s, q.parts, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
+  }
   return launch_status("grouped_linear_bwd");
 }
 
@@ -251,7 +1020,8 @@ extern "C" int gs_grouped_linear_fwd(const gs_grouped_params* p, const void* x,
 
 extern "C" size_t gs_grouped_linear_bwd_workspace_size(const gs_grouped_params* p) {
   if (bad_params(p) != GS_OK) return 0;
-  return p->use_row_ids && p->dtype != GS_F32 ? sizeof(float) * (size_t)p->n * p->in_features : 0;
+  const Plan q = plan_of(p);
+  return sizeof(float) * (q.part_floats + q.sum_floats);
 }
 
 extern "C" int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
@@ -266,12 +1036,12 @@ extern "C" int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
                        (p->use_row_ids && !row_ids))))
     return invalid("grouped_linear: missing buffer");
   const size_t need = gs_grouped_linear_bwd_workspace_size(p);
-  if (need > 0 && (!workspace || workspace_bytes < need)) {
-    set_error("grouped_linear: workspace of %zu bytes needed", need);
+  if (!workspace || workspace_bytes < need || !on16(workspace)) {
+    set_error("grouped_linear: a workspace of %zu bytes on a 16-byte boundary is needed", need);
     return GS_ERR_WORKSPACE;
   }
   if (!p->use_row_ids) row_ids = nullptr;
   const Shape s{p->rows, p->n, p->groups, p->in_features, p->out_features};
-  GROUPED_DISPATCH(p, run_bwd, s, p->use_row_ids != 0, x, row_ids, offsets, weights, y, v_y, v_x, v_weights, v_biases,
-                   workspace, as_stream(stream));
+  GROUPED_DISPATCH(p, run_bwd, p, s, x, row_ids, offsets, weights, y, v_y, v_x, v_weights, v_biases,
+                   static_cast<float*>(workspace), as_stream(stream));
 }

@@ -1,0 +1,127 @@
+// The few tcgen05 / mbarrier instructions that the grouped products use, and
+// the formats of their descriptors (PTX ISA, "tcgen05" and "matrix
+// descriptors").  Operands lie in shared memory K-major with the 128-byte
+// swizzle: row r of a panel is 128 bytes at r * 128, its 16-byte chunk c at
+// (c ^ (r & 7)) * 16; panels start on 1024 bytes.
+#pragma once
+
+#include <stdint.h>
+
+namespace gsb {
+namespace tc {
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// Shared-memory descriptor: start and stride (8 rows = 1024 bytes) in units
+// of 16 bytes, version 1, swizzle mode 2 (128 bytes).  A step along K inside
+// the 128-byte row adds its bytes to the start.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (uint64_t(1) << 16) |
+         (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
+enum Format : uint32_t { kF16 = 0, kBF16 = 1, kTF32 = 2 };
+
+// Instruction descriptor: fp32 accumulators, A and B of one format, both
+// K-major, M = 128 lanes, N columns (a multiple of 16).
+__device__ __forceinline__ uint32_t instr_desc(uint32_t format, uint32_t n) {
+  return (1u << 4) | (format << 7) | (format << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+template <bool TF32>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                    bool accumulate) {
+  const uint32_t acc = accumulate;
+  if (TF32)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+
+// Arrives on the barrier once every MMA that this thread issued is done.
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+               ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void fence_before_sync() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void fence_after_sync() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// Generic writes to shared memory become visible to the tensor core.
+__device__ __forceinline__ void fence_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// One warp; columns a power of two from 32 to 512.
+__device__ __forceinline__ void alloc(uint32_t* smem_slot, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+               ::"r"(smem_addr(smem_slot)), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void dealloc(uint32_t tmem, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns)
+               : "memory");
+}
+
+// 16 columns of the warp's 32 lanes: thread l gets lane l's.  The wait is in
+// the same statement, so that no use of the values can move in front of it.
+__device__ __forceinline__ void load16(uint32_t taddr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+
+// Waits for the phase to end, up to `limit` polls of the hardware's own
+// bounded wait; false when it gave up.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
+  uint32_t done = 0;
+  do {
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  } while (!done && limit-- > 0);
+  return done != 0;
+}
+
+// x = hi + lo (+ 2^-22 |x| at most), both with the 11 significant bits of a
+// tf32 operand.  lo = 0 for what is not finite, so that hi alone says what x
+// is; a value whose rounding would overflow is cut instead.
+__device__ __forceinline__ float round_tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return __uint_as_float(r);
+}
+__device__ __forceinline__ void split_tf32(float x, float& hi, float& lo) {
+  hi = round_tf32(x);
+  if (!(fabsf(hi) < INFINITY)) {
+    if (fabsf(x) < INFINITY) hi = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
+    else { lo = 0.0f; return; }
+  }
+  lo = round_tf32(x - hi);
+}
+
+}  // namespace tc
+}  // namespace gsb
