@@ -8,8 +8,11 @@
 // A row's group is found by binary search over the offsets; the search's
 // invariant off[g] <= r < off[g + 1] holds for the pair that it ends at even
 // where the offsets do not ascend, so no index leaves its buffer.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -46,8 +49,12 @@ __device__ __forceinline__ int group_of(const int32_t* __restrict__ off, int G, 
 
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
-  if (ACT == GS_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN passes
-  if (ACT == GS_ACT_SIGMOID) return 1.0f / (1.0f + expf(-z));
+  if (ACT == GS_ACT_RELU) {  // NaN passes
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+    return r;
+  }
+  if (ACT == GS_ACT_SIGMOID) return __fdividef(1.0f, 1.0f + expf(-z));
   return z;
 }
 // v_z from v and the activated y
@@ -61,11 +68,11 @@ __device__ __forceinline__ float through(float v, float y) {
 // ------------------------------------------------------------ tensor-core tiles
 //
 // Operands in 16 bits go to the tensor core as they are.  An fp32 value goes
-// as two tf32 parts, x = hi + lo; the products hi hi are summed in one
-// accumulator and hi lo + lo hi in a second (the neglected lo lo is 2^-22 of
-// the product), which are added in fp32 when the sum is read: about the
-// accuracy of fp32 multiply-adds.  Where the first is not finite it is the
-// result: the second cannot be trusted with infinities (inf * 0).  v_z of the
+// as two tf32 parts, x = hi + lo to 2^-22 |x|; the products hi hi are summed
+// in one accumulator and the three others in a second, which are added in
+// fp32 when the sum is read: about the accuracy of fp32 multiply-adds.  Where the first is not finite it is the
+// result: the second has inf - inf and inf * 0 there, and is not finite only
+// where the first is not.  v_z of the
 // sigmoid in 16 bits goes as two parts in the same manner, so that it is not
 // rounded to 16 bits on its way.
 __device__ unsigned int g_wait_gave_up;
@@ -88,6 +95,7 @@ template <> struct Mma<__half> {
 constexpr int kThreads = 256;
 constexpr int kTile = 128;               // rows of a tile: the lanes of an accumulator
 constexpr int kPanel = kTile * 128;      // bytes of 128 operand rows, 128 bytes deep
+constexpr int kSlotsMost = 6;            // panels of a ring
 
 // The values of one 16-byte chunk.
 template <typename T>
@@ -105,25 +113,30 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 
 // Writes f[0..E) as one operand chunk: one part, or two at a panel's distance.
 template <typename T, bool SPLIT>
-__device__ __forceinline__ void put_chunk(char* at, uint32_t lo_offset, const float* f) {
+__device__ __forceinline__ void put_chunk(char* at, ptrdiff_t lo_offset, const float* f) {
   Chunk<T> hi, lo;
 #pragma unroll
   for (int e = 0; e < Chunk<T>::E; ++e) {
-    if (sizeof(T) == 4) {
-      float a, b;
-      tc::split_tf32(f[e], a, b);
-      hi.v[e] = from_f<T>(a);
-      lo.v[e] = from_f<T>(b);
-    } else {
-      hi.v[e] = from_f<T>(f[e]);
-      if (SPLIT) {
-        const float back = to_f(hi.v[e]);
-        lo.v[e] = from_f<T>(fabsf(back) < INFINITY ? f[e] - back : 0.0f);
-      }
-    }
+    hi.v[e] = from_f<T>(f[e]);
+    if (SPLIT && sizeof(T) == 2) lo.v[e] = from_f<T>(f[e] - to_f(hi.v[e]));
   }
   *reinterpret_cast<uint4*>(at) = hi.q;
-  if (SPLIT || sizeof(T) == 4) *reinterpret_cast<uint4*>(at + lo_offset) = lo.q;
+  if constexpr (sizeof(T) == 4) put_low(at + lo_offset, hi);
+  else if (SPLIT) *reinterpret_cast<uint4*>(at + lo_offset) = lo.q;
+}
+
+// The low part of a chunk of fp32 operands whose upper parts the tensor core
+// takes from the values themselves: x without its 13 low bits; the rest is
+// exact, has 13 bits, and is rounded to the 11 of a tf32 operand (the
+// addition; the bits behind are ignored), which leaves 2^-22 |x|.
+__device__ __forceinline__ void put_low(char* at, const Chunk<float>& x) {
+  Chunk<float> lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float hi = __uint_as_float(__float_as_uint(x.v[e]) & 0xFFFFE000u);
+    lo.v[e] = __uint_as_float(__float_as_uint(x.v[e] - hi) + 0x1000u);
+  }
+  *reinterpret_cast<uint4*>(at) = lo.q;
 }
 
 // E values from p: one access, or one by one where p is not aligned or fewer
@@ -142,14 +155,14 @@ __device__ __forceinline__ uint4 get_chunk(const T* __restrict__ p, int there) {
 
 // Consecutive rows of one group, at most `most` of them, up to `end`.
 struct Run {
-  int64_t row;
+  int row;
   int n;      // 0: no rows are left
   int g;      // -1 or G: outside every group
-  int64_t group_end;
+  int group_end;
 };
 
-__device__ __forceinline__ Run run_from(const int32_t* __restrict__ off, int G, int64_t row,
-                                        int64_t end, int most, Run prev) {
+__device__ __forceinline__ Run run_from(const int32_t* __restrict__ off, int G, int row, int end,
+                                        int most, Run prev) {
   Run t;
   t.row = row;
   t.g = prev.g;
@@ -160,10 +173,10 @@ __device__ __forceinline__ Run run_from(const int32_t* __restrict__ off, int G, 
   }
   if (row >= t.group_end) {
     t.g = group_of(off, G, row);
-    const int64_t stop = t.g < 0 ? __ldg(off) : t.g < G ? __ldg(off + t.g + 1) : end;
+    const int stop = t.g < 0 ? __ldg(off) : t.g < G ? __ldg(off + t.g + 1) : end;
     t.group_end = min(stop, end);
   }
-  t.n = (int)min((int64_t)most, t.group_end - row);
+  t.n = min(most, t.group_end - row);
   return t;
 }
 
@@ -186,302 +199,499 @@ struct RowsArgs {
   int nt;                  // columns of a CTA's tile: a multiple of 32
   int panels;              // of `depth`
   int resident;            // all weight panels of the tile stay in shared memory
+  int slots;               // panels of rows that are in flight or in use
   int wide_w, wide_out;    // 16-byte accesses are aligned
 };
 
 enum { kForward, kBackward, kScatter };
 
-template <typename T, bool SPLIT>
+template <typename T, int ACT, int MODE, bool SPLIT>
 struct RowsLayout {
-  static constexpr int kTerms = SPLIT || sizeof(T) == 4 ? 2 : 1;  // parts of a row value
-  static constexpr int kWTerms = sizeof(T) == 4 ? 2 : 1;          // of a weight
-  // also the warps' staging of results: 8 x 32 rows x 32 columns
-  static constexpr int kA = kTerms * kPanel > 32768 ? kTerms * kPanel : 32768;
-  static int weight_panels(const RowsArgs& p) { return p.resident ? p.panels : 1; }
+  static constexpr bool kY = MODE != kForward && ACT != GS_ACT_NONE;  // y is read too
+  static constexpr int kTerms = SPLIT || sizeof(T) == 4 ? 2 : 1;      // parts of a row value
+  static constexpr int kWTerms = sizeof(T) == 4 ? 2 : 1;              // of a weight
+  // low parts of two panels; with y they take the place of the panel's y
+  static constexpr int kLow = kTerms == 2 && !kY ? 2 * kPanel : 0;
+  static constexpr int kStage = 8 * 2048;                             // the warps' results
   static int smem(const RowsArgs& p) {
-    return 1024 + kA + weight_panels(p) * kWTerms * p.nt * 128;
+    return 1024 + kLow + kStage + p.slots * kPanel * (kY ? 2 : 1) +
+           (p.resident ? p.panels : 1) * kWTerms * p.nt * 128;
   }
+  // two accumulators (of two parts), so that one is read while the next
+  // tile's is made
   static int columns(int nt) {
     int c = 32;
-    while (c < nt * kTerms) c *= 2;
+    while (c < 2 * nt * kTerms) c *= 2;
     return c;
   }
 };
 
+// Eight sums as a chunk of 16-bit results; two convert in one instruction.
+template <typename T>
+__device__ __forceinline__ uint4 round_chunk(const float* v) {
+  uint4 q;
+  uint32_t* const r = &q.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same<T, __half>::value)
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+    else
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+  }
+  return q;
+}
+
+// One chunk of a row on its way to shared memory: `there` values from p (none
+// where there <= 0), zeros behind them.  WIDE: 16 bytes at once.  Else by
+// single fp32 values, or, for 16-bit rows off the boundary, through
+// registers.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void send_chunk(char* to, const T* __restrict__ p, int there) {
+  constexpr int E = Chunk<T>::E;
+  if (there <= 0) {
+    *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+  } else if constexpr (WIDE) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                 ::"r"(tc::smem_addr(to)), "l"(p) : "memory");
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                   ::"r"(tc::smem_addr(to + 4 * e)), "l"(e < there ? p + e : p),
+                   "r"(e < there ? 4 : 0) : "memory");
+  } else {
+    *reinterpret_cast<uint4*>(to) = get_chunk<T, false>(p, there);
+  }
+}
+__device__ __forceinline__ void send_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the last `n` groups have arrived.
+__device__ __forceinline__ void arrived(int n) {
+  if (n >= 4) asm volatile("cp.async.wait_group 4;" ::: "memory");
+  else if (n == 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (n == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (n == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
 // out[row] = f(rows a, weights of the row's group): the forward, and v_x.
 //
-// A CTA streams its consecutive 128-row tiles; the rows' 16-byte chunks go
-// through registers (16 KB a CTA in flight, the next panel's while this one
-// is multiplied and stored) into swizzled panels, which lets the gather, the
-// activation's reverse mode, the split into parts and the zeros behind K
-// happen on the way; one thread issues the MMAs.  The group's weights are
-// staged once per group, and stay.
-template <typename T, int ACT, int MODE, bool WIDE, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 2) rows_mma_kernel(RowsArgs p, int columns) {
-  using L = RowsLayout<T, SPLIT>;
+// One CTA an SM streams consecutive 128-row tiles, a panel (128 bytes of
+// depth) at a time, through a ring of `slots` panels.  Its front half (8
+// warps) has the panels filled -- TMA: rows that lie together; asynchronous
+// 16- or 4-byte copies: gathered rows and fp32 rows off the boundary --,
+// makes operands of them, and issues the MMAs; its back half takes a tile's
+// accumulator while the front is at the next tile's.  16-bit rows are
+// multiplied as they arrive; of fp32 rows the tensor core reads the upper
+// part itself (it ignores the 13 low bits) and the low part is written beside;
+// the backward through an activation rewrites the panel as v_z.  The group's
+// weights are staged once per group, and stay.
+//
+// Front and back run one after the other in an earlier form (two CTAs an SM,
+// 128-128 bf16, 2 M rows): 211 us; a tile took 1900 cycles a panel and 2300 for
+// its results.
+enum { kTma, kCopy };  // how rows arrive
+
+template <typename T, int ACT, int MODE, int LOAD, bool WIDE, bool SPLIT>
+__global__ void __launch_bounds__(2 * kThreads, 1)
+    rows_mma_kernel(RowsArgs p, int columns, const __grid_constant__ CUtensorMap map_a,
+                    const __grid_constant__ CUtensorMap map_y) {
+  using L = RowsLayout<T, ACT, MODE, SPLIT>;
   constexpr int E = Chunk<T>::E;
   constexpr int DP = 128 / sizeof(T);   // depth of a panel
   constexpr int STEP = 32 / sizeof(T);  // depth of an MMA
   constexpr bool BACK = MODE != kForward;
   extern __shared__ char smem_raw[];
-  __shared__ uint64_t s_bar;
+  __shared__ uint64_t s_bars[2 * kSlotsMost + 4];
   __shared__ uint32_t s_tmem;
-  __shared__ int32_t s_ids[4][kTile];
-  __shared__ float s_bias[kTile];
-  char* const s_a = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
-  char* const s_w = s_a + L::kA;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ __align__(16) float s_bias[8][kTile];
+  char* const s_low = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
+  char* const s_stage = s_low + L::kLow;
+  char* const s_rows = s_stage + L::kStage;
+  char* const s_y = s_rows + p.slots * kPanel;
+  char* const s_w = s_y + (L::kY ? p.slots * kPanel : 0);
+  const uint32_t bar0 = tc::smem_addr(s_bars);
+  auto full = [&](int i) { return bar0 + 8 * i; };                       // a slot has its rows
+  auto free_ = [&](int i) { return bar0 + 8 * (kSlotsMost + i); };       // its MMAs are done
+  auto made = [&](int i) { return bar0 + 8 * (2 * kSlotsMost + i); };    // an accumulator is
+  auto taken = [&](int i) { return bar0 + 8 * (2 * kSlotsMost + 2 + i); };
+  const int lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be uniform
   const int n0 = blockIdx.y * p.nt;
   const int cols = min(p.nt, p.width - n0);
   const int wbytes = p.nt * 128;  // of a weight panel's part
-  const T* const a = static_cast<const T*>(p.a);
-  const T* const y = static_cast<const T*>(p.y);
-  const T* const w = static_cast<const T*>(p.w);
-  const T* const bias = static_cast<const T*>(p.bias);
 
   if (warp == 0) tc::alloc(&s_tmem, columns);
-  if (tid == 0) tc::bar_init(tc::smem_addr(&s_bar), 1);
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < p.slots; ++i) {
+      tc::bar_init(full(i), 1);
+      tc::bar_init(free_(i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::bar_init(made(i), 1);
+      tc::bar_init(taken(i), 8);
+    }
+    tc::bar_init_done();
+  }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = s_tmem, bar = tc::smem_addr(&s_bar);
-  const uint32_t idesc = tc::instr_desc(Mma<T>::format, (cols + 15) / 16 * 16);
-  uint32_t phase = 0, limit = kWaitLimit;
-  auto wait_mma = [&]() {
-    if (!tc::bar_wait(bar, phase, limit)) {
+  const uint32_t tmem = s_tmem;
+  uint32_t limit = kWaitLimit;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (!tc::bar_wait(bar, parity & 1, limit)) {
       limit = 0;  // results are void: no later wait holds the kernel up
       g_wait_gave_up = 1;
     }
-    phase ^= 1;
-    tc::fence_after_sync();
   };
 
   const int64_t tiles = (p.s.R + kTile - 1) / kTile;
-  const int64_t end = min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
+  const int end = (int)min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
   Run none;
-  none.row = 0, none.n = 0, none.g = -1, none.group_end = 0;
-  Run cur = run_from(p.off, p.s.G, first_tile(tiles, gridDim.x, blockIdx.x) * kTile, end, kTile, none);
-  Run nxt = run_from(p.off, p.s.G, cur.row + cur.n, end, kTile, cur);
+  none.row = (int)(first_tile(tiles, gridDim.x, blockIdx.x) * kTile);
+  none.n = 0, none.g = -1, none.group_end = 0;
+  auto after = [&](const Run& t) { return run_from(p.off, p.s.G, t.row + t.n, end, kTile, t); };
 
-  auto id_of = [&](const Run& t, int i) {
-    return p.ids && i < t.n ? __ldg(p.ids + t.row + i) : -1;
-  };
-  uint4 ra[4], ry[BACK && ACT ? 4 : 1];
-  // this thread's four chunks of panel j of tile t (number k of this CTA's)
-  auto load_panel = [&](const Run& t, int k, int j) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = (tid >> 3) + 32 * i, d = j * DP + (tid & 7) * E;
-      int64_t at = t.row + row;
-      bool ok = row < t.n && t.g >= 0 && t.g < p.s.G;
-      if (!BACK && p.ids) {
-        at = s_ids[k & 3][row];
-        ok = ok && at >= 0 && at < p.s.n;
+  if (warp < 8) {
+    // ------------------------------------------------------------ front half
+    const int tid = threadIdx.x;
+    const T* const a = static_cast<const T*>(p.a);
+    const T* const y = static_cast<const T*>(p.y);
+    const T* const w = static_cast<const T*>(p.w);
+    const uint32_t idesc = tc::instr_desc(Mma<T>::format, (cols + 15) / 16 * 16);
+    auto after_live = [&](Run t) {  // rows outside every group are not the front's
+      t = after(t);
+      while (t.n > 0 && (t.g < 0 || t.g >= p.s.G)) {
+        t.n = t.group_end - t.row;
+        t = after(t);
       }
-      const int there = ok ? p.depth - d : 0;
-      const int64_t from = ok ? at * p.depth + d : 0;
-      ra[i] = get_chunk<T, WIDE>(a + from, there);
-      if (BACK && ACT) ry[BACK && ACT ? i : 0] = get_chunk<T, WIDE>(y + from, there);
-    }
-  };
-  // weight panels [j0, j1) of group g: rows n (columns of the result) x depth
-  auto stage_weights = [&](int g, int j0, int j1) {
-    const T* const wg = w + (int64_t)g * p.s.M * p.s.K;
-    const int units = (j1 - j0) * 8 * cols;
-    for (int u = tid; u < units; u += kThreads) {
-      int n, c, j;
-      Chunk<T> q;
-      if (!BACK) {  // chunks of a weight row
-        c = u & 7, n = (u >> 3) % cols, j = (u >> 3) / cols;
-        const int d = (j0 + j) * DP + c * E;
-        const T* const from = wg + (int64_t)(n0 + n) * p.depth + d;
-        if (p.wide_w)
-          q.q = get_chunk<T, true>(d < p.depth ? from : wg, p.depth - d);
-        else
-          q.q = get_chunk<T, false>(from, p.depth - d);
-      } else {      // down a weight column; neighbours are neighbouring threads'
-        n = u % cols, c = (u / cols) & 7, j = u / cols / 8;
-        const int d = (j0 + j) * DP + c * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          q.v[e] = d + e < p.depth ? wg[(int64_t)(d + e) * p.width + n0 + n] : from_f<T>(0.0f);
-      }
-      float f[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = to_f(q.v[e]);
-      put_chunk<T, false>(s_w + j * L::kWTerms * wbytes + chunk_at(n, c), wbytes, f);
-    }
-  };
-
-  if (tid < kTile) s_ids[0][tid] = id_of(cur, tid);
-  int next_id = tid < kTile ? id_of(nxt, tid) : -1;
-  __syncthreads();
-  load_panel(cur, 0, 0);
-  int staged = -2;
-
-  for (int k = 0; cur.n > 0; ++k) {
-    const bool live = cur.g >= 0 && cur.g < p.s.G;
-    if (live && cur.g != staged) {  // every MMA of the group before is done
-      if (p.resident) stage_weights(cur.g, 0, p.panels);
-      if (tid < kTile)
-        s_bias[tid] = !BACK && bias && tid < cols ? to_f(bias[(int64_t)cur.g * p.s.M + n0 + tid]) : 0.0f;
-      staged = cur.g;
-    }
-    Run after = nxt;
-    for (int j = 0; j < p.panels; ++j) {
-      if (live) {
-        if (j > 0) wait_mma();  // the panel's memory is free again
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          char* const to = s_a + chunk_at((tid >> 3) + 32 * i, tid & 7);
-          Chunk<T> q;
-          q.q = ra[i];
-          if (sizeof(T) == 2 && !SPLIT && !(BACK && ACT)) {
-            *reinterpret_cast<uint4*>(to) = q.q;
-            continue;
-          }
-          float f[E];
-#pragma unroll
-          for (int e = 0; e < E; ++e) f[e] = to_f(q.v[e]);
-          if (BACK && ACT) {
-            Chunk<T> o;
-            o.q = ry[BACK && ACT ? i : 0];
-#pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = through<ACT>(f[e], to_f(o.v[e]));
-          }
-          put_chunk<T, SPLIT>(to, kPanel, f);
-        }
-        if (!p.resident) stage_weights(cur.g, j, j + 1);
-      }
-      if (j == 0 && tid < kTile) s_ids[(k + 1) & 3][tid] = next_id;
-      tc::fence_smem();
-      tc::fence_before_sync();
-      __syncthreads();
-      if (live && tid == 0) {
-        tc::fence_after_sync();
-        const int steps = (min(DP, p.depth - j * DP) + STEP - 1) / STEP;
-        const uint64_t da = tc::smem_desc(tc::smem_addr(s_a));
-        const uint64_t dw = tc::smem_desc(tc::smem_addr(s_w + (p.resident ? j : 0) * L::kWTerms * wbytes));
-        const uint64_t lo_a = kPanel >> 4, lo_w = wbytes >> 4;
-        for (int i = 0; i < steps; ++i) {
-          const uint64_t at = 2 * i;  // 32 bytes
-          const bool more = j > 0 || i > 0;
-          if (L::kTerms == 2) {
-            tc::mma<Mma<T>::TF32>(tmem + p.nt, da + lo_a + at, dw + at, idesc, more);
-            if (L::kWTerms == 2)
-              tc::mma<Mma<T>::TF32>(tmem + p.nt, da + at, dw + lo_w + at, idesc, true);
-          }
-          tc::mma<Mma<T>::TF32>(tmem, da + at, dw + at, idesc, more);
-        }
-        tc::commit(bar);
-      }
-      // the next panel's rows are on their way while this one is multiplied
-      if (j + 1 < p.panels) {
-        load_panel(cur, k, j + 1);
-      } else if (nxt.n > 0) {
-        load_panel(nxt, k + 1, 0);
-        after = run_from(p.off, p.s.G, nxt.row + nxt.n, end, kTile, nxt);
-        if (tid < kTile) next_id = id_of(after, tid);
-      } else {
-        after.n = 0;
-      }
-    }
-    if (live) wait_mma();
-
-    // 32 rows x 32 columns at a time: out of the accumulator, through the
-    // warp's own part of the operand memory, and in whole rows to `out`
-    constexpr int OB = MODE == kScatter ? 4 : sizeof(T);  // bytes of a result
-    constexpr int OE = 16 / OB;
-    constexpr int CH = 32 / OE;                           // chunks of 32 columns
-    char* const stage = s_a + warp * (32 * 32 * OB);
-    auto stage_at = [&](int r, int c) {
-      return stage + r * (32 * OB) + ((c ^ (CH == 8 ? r & 7 : (r >> 1) & 3)) << 4);
+      return t;
     };
-    const int row0 = (warp & 3) * 32;
-    const int rows = min(32, cur.n - row0);
-    for (int c0 = (warp >> 2) * 32; c0 < cols; c0 += 64) {
+    auto steps_of = [&](int j) { return (min(DP, p.depth - j * DP) + STEP - 1) / STEP; };
+    const int c16 = tid & 7, r16 = tid >> 3;  // this thread's chunk, and its rows r16 + 32 i
+    const uint32_t o16 = chunk_at(r16, c16);  // + 4096 i in a panel
+
+    // The panel that is sent next: panel ahead_j of the tile `ahead`, number
+    // `ahead_q` of the CTA's, into slot `ahead_s`.
+    Run ahead = after_live(none), behind = ahead;
+    int ahead_j = 0, ahead_q = 0, ahead_s = 0;
+    int at[4], id[4];  // rows of x, gathered: validated, and as read for the tile after
+    auto read_ids = [&](const Run& t) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[16];
-        if (live) {
-          const uint32_t from = tmem + ((uint32_t)row0 << 16) + c0 + h * 16;
-          tc::load16(from, v);
-          if (L::kTerms == 2) {
-            float u[16];
-            tc::load16(from + p.nt, u);
+      for (int i = 0; i < 4; ++i)
+        id[i] = p.ids && !BACK && r16 + 32 * i < t.n ? __ldg(p.ids + t.row + r16 + 32 * i) : -1;
+    };
+    auto settle = [&]() {  // of the tile that is sent now
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (fabsf(v[i]) < INFINITY) v[i] += u[i];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (!live) v[i] = 0.0f;
-          else if (!BACK) v[i] = activate<ACT>(v[i] + s_bias[c0 + h * 16 + i]);
-        }
-#pragma unroll
-        for (int c = 0; c < CH / 2; ++c) {
-          char* const to = stage_at(lane, h * (CH / 2) + c);
-          if constexpr (OB == 4) {
-            *reinterpret_cast<float4*>(to) =
-                make_float4(v[c * OE], v[c * OE + 1], v[c * OE + 2], v[c * OE + 3]);
-          } else {
-            Chunk<T> q;
-#pragma unroll
-            for (int e = 0; e < OE; ++e) q.v[e] = from_f<T>(v[c * OE + e]);
-            *reinterpret_cast<uint4*>(to) = q.q;
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int row = r16 + 32 * i;
+        if (p.ids && !BACK) at[i] = id[i] < p.s.n ? id[i] : -1;
+        else at[i] = row < ahead.n ? ahead.row + row : -1;
       }
-      __syncwarp();
-      const int width = min(32, cols - c0);  // columns here
-      if (MODE == kScatter) {
-        float* const sum = static_cast<float*>(p.out);
-        if (live) {
-          const int c = lane & 7;
-          for (int r = lane >> 3; r < rows; r += 4) {
-            const int32_t at = s_ids[k & 3][row0 + r];
-            if (at < 0 || at >= p.s.n || c * 4 >= width) continue;
-            float* const to = sum + (int64_t)at * p.width + n0 + c0 + c * 4;
-            const float4 q = *reinterpret_cast<const float4*>(stage_at(r, c));
-            if (p.wide_out) {
-              asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
-                           ::"l"(to), "f"(q.x), "f"(q.y), "f"(q.z), "f"(q.w) : "memory");
-            } else {
-              atomicAdd(to, q.x);
-              if (c * 4 + 1 < width) atomicAdd(to + 1, q.y);
-              if (c * 4 + 2 < width) atomicAdd(to + 2, q.z);
-              if (c * 4 + 3 < width) atomicAdd(to + 3, q.w);
+    };
+    if (LOAD == kCopy) {
+      read_ids(ahead);
+      settle();
+      behind = after_live(ahead);
+      read_ids(behind);
+    }
+    auto send = [&]() {
+      if (ahead.n > 0) {
+        if (LOAD == kTma) {
+          if (warp == 1) {
+            // the slot's former panel is done with
+            if (ahead_q >= p.slots) wait(free_(ahead_s), ahead_q / p.slots - 1);
+            if (tc::elected()) {
+              const uint32_t to = tc::smem_addr(s_rows + ahead_s * kPanel);
+              tc::expect(full(ahead_s), kPanel * (L::kY ? 2 : 1));
+              tc::load_box(to, &map_a, ahead_j * DP, ahead.row, full(ahead_s));
+              if (L::kY)
+                tc::load_box(to + p.slots * kPanel, &map_y, ahead_j * DP, ahead.row, full(ahead_s));
+            }
+            __syncwarp();
+          }
+        } else {
+          if (ahead_q >= p.slots) wait(free_(ahead_s), ahead_q / p.slots - 1);
+          if (c16 < 2 * steps_of(ahead_j)) {
+            const int d = ahead_j * DP + c16 * E;
+            const uint32_t to = ahead_s * kPanel + o16;
+            const T* const ad = a + d;
+            const T* const yd = L::kY ? y + d : nullptr;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int there = at[i] >= 0 ? p.depth - d : 0;
+              const int64_t from = (int64_t)at[i] * p.depth;
+              send_chunk<T, WIDE>(s_rows + to + 4096 * i, ad + from, there);
+              if (L::kY) send_chunk<T, WIDE>(s_y + to + 4096 * i, yd + from, there);
             }
           }
         }
-      } else {
-        T* const out = static_cast<T*>(p.out) + (cur.row + row0) * p.width + n0 + c0;
-        if (p.wide_out) {
-          const int c = lane & (CH - 1);
-          if (c * OE < width)
-            for (int r = lane / CH; r < rows; r += 32 / CH)
-              *reinterpret_cast<uint4*>(out + (int64_t)r * p.width + c * OE) =
-                  *reinterpret_cast<const uint4*>(stage_at(r, c));
-        } else if (p.width <= 32) {  // whole rows: one run of memory
-          const int total = rows * width;
-          for (int i = lane; i < total; i += 32) {
-            const int r = i / width, c = i - r * width;
-            out[i] = reinterpret_cast<const T*>(stage_at(r, c / OE))[c % OE];
+        ++ahead_q;
+        ahead_s = ahead_s + 1 == p.slots ? 0 : ahead_s + 1;
+        if (++ahead_j == p.panels) {
+          ahead_j = 0;
+          if (LOAD == kCopy) {
+            ahead = behind;
+            settle();
+            behind = after_live(ahead);
+            read_ids(behind);
+          } else {
+            ahead = after_live(ahead);
           }
-        } else if (lane < width) {
-          for (int r = 0; r < rows; ++r)
-            out[(int64_t)r * p.width + lane] =
-                reinterpret_cast<const T*>(stage_at(r, lane / OE))[lane % OE];
         }
       }
-      __syncwarp();
+      if (LOAD == kCopy) send_done();  // also where nothing is left, to keep the count
+    };
+
+    // weight panels [j0, j1) of group g: rows n (columns of the result) x depth
+    const int wlog = p.nt > 64 ? 7 : p.nt > 32 ? 6 : 5;
+    auto stage_weights = [&](int g, int j0, int j1) {
+      const T* const wg = w + (int64_t)g * p.s.M * p.s.K;
+      const int units = (j1 - j0) * 8 << wlog;
+      for (int u0 = tid; u0 < units; u0 += 4 * kThreads) {  // four loads in flight
+        Chunk<T> q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int u = u0 + i * kThreads;
+          if (!BACK) {  // chunks of a weight row
+            const int c = u & 7, n = (u >> 3) & ((1 << wlog) - 1), j = u >> (3 + wlog);
+            const int d = (j0 + j) * DP + c * E;
+            const int there = u < units && n < cols ? p.depth - d : 0;
+            const T* const from = wg + (there > 0 ? (int64_t)(n0 + n) * p.depth + d : 0);
+            q[i].q = p.wide_w ? get_chunk<T, true>(from, there) : get_chunk<T, false>(from, there);
+          } else {      // down a weight column; neighbours are neighbouring threads'
+            const int n = u & ((1 << wlog) - 1), c = (u >> wlog) & 7, j = u >> (3 + wlog);
+            const int d = (j0 + j) * DP + c * E;
+            const bool in = u < units && n < cols;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              q[i].v[e] = in && d + e < p.depth ? wg[(int64_t)(d + e) * p.width + n0 + n]
+                                                : from_f<T>(0.0f);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int u = u0 + i * kThreads;
+          const int c = BACK ? (u >> wlog) & 7 : u & 7, j = u >> (3 + wlog);
+          const int n = (BACK ? u : u >> 3) & ((1 << wlog) - 1);
+          if (u < units && n < p.nt) {
+            char* const to = s_w + j * L::kWTerms * wbytes + chunk_at(n, c);
+            *reinterpret_cast<uint4*>(to) = q[i].q;
+            if constexpr (sizeof(T) == 4) put_low(to + wbytes, q[i]);
+          }
+        }
+      }
+    };
+
+    for (int i = 1; i < p.slots; ++i) send();
+    int staged = -1, slot = 0, q = 0, t = 0;
+    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur), ++t) {
+      if (cur.g != staged) {
+        // every MMA of the group before is done
+        if (q > 0) wait(free_(slot == 0 ? p.slots - 1 : slot - 1), (q - 1) / p.slots);
+        if (p.resident) stage_weights(cur.g, 0, p.panels);
+        staged = cur.g;
+      }
+      for (int j = 0; j < p.panels; ++j, ++q) {
+        const int steps = steps_of(j);
+        char* const here = s_rows + slot * kPanel;
+        char* const low = L::kY ? s_y + slot * kPanel : s_low + (q & 1) * kPanel;
+        if (LOAD == kCopy) arrived(p.slots - 2);
+        else wait(full(slot), q / p.slots);
+        if (!p.resident) {
+          if (q > 0) wait(free_(slot == 0 ? p.slots - 1 : slot - 1), (q - 1) / p.slots);
+          stage_weights(cur.g, j, j + 1);
+        }
+        if (L::kTerms == 2 || L::kY) {
+          if (L::kLow && q > 1) {  // the low parts of two panels ago are done with
+            const int before = slot > 1 ? slot - 2 : slot + p.slots - 2;
+            wait(free_(before), (q - 2) / p.slots);
+          }
+          if (c16 < 2 * steps) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t o = o16 + 4096 * i;
+              Chunk<T> v;
+              v.q = *reinterpret_cast<const uint4*>(here + o);
+              if constexpr (L::kY) {
+                Chunk<T> z;
+                z.q = *reinterpret_cast<const uint4*>(low + o);
+                float f[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) f[e] = through<ACT>(to_f(v.v[e]), to_f(z.v[e]));
+                put_chunk<T, SPLIT>(here + o, low - here, f);
+              } else if constexpr (sizeof(T) == 4) {
+                put_low(low + o, v);
+              }
+            }
+          }
+        }
+        tc::fence_smem();
+        tc::bar_sync(1, kThreads);
+        if (warp == 0) {
+          if (j == 0 && t > 1) wait(taken(t & 1), (t >> 1) - 1);
+          tc::fence_after_sync();
+          const uint32_t leader = tc::elected();
+          const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms;
+          const uint64_t da = tc::smem_desc(tc::smem_addr(here));
+          const uint64_t dl = tc::smem_desc(tc::smem_addr(low));
+          const uint64_t dw =
+              tc::smem_desc(tc::smem_addr(s_w + (p.resident ? j : 0) * L::kWTerms * wbytes));
+          const uint64_t lo_w = wbytes >> 4;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i >= steps) break;
+            const uint64_t step = 2 * i;  // 32 bytes
+            const bool more = j > 0 || i > 0;
+            if (L::kTerms == 2) {
+              tc::mma<Mma<T>::TF32>(leader, acc + p.nt, dl + step, dw + step, idesc, more);
+              if (L::kWTerms == 2) {
+                tc::mma<Mma<T>::TF32>(leader, acc + p.nt, da + step, dw + lo_w + step, idesc, true);
+                tc::mma<Mma<T>::TF32>(leader, acc + p.nt, dl + step, dw + lo_w + step, idesc, true);
+              }
+            }
+            tc::mma<Mma<T>::TF32>(leader, acc, da + step, dw + step, idesc, more);
+          }
+          tc::commit(leader, free_(slot));
+          if (j + 1 == p.panels) tc::commit(leader, made(t & 1));
+        }
+        send();
+        slot = slot + 1 == p.slots ? 0 : slot + 1;
+      }
     }
-    tc::fence_before_sync();
-    __syncthreads();  // the operand memory and the accumulators are free
-    cur = nxt;
-    nxt = after;
+    if (LOAD == kCopy) arrived(0);
+    // every MMA is done before the memory goes
+    if (q > 0) wait(free_(slot == 0 ? p.slots - 1 : slot - 1), (q - 1) / p.slots);
+  } else {
+    // ------------------------------------------------------------- back half
+    const T* const bias = static_cast<const T*>(p.bias);
+    const int bw = warp - 8, row0 = (bw & 3) * 32;  // lanes of the accumulator
+    float* const my_bias = s_bias[bw];
+    int biased = -1, t = 0;
+    // 32 rows x 64 bytes at a time: out of the accumulator, through the warp's
+    // own piece of shared memory, and in pieces of rows to `out`
+    constexpr int OB = MODE == kScatter ? 4 : sizeof(T);  // bytes of a result
+    constexpr int OE = 16 / OB, SC = 64 / OB;             // results in 16 and in 64 bytes
+    char* const stage = s_stage + bw * 2048;
+    auto stage_at = [&](int r, int c) { return stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4); };
+
+    for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
+      const bool live = cur.g >= 0 && cur.g < p.s.G;
+      const int rows = min(32, cur.n - row0);
+      int32_t into = -1;  // where lane's row is added up
+      if (MODE == kScatter && live && lane < rows) into = __ldg(p.ids + cur.row + row0 + lane);
+      const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms + ((uint32_t)row0 << 16);
+      if (live) {
+        if (!BACK && cur.g != biased) {
+          __syncwarp();
+          for (int i = lane; i < p.nt; i += 32)
+            my_bias[i] = bias && i < cols ? to_f(bias[(int64_t)cur.g * p.s.M + n0 + i]) : 0.0f;
+          __syncwarp();
+          biased = cur.g;
+        }
+        wait(made(t & 1), t >> 1);
+        tc::fence_after_sync();
+      }
+      if (into >= p.s.n) into = -1;
+      for (int c0 = (bw >> 2) * SC; c0 < cols; c0 += 2 * SC) {
+        const int width = min(SC, cols - c0);  // columns here
+#pragma unroll
+        for (int h = 0; h < SC / 16; ++h) {
+          if (h * 16 >= width) break;
+          float v[16];
+          if (live) {
+            tc::load16(acc + c0 + h * 16, v);
+            if (L::kTerms == 2) {
+              float u[16];
+              tc::load16(acc + p.nt + c0 + h * 16, u);
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+            }
+          }
+          if (!live) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+          } else if (!BACK) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (ACT == GS_ACT_SIGMOID && h * 16 + k * 4 >= width) break;  // 20 instructions each
+              const float4 b = *reinterpret_cast<const float4*>(my_bias + c0 + h * 16 + k * 4);
+              v[k * 4] = activate<ACT>(v[k * 4] + b.x);
+              v[k * 4 + 1] = activate<ACT>(v[k * 4 + 1] + b.y);
+              v[k * 4 + 2] = activate<ACT>(v[k * 4 + 2] + b.z);
+              v[k * 4 + 3] = activate<ACT>(v[k * 4 + 3] + b.w);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 16 / OE; ++c) {
+            char* const to = stage_at(lane, h * (16 / OE) + c);
+            if constexpr (OB == 4)
+              *reinterpret_cast<float4*>(to) =
+                  make_float4(v[c * OE], v[c * OE + 1], v[c * OE + 2], v[c * OE + 3]);
+            else
+              *reinterpret_cast<uint4*>(to) = round_chunk<T>(v + c * OE);
+          }
+        }
+        __syncwarp();
+        const int c = lane & 3;
+        if constexpr (MODE == kScatter) {
+          float* const sum = static_cast<float*>(p.out);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = (lane >> 2) + 8 * i;
+            const int32_t to_row = __shfl_sync(0xffffffffu, into, r);
+            if (to_row < 0 || c * 4 >= width) continue;
+            float* const to = sum + (int64_t)to_row * p.width + n0 + c0 + c * 4;
+            const float4 v = *reinterpret_cast<const float4*>(stage_at(r, c));
+            if (p.wide_out) {
+              asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
+                           ::"l"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+            } else {
+              atomicAdd(to, v.x);
+              if (c * 4 + 1 < width) atomicAdd(to + 1, v.y);
+              if (c * 4 + 2 < width) atomicAdd(to + 2, v.z);
+              if (c * 4 + 3 < width) atomicAdd(to + 3, v.w);
+            }
+          }
+        } else {
+          T* const out = static_cast<T*>(p.out) + (int64_t)(cur.row + row0) * p.width + n0 + c0;
+          if (p.wide_out) {
+            if (c * OE < width) {
+              T* to = out + (int64_t)(lane >> 2) * p.width + c * OE;
+              const int64_t down = (int64_t)8 * p.width;
+#pragma unroll
+              for (int i = 0; i < 4; ++i, to += down)
+                if ((lane >> 2) + 8 * i < rows)
+                  *reinterpret_cast<uint4*>(to) =
+                      *reinterpret_cast<const uint4*>(stage_at((lane >> 2) + 8 * i, c));
+            }
+          } else if (p.width <= SC) {  // whole rows: one run of memory
+            const int total = rows * width;
+            for (int i = lane; i < total; i += 32) {
+              const int r = i / width, e = i - r * width;
+              out[i] = reinterpret_cast<const T*>(stage_at(r, e / OE))[e % OE];
+            }
+          } else {
+            constexpr int LR = 32 / SC;  // rows that the lanes cover
+            const int e = lane & (SC - 1);
+            if (e < width)
+              for (int r = lane / SC; r < rows; r += LR)
+                out[(int64_t)r * p.width + e] =
+                    reinterpret_cast<const T*>(stage_at(r, e / OE))[e % OE];
+          }
+        }
+        __syncwarp();
+      }
+      if (live) {
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::arrive(taken(t & 1));
+        ++t;
+      }
+    }
   }
+  tc::fence_before_sync();
+  __syncthreads();
   if (warp == 0) tc::dealloc(tmem, columns);
 }
 
@@ -527,7 +737,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
   __shared__ int32_t s_ids[4][DP];
   char* const s_x = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
   char* const s_v = s_x + XTERMS * kPanel;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int k0 = (blockIdx.y % p.kt) * 128, m0 = (blockIdx.y / p.kt) * NT;
   const int kn = min(128, p.s.K - k0), mn = min(NT, p.s.M - m0);
   const T* const x = static_cast<const T*>(p.x);
@@ -535,7 +746,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
   const T* const vy = static_cast<const T*>(p.vy);
 
   if (warp == 0) tc::alloc(&s_tmem, columns);
-  if (tid == 0) tc::bar_init(tc::smem_addr(&s_bar), 1);
+  if (tid == 0) {
+    tc::bar_init(tc::smem_addr(&s_bar), 1);
+    tc::bar_init_done();
+  }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -570,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
   for (int e = 0; e < E; ++e) bsum[e] = 0.0f;
 
   const int64_t tiles = (p.s.R + kTile - 1) / kTile;
-  const int64_t end = min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
+  const int end = (int)min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
   auto next_run = [&](Run t) {  // skips rows outside every group
     Run n = run_from(p.off, p.s.G, t.row + t.n, end, DP, t);
     while (n.n > 0 && (n.g < 0 || n.g >= p.s.G))
@@ -578,8 +792,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
     return n;
   };
   Run none;
-  none.row = first_tile(tiles, gridDim.x, blockIdx.x) * kTile, none.n = 0, none.g = -1;
-  none.group_end = 0;
+  none.row = (int)(first_tile(tiles, gridDim.x, blockIdx.x) * kTile);
+  none.n = 0, none.g = -1, none.group_end = 0;
   Run cur = next_run(none);
   Run nxt = next_run(cur);
   auto id_of = [&](const Run& t, int i) {
@@ -590,18 +804,18 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
     for (int i = 0; i < E; ++i) {
       const bool in = rb + i < t.n;
       if (has_x) {
-        int64_t at = t.row + rb + i;
+        int at = t.row + rb + i;
         bool ok = in;
         if (p.ids) {
           at = s_ids[k & 3][rb + i];
           ok = at >= 0 && at < p.s.n;
         }
-        const T* const from = x + (ok ? at * p.s.K + k0 + xc : 0);
+        const T* const from = x + (ok ? (int64_t)at * p.s.K + k0 + xc : 0);
         const int there = ok ? kn - xc : 0;
         rx[i] = p.wide_x ? get_chunk<T, true>(from, there) : get_chunk<T, false>(from, there);
       }
       if (has_v) {
-        const int64_t from = in ? (t.row + rb + i) * p.s.M + m0 + vc : 0;
+        const int64_t from = in ? (int64_t)(t.row + rb + i) * p.s.M + m0 + vc : 0;
         const int there = in ? mn - vc : 0;
         rv(i) = p.wide_y ? get_chunk<T, true>(vy + from, there) : get_chunk<T, false>(vy + from, there);
         if (ACT)
@@ -681,21 +895,27 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
     tc::fence_smem();
     tc::fence_before_sync();
     __syncthreads();
-    if (tid == 0) {
+    if (warp == 0) {
       tc::fence_after_sync();
+      const uint32_t leader = tc::elected();
       const uint64_t dx = tc::smem_desc(tc::smem_addr(s_x)), dv = tc::smem_desc(tc::smem_addr(s_v));
       const int steps = (cur.n + STEP - 1) / STEP;
-      for (int i = 0; i < steps; ++i) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= steps) break;
         const uint64_t at = 2 * i;
         const bool more = pending > 0 || i > 0;
         if (VTERMS == 2) {
-          tc::mma<Mma<T>::TF32>(tmem + NT, dx + at, dv + (VPANEL >> 4) + at, idesc, more);
-          if (XTERMS == 2)
-            tc::mma<Mma<T>::TF32>(tmem + NT, dx + (kPanel >> 4) + at, dv + at, idesc, true);
+          tc::mma<Mma<T>::TF32>(leader, tmem + NT, dx + at, dv + (VPANEL >> 4) + at, idesc, more);
+          if (XTERMS == 2) {
+            tc::mma<Mma<T>::TF32>(leader, tmem + NT, dx + (kPanel >> 4) + at, dv + at, idesc, true);
+            tc::mma<Mma<T>::TF32>(leader, tmem + NT, dx + (kPanel >> 4) + at, dv + (VPANEL >> 4) + at,
+                                  idesc, true);
+          }
         }
-        tc::mma<Mma<T>::TF32>(tmem, dx + at, dv + at, idesc, more);
+        tc::mma<Mma<T>::TF32>(leader, tmem, dx + at, dv + at, idesc, more);
       }
-      tc::commit(bar);
+      tc::commit(leader, bar);
     }
     ++pending;
     Run after = nxt;
@@ -809,7 +1029,9 @@ __global__ void __launch_bounds__(256) offsets_kernel(int64_t n, const int32_t* 
 // ------------------------------------------------------------------- host side
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-constexpr int kSmemMost = 227 * 1024 - 4096;  // dynamic, beside the static arrays
+// Dynamic shared memory of a CTA that has an SM to itself, beside its static
+// arrays.
+constexpr int kSmemMost = 227 * 1024 - 5120;
 
 // Lets a kernel use kSmemMost bytes on the current device; asked once for
 // each kernel (the instantiation is the kernel's own) and device.
@@ -828,46 +1050,92 @@ int allow_smem() {
   return GS_OK;
 }
 
-// CTAs of 256 threads that an SM holds, by shared memory and accumulator
-// columns (a CTA that found none free would wait for another to end).
-int per_sm(int smem, int columns, int by_registers) {
-  int n = 227 * 1024 / (smem + 4096);
-  n = n < 512 / columns ? n : 512 / columns;
-  n = n < by_registers ? n : by_registers;
-  return n < 1 ? 1 : n;
+// A map of rows [n, depth] in boxes of 128 rows x 128 bytes, swizzled as the
+// operands are; what lies outside reads as zeros.
+int make_map(CUtensorMap* map, const void* rows, int dtype, int64_t n, int depth) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                              const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (!encode) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) !=
+            cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      set_error("grouped_linear: no cuTensorMapEncodeTiled in this driver");
+      return GS_ERR_CUDA;
+    }
+    encode = reinterpret_cast<Encode>(f);
+  }
+  const cuuint64_t es = dtype == GS_F32 ? 4 : 2;
+  const cuuint64_t dims[2] = {(cuuint64_t)depth, (cuuint64_t)n}, pitch[1] = {depth * es};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), kTile}, ones[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == GS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == GS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (encode(map, type, 2, const_cast<void*>(rows), dims, pitch, box, ones,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) !=
+      CUDA_SUCCESS) {
+    set_error("grouped_linear: rows [%lld, %d] cannot be mapped", (long long)n, depth);
+    return GS_ERR_CUDA;
+  }
+  return GS_OK;
 }
 
-template <typename T, int ACT, int MODE, bool WIDE, bool SPLIT>
+template <typename T> constexpr int dtype_of = GS_F32;
+template <> constexpr int dtype_of<__nv_bfloat16> = GS_BF16;
+template <> constexpr int dtype_of<__half> = GS_F16;
+
+template <typename T, int ACT, int MODE, int LOAD, bool WIDE, bool SPLIT>
 int launch_rows(RowsArgs p, cudaStream_t st) {
-  using L = RowsLayout<T, SPLIT>;
-  constexpr auto kernel = rows_mma_kernel<T, ACT, MODE, WIDE, SPLIT>;
+  using L = RowsLayout<T, ACT, MODE, SPLIT>;
+  constexpr auto kernel = rows_mma_kernel<T, ACT, MODE, LOAD, WIDE, SPLIT>;
   if (int rc = allow_smem<kernel>()) return rc;
   p.panels = (int)ceil_div(p.depth, 128 / (int)sizeof(T));
   // The widest tile whose weights stay in shared memory: half the width
   // reads the rows twice, which costs less than staging the weights again
   // for every tile.
-  p.nt = p.width >= 128 ? 128 : (int)ceil_div(p.width, 32) * 32;
+  const int widest = p.width >= 128 ? 128 : (int)ceil_div(p.width, 32) * 32;
+  p.nt = widest;
+  p.slots = 2;
   p.resident = 1;
   while (L::smem(p) > kSmemMost && p.nt > 32) p.nt = (p.nt / 2 + 31) / 32 * 32;
-  if (L::smem(p) > kSmemMost) {
-    p.resident = 0;
-    p.nt = p.width >= 128 ? 128 : (int)ceil_div(p.width, 32) * 32;
+  if (L::smem(p) > kSmemMost) p.resident = 0, p.nt = widest;
+  // as many panels in flight as there is room for
+  while (p.slots < kSlotsMost) {
+    ++p.slots;
+    if (L::smem(p) > kSmemMost) {
+      --p.slots;
+      break;
+    }
   }
-  const int smem = L::smem(p), columns = L::columns(p.nt);
   const int64_t ny = ceil_div(p.width, p.nt);
   if (ny > 65535) return invalid("grouped_linear: too many features");
   const int64_t tiles = ceil_div(p.s.R, kTile);
-  int64_t nx = (int64_t)sm_count() * per_sm(smem, columns, 2) / ny;
+  int64_t nx = sm_count() / ny;
   nx = nx < 1 ? 1 : nx > tiles ? tiles : nx;
-  kernel<<<dim3((unsigned)nx, (unsigned)ny), kThreads, smem, st>>>(p, columns);
+  CUtensorMap map_a{}, map_y{};
+  if (LOAD == kTma) {
+    if (int rc = make_map(&map_a, p.a, dtype_of<T>, p.s.R, p.depth)) return rc;
+    if (L::kY)
+      if (int rc = make_map(&map_y, p.y, dtype_of<T>, p.s.R, p.depth)) return rc;
+  }
+  kernel<<<dim3((unsigned)nx, (unsigned)ny), 2 * kThreads, L::smem(p), st>>>(
+      p, L::columns(p.nt), map_a, map_y);
   return launch_status("grouped_linear");
 }
 
 template <typename T, int ACT, int MODE, bool SPLIT>
 int launch_rows(const RowsArgs& p, cudaStream_t st) {
   const bool wide = p.depth * sizeof(T) % 16 == 0 && on16(p.a) && (!p.y || on16(p.y));
-  return wide ? launch_rows<T, ACT, MODE, true, SPLIT>(p, st)
-              : launch_rows<T, ACT, MODE, false, SPLIT>(p, st);
+  if (!wide) return launch_rows<T, ACT, MODE, kCopy, false, SPLIT>(p, st);
+  if constexpr (MODE == kForward)
+    if (p.ids) return launch_rows<T, ACT, MODE, kCopy, true, SPLIT>(p, st);
+  return launch_rows<T, ACT, MODE, kTma, true, SPLIT>(p, st);
 }
 
 template <typename T, int ACT>

@@ -1,4 +1,4 @@
-// The few tcgen05 / mbarrier instructions that the grouped products use, and
+// The few tcgen05, TMA and mbarrier instructions that the grouped products use, and
 // the formats of their descriptors (PTX ISA, "tcgen05" and "matrix
 // descriptors").  Operands lie in shared memory K-major with the 128-byte
 // swizzle: row r of a panel is 128 bytes at r * 128, its 16-byte chunk c at
@@ -30,26 +30,39 @@ __device__ __forceinline__ uint32_t instr_desc(uint32_t format, uint32_t n) {
   return (1u << 4) | (format << 7) | (format << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+// One lane of the (converged) warp.  The whole warp runs the issuing code and
+// only the instructions themselves are predicated: with a branch around it
+// the descriptors, which the instruction takes from uniform registers, are
+// moved there one by one, which took longer than the multiplication.
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(p));
+  return p;
+}
+
 template <bool TF32>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                    bool accumulate) {
+__device__ __forceinline__ void mma(uint32_t leader, uint32_t d, uint64_t a, uint64_t b,
+                                    uint32_t idesc, bool accumulate) {
   const uint32_t acc = accumulate;
   if (TF32)
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader) : "memory");
   else
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader) : "memory");
 }
 
-// Arrives on the barrier once every MMA that this thread issued is done.
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               ::"r"(bar) : "memory");
+// Arrives on the barrier once every MMA that the leader issued is done.
+__device__ __forceinline__ void commit(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
+      ::"r"(bar), "r"(leader) : "memory");
 }
 
 __device__ __forceinline__ void fence_before_sync() {
@@ -90,7 +103,29 @@ __device__ __forceinline__ void load16(uint32_t taddr, float (&v)[16]) {
 
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_init_done() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Arrives, and has the phase wait for `bytes` of bulk copies.
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+// A box of a 2-D tensor map, from (x, row) on, to shared memory.
+__device__ __forceinline__ void load_box(uint32_t to, const void* map, int x, int row,
+                                         uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];"
+      ::"r"(to), "l"(map), "r"(x), "r"(row), "r"(bar) : "memory");
+}
+// A barrier of `threads` of the CTA's threads.
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 // Waits for the phase to end, up to `limit` polls of the hardware's own
@@ -104,23 +139,6 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t
         : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   } while (!done && limit-- > 0);
   return done != 0;
-}
-
-// x = hi + lo (+ 2^-22 |x| at most), both with the 11 significant bits of a
-// tf32 operand.  lo = 0 for what is not finite, so that hi alone says what x
-// is; a value whose rounding would overflow is cut instead.
-__device__ __forceinline__ float round_tf32(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return __uint_as_float(r);
-}
-__device__ __forceinline__ void split_tf32(float x, float& hi, float& lo) {
-  hi = round_tf32(x);
-  if (!(fabsf(hi) < INFINITY)) {
-    if (fabsf(x) < INFINITY) hi = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
-    else { lo = 0.0f; return; }
-  }
-  lo = round_tf32(x - hi);
 }
 
 }  // namespace tc

@@ -171,7 +171,10 @@ def test_non_finite_values(gs, cuda, dtype, K, M):
     inf = torch.isinf(want)
     assert torch.equal(got[inf], want[inf])
     assert bool(torch.isfinite(got[fine]).all())
-    assert torch.allclose(got[200], want[200], rtol=4 * half_step(dt), atol=0)
+    # one product: fp32 factors are carried to 2^-22 of themselves each, which
+    # is 8 half steps of 2^-24, and the two partial sums and their join take a
+    # rounding of up to a step each; 16-bit ones are exact up to the last
+    assert torch.allclose(got[200], want[200], rtol=(8 + 6) * half_step(dt), atol=0)
     # the backward: a NaN row of v_y stays in its row of v_x, its column of v_weights
     c, v_y = _case([300, 200], 0, K, M, dt, bias=True)
     y = grouped_linear_forward(c)
