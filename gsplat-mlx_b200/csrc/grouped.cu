@@ -276,23 +276,20 @@ __device__ __forceinline__ void arrived(int n) {
 // out[row] = f(rows a, weights of the row's group): the forward, and v_x.
 //
 // One CTA an SM streams consecutive 128-row tiles, a panel (128 bytes of
-// depth) at a time, through a ring of `slots` panels.  Its front half (8
-// warps) has the panels filled -- TMA: rows that lie together; asynchronous
-// 16- or 4-byte copies: gathered rows and fp32 rows off the boundary --,
-// makes operands of them, and issues the MMAs; its back half takes a tile's
-// accumulator while the front is at the next tile's.  16-bit rows are
-// multiplied as they arrive; of fp32 rows the tensor core reads the upper
+// depth) at a time, through a ring of `slots` panels.  One warp has the
+// panels filled by TMA where rows lie together; gathered rows, and fp32 rows
+// off the boundary, the eight front warps copy asynchronously.  These make
+// operands of the panels, another warp issues the MMAs, and the eight back
+// warps take a tile's accumulator while the next tile's is made.  16-bit rows
+// are multiplied as they arrive; of fp32 rows the tensor core reads the upper
 // part itself (it ignores the 13 low bits) and the low part is written beside;
 // the backward through an activation rewrites the panel as v_z.  The group's
 // weights are staged once per group, and stay.
 //
-// Front and back run one after the other in an earlier form (two CTAs an SM,
-// 128-128 bf16, 2 M rows): 211 us; a tile took 1900 cycles a panel and 2300 for
-// its results.
 enum { kTma, kCopy };  // how rows arrive
 
 template <typename T, int ACT, int MODE, int LOAD, bool WIDE, bool SPLIT>
-__global__ void __launch_bounds__(2 * kThreads, 1)
+__global__ void __launch_bounds__(2 * kThreads + 64, 1)
     rows_mma_kernel(RowsArgs p, int columns, const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_y) {
   using L = RowsLayout<T, ACT, MODE, SPLIT>;
@@ -301,7 +298,7 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
   constexpr int STEP = 32 / sizeof(T);  // depth of an MMA
   constexpr bool BACK = MODE != kForward;
   extern __shared__ char smem_raw[];
-  __shared__ uint64_t s_bars[2 * kSlotsMost + 4];
+  __shared__ uint64_t s_bars[3 * kSlotsMost + 5];
   __shared__ uint32_t s_tmem;
   __shared__ __align__(16) float s_bias[8][kTile];
   char* const s_low = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
@@ -312,8 +309,10 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
   const uint32_t bar0 = tc::smem_addr(s_bars);
   auto full = [&](int i) { return bar0 + 8 * i; };                       // a slot has its rows
   auto free_ = [&](int i) { return bar0 + 8 * (kSlotsMost + i); };       // its MMAs are done
-  auto made = [&](int i) { return bar0 + 8 * (2 * kSlotsMost + i); };    // an accumulator is
-  auto taken = [&](int i) { return bar0 + 8 * (2 * kSlotsMost + 2 + i); };
+  auto ready = [&](int i) { return bar0 + 8 * (2 * kSlotsMost + i); };   // it has operands
+  auto made = [&](int i) { return bar0 + 8 * (3 * kSlotsMost + i); };    // an accumulator is
+  auto taken = [&](int i) { return bar0 + 8 * (3 * kSlotsMost + 2 + i); };
+  const uint32_t weighed = bar0 + 8 * (3 * kSlotsMost + 4);              // the weights are there
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be uniform
   const int n0 = blockIdx.y * p.nt;
@@ -325,7 +324,9 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
     for (int i = 0; i < p.slots; ++i) {
       tc::bar_init(full(i), 1);
       tc::bar_init(free_(i), 1);
+      tc::bar_init(ready(i), 8);
     }
+    tc::bar_init(weighed, 8);
     for (int i = 0; i < 2; ++i) {
       tc::bar_init(made(i), 1);
       tc::bar_init(taken(i), 8);
@@ -351,36 +352,100 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
   none.n = 0, none.g = -1, none.group_end = 0;
   auto after = [&](const Run& t) { return run_from(p.off, p.s.G, t.row + t.n, end, kTile, t); };
 
-  if (warp < 8) {
-    // ------------------------------------------------------------ front half
+  auto after_live = [&](Run t) {  // rows outside every group are the back's alone
+    t = after(t);
+    while (t.n > 0 && (t.g < 0 || t.g >= p.s.G)) {
+      t.n = t.group_end - t.row;
+      t = after(t);
+    }
+    return t;
+  };
+  auto steps_of = [&](int j) { return (min(DP, p.depth - j * DP) + STEP - 1) / STEP; };
+  // the slot of the panel `back` panels before the one in `slot`
+  auto slot_before = [&](int slot, int back) {
+    return slot >= back ? slot - back : slot + p.slots - back;
+  };
+  // the front makes operands of the panels; else they are multiplied as they are
+  constexpr bool kWork = LOAD == kCopy || L::kTerms == 2 || L::kY;
+
+  if (warp == 17) {
+    // ------------------------------------------------------------- TMA
+    if (LOAD == kTma) {
+      int slot = 0, q = 0;
+      for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
+        for (int j = 0; j < p.panels; ++j, ++q) {
+          if (q >= p.slots) wait(free_(slot), q / p.slots - 1);
+          if (tc::elected()) {
+            const uint32_t to = tc::smem_addr(s_rows + slot * kPanel);
+            tc::expect(full(slot), kPanel * (L::kY ? 2 : 1));
+            tc::load_box(to, &map_a, j * DP, cur.row, full(slot));
+            if (L::kY) tc::load_box(to + p.slots * kPanel, &map_y, j * DP, cur.row, full(slot));
+          }
+          __syncwarp();
+          slot = slot + 1 == p.slots ? 0 : slot + 1;
+        }
+    }
+  } else if (warp == 16) {
+    // ------------------------------------------------------------- MMAs
+    const uint32_t idesc = tc::instr_desc(Mma<T>::format, (cols + 15) / 16 * 16);
+    const uint32_t leader = tc::elected();
+    int staged = -1, stagings = 0, slot = 0, q = 0, t = 0;
+    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur), ++t) {
+      for (int j = 0; j < p.panels; ++j, ++q) {
+        if (cur.g != staged || !p.resident) wait(weighed, stagings++);
+        staged = cur.g;
+        wait(kWork ? ready(slot) : full(slot), q / p.slots);
+        if (j == 0 && t > 1) wait(taken(t & 1), (t >> 1) - 1);
+        tc::fence_after_sync();
+        const int steps = steps_of(j);
+        const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms;
+        const uint64_t da = tc::smem_desc(tc::smem_addr(s_rows + slot * kPanel));
+        const uint64_t dl = tc::smem_desc(
+            tc::smem_addr(L::kY ? s_y + slot * kPanel : s_low + (q & 1) * kPanel));
+        const uint64_t dw =
+            tc::smem_desc(tc::smem_addr(s_w + (p.resident ? j : 0) * L::kWTerms * wbytes));
+        const uint64_t lo_w = wbytes >> 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i >= steps) break;
+          const uint64_t step = 2 * i;  // 32 bytes
+          const bool more = j > 0 || i > 0;
+          if (L::kTerms == 2) {
+            tc::mma<Mma<T>::TF32>(leader, acc + p.nt, dl + step, dw + step, idesc, more);
+            if (L::kWTerms == 2) {
+              tc::mma<Mma<T>::TF32>(leader, acc + p.nt, da + step, dw + lo_w + step, idesc, true);
+              tc::mma<Mma<T>::TF32>(leader, acc + p.nt, dl + step, dw + lo_w + step, idesc, true);
+            }
+          }
+          tc::mma<Mma<T>::TF32>(leader, acc, da + step, dw + step, idesc, more);
+        }
+        tc::commit(leader, free_(slot));
+        if (j + 1 == p.panels) tc::commit(leader, made(t & 1));
+        slot = slot + 1 == p.slots ? 0 : slot + 1;
+      }
+    }
+    // every MMA is done before the memory goes
+    if (q > 0) wait(free_(slot_before(slot, 1)), (q - 1) / p.slots);
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ front warps
     const int tid = threadIdx.x;
     const T* const a = static_cast<const T*>(p.a);
     const T* const y = static_cast<const T*>(p.y);
     const T* const w = static_cast<const T*>(p.w);
-    const uint32_t idesc = tc::instr_desc(Mma<T>::format, (cols + 15) / 16 * 16);
-    auto after_live = [&](Run t) {  // rows outside every group are not the front's
-      t = after(t);
-      while (t.n > 0 && (t.g < 0 || t.g >= p.s.G)) {
-        t.n = t.group_end - t.row;
-        t = after(t);
-      }
-      return t;
-    };
-    auto steps_of = [&](int j) { return (min(DP, p.depth - j * DP) + STEP - 1) / STEP; };
     const int c16 = tid & 7, r16 = tid >> 3;  // this thread's chunk, and its rows r16 + 32 i
     const uint32_t o16 = chunk_at(r16, c16);  // + 4096 i in a panel
 
-    // The panel that is sent next: panel ahead_j of the tile `ahead`, number
-    // `ahead_q` of the CTA's, into slot `ahead_s`.
-    Run ahead = after_live(none), behind = ahead;
-    int ahead_j = 0, ahead_q = 0, ahead_s = 0;
+    // The panel that is copied next: panel ahead_j of the tile `ahead`, into
+    // slot `ahead_s`.
+    Run ahead = none, behind = none;
+    int ahead_j = 0, ahead_s = 0;
     int at[4], id[4];  // rows of x, gathered: validated, and as read for the tile after
     auto read_ids = [&](const Run& t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         id[i] = p.ids && !BACK && r16 + 32 * i < t.n ? __ldg(p.ids + t.row + r16 + 32 * i) : -1;
     };
-    auto settle = [&]() {  // of the tile that is sent now
+    auto settle = [&]() {  // of the tile that is copied now
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = r16 + 32 * i;
@@ -388,58 +453,31 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
         else at[i] = row < ahead.n ? ahead.row + row : -1;
       }
     };
-    if (LOAD == kCopy) {
-      read_ids(ahead);
-      settle();
-      behind = after_live(ahead);
-      read_ids(behind);
-    }
     auto send = [&]() {
       if (ahead.n > 0) {
-        if (LOAD == kTma) {
-          if (warp == 1) {
-            // the slot's former panel is done with
-            if (ahead_q >= p.slots) wait(free_(ahead_s), ahead_q / p.slots - 1);
-            if (tc::elected()) {
-              const uint32_t to = tc::smem_addr(s_rows + ahead_s * kPanel);
-              tc::expect(full(ahead_s), kPanel * (L::kY ? 2 : 1));
-              tc::load_box(to, &map_a, ahead_j * DP, ahead.row, full(ahead_s));
-              if (L::kY)
-                tc::load_box(to + p.slots * kPanel, &map_y, ahead_j * DP, ahead.row, full(ahead_s));
-            }
-            __syncwarp();
-          }
-        } else {
-          if (ahead_q >= p.slots) wait(free_(ahead_s), ahead_q / p.slots - 1);
-          if (c16 < 2 * steps_of(ahead_j)) {
-            const int d = ahead_j * DP + c16 * E;
-            const uint32_t to = ahead_s * kPanel + o16;
-            const T* const ad = a + d;
-            const T* const yd = L::kY ? y + d : nullptr;
+        if (c16 < 2 * steps_of(ahead_j)) {
+          const int d = ahead_j * DP + c16 * E;
+          const uint32_t to = ahead_s * kPanel + o16;
+          const T* const ad = a + d;
+          const T* const yd = L::kY ? y + d : nullptr;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int there = at[i] >= 0 ? p.depth - d : 0;
-              const int64_t from = (int64_t)at[i] * p.depth;
-              send_chunk<T, WIDE>(s_rows + to + 4096 * i, ad + from, there);
-              if (L::kY) send_chunk<T, WIDE>(s_y + to + 4096 * i, yd + from, there);
-            }
+          for (int i = 0; i < 4; ++i) {
+            const int there = at[i] >= 0 ? p.depth - d : 0;
+            const int64_t from = (int64_t)at[i] * p.depth;
+            send_chunk<T, WIDE>(s_rows + to + 4096 * i, ad + from, there);
+            if (L::kY) send_chunk<T, WIDE>(s_y + to + 4096 * i, yd + from, there);
           }
         }
-        ++ahead_q;
         ahead_s = ahead_s + 1 == p.slots ? 0 : ahead_s + 1;
         if (++ahead_j == p.panels) {
           ahead_j = 0;
-          if (LOAD == kCopy) {
-            ahead = behind;
-            settle();
-            behind = after_live(ahead);
-            read_ids(behind);
-          } else {
-            ahead = after_live(ahead);
-          }
+          ahead = behind;
+          settle();
+          behind = after_live(ahead);
+          read_ids(behind);
         }
       }
-      if (LOAD == kCopy) send_done();  // also where nothing is left, to keep the count
+      send_done();  // also where nothing is left, to keep the count
     };
 
     // weight panels [j0, j1) of group g: rows n (columns of the result) x depth
@@ -482,31 +520,48 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
       }
     };
 
-    for (int i = 1; i < p.slots; ++i) send();
-    int staged = -1, slot = 0, q = 0, t = 0;
-    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur), ++t) {
-      if (cur.g != staged) {
+    // A slot is filled again `lag` panels after its own, when its MMAs are
+    // long done.
+    const int lag = p.slots > 2 ? 2 : 1;
+    if (LOAD == kCopy) {
+      ahead = after_live(none);
+      read_ids(ahead);
+      settle();
+      behind = after_live(ahead);
+      read_ids(behind);
+      for (int i = lag; i < p.slots; ++i) send();
+    }
+    int staged = -1, slot = 0, q = 0;
+    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur)) {
+      if (cur.g != staged && p.resident) {
         // every MMA of the group before is done
-        if (q > 0) wait(free_(slot == 0 ? p.slots - 1 : slot - 1), (q - 1) / p.slots);
-        if (p.resident) stage_weights(cur.g, 0, p.panels);
+        if (q > 0) wait(free_(slot_before(slot, 1)), (q - 1) / p.slots);
+        stage_weights(cur.g, 0, p.panels);
+        tc::fence_smem();
+        __syncwarp();
+        if (lane == 0) tc::arrive(weighed);
         staged = cur.g;
       }
       for (int j = 0; j < p.panels; ++j, ++q) {
-        const int steps = steps_of(j);
-        char* const here = s_rows + slot * kPanel;
-        char* const low = L::kY ? s_y + slot * kPanel : s_low + (q & 1) * kPanel;
-        if (LOAD == kCopy) arrived(p.slots - 2);
-        else wait(full(slot), q / p.slots);
         if (!p.resident) {
-          if (q > 0) wait(free_(slot == 0 ? p.slots - 1 : slot - 1), (q - 1) / p.slots);
+          if (q > 0) wait(free_(slot_before(slot, 1)), (q - 1) / p.slots);
           stage_weights(cur.g, j, j + 1);
+          tc::fence_smem();
+          __syncwarp();
+          if (lane == 0) tc::arrive(weighed);
         }
-        if (L::kTerms == 2 || L::kY) {
-          if (L::kLow && q > 1) {  // the low parts of two panels ago are done with
-            const int before = slot > 1 ? slot - 2 : slot + p.slots - 2;
-            wait(free_(before), (q - 2) / p.slots);
+        if (kWork) {
+          // the panel `lag` before is done with: its slot, and its low parts
+          if (q >= lag) wait(free_(slot_before(slot, lag)), (q - lag) / p.slots);
+          if (LOAD == kCopy) {
+            send();
+            arrived(p.slots - lag);
+          } else {
+            wait(full(slot), q / p.slots);
           }
-          if (c16 < 2 * steps) {
+          if ((L::kTerms == 2 || L::kY) && c16 < 2 * steps_of(j)) {
+            char* const here = s_rows + slot * kPanel;
+            char* const low = L::kY ? s_y + slot * kPanel : s_low + (q & 1) * kPanel;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const uint32_t o = o16 + 4096 * i;
@@ -524,45 +579,20 @@ __global__ void __launch_bounds__(2 * kThreads, 1)
               }
             }
           }
+          tc::fence_smem();
+          __syncwarp();
+          if (lane == 0) tc::arrive(ready(slot));
+        } else {
+          // keeps pace: a barrier says whether its last phase is over, not
+          // which one that is
+          wait(free_(slot), q / p.slots);
         }
-        tc::fence_smem();
-        tc::bar_sync(1, kThreads);
-        if (warp == 0) {
-          if (j == 0 && t > 1) wait(taken(t & 1), (t >> 1) - 1);
-          tc::fence_after_sync();
-          const uint32_t leader = tc::elected();
-          const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms;
-          const uint64_t da = tc::smem_desc(tc::smem_addr(here));
-          const uint64_t dl = tc::smem_desc(tc::smem_addr(low));
-          const uint64_t dw =
-              tc::smem_desc(tc::smem_addr(s_w + (p.resident ? j : 0) * L::kWTerms * wbytes));
-          const uint64_t lo_w = wbytes >> 4;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (i >= steps) break;
-            const uint64_t step = 2 * i;  // 32 bytes
-            const bool more = j > 0 || i > 0;
-            if (L::kTerms == 2) {
-              tc::mma<Mma<T>::TF32>(leader, acc + p.nt, dl + step, dw + step, idesc, more);
-              if (L::kWTerms == 2) {
-                tc::mma<Mma<T>::TF32>(leader, acc + p.nt, da + step, dw + lo_w + step, idesc, true);
-                tc::mma<Mma<T>::TF32>(leader, acc + p.nt, dl + step, dw + lo_w + step, idesc, true);
-              }
-            }
-            tc::mma<Mma<T>::TF32>(leader, acc, da + step, dw + step, idesc, more);
-          }
-          tc::commit(leader, free_(slot));
-          if (j + 1 == p.panels) tc::commit(leader, made(t & 1));
-        }
-        send();
         slot = slot + 1 == p.slots ? 0 : slot + 1;
       }
     }
     if (LOAD == kCopy) arrived(0);
-    // every MMA is done before the memory goes
-    if (q > 0) wait(free_(slot == 0 ? p.slots - 1 : slot - 1), (q - 1) / p.slots);
   } else {
-    // ------------------------------------------------------------- back half
+    // ------------------------------------------------------------- back warps
     const T* const bias = static_cast<const T*>(p.bias);
     const int bw = warp - 8, row0 = (bw & 3) * 32;  // lanes of the accumulator
     float* const my_bias = s_bias[bw];
@@ -1124,7 +1154,7 @@ int launch_rows(RowsArgs p, cudaStream_t st) {
     if (L::kY)
       if (int rc = make_map(&map_y, p.y, dtype_of<T>, p.s.R, p.depth)) return rc;
   }
-  kernel<<<dim3((unsigned)nx, (unsigned)ny), 2 * kThreads, L::smem(p), st>>>(
+  kernel<<<dim3((unsigned)nx, (unsigned)ny), 2 * kThreads + 64, L::smem(p), st>>>(
       p, L::columns(p.nt), map_a, map_y);
   return launch_status("grouped_linear");
 }
