@@ -273,6 +273,112 @@ __device__ __forceinline__ void arrived(int n) {
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
+// A warp's 32 lanes of an accumulator (columns of its half), 64 bytes of
+// results at a time: through `stage`, the warp's own 2 KB of shared memory, and
+// in pieces of rows to `out_rows`.  into: the row that lane's row is added to
+// (kScatter).  A tile that is not live gives zeros.
+template <typename T, int ACT, int MODE, int TERMS>
+__device__ __forceinline__ void take_results(bool live, uint32_t acc, int second, int half,
+                                             int rows, int cols, const float* my_bias, int into,
+                                             char* stage, void* out_rows, int row, int pitch,
+                                             int n0, int wide_out) {
+  constexpr bool BACK = MODE != kForward;
+  constexpr int OB = MODE == kScatter ? 4 : sizeof(T);  // bytes of a result
+  constexpr int OE = 16 / OB, SC = 64 / OB;             // results in 16 and in 64 bytes
+  const int lane = threadIdx.x & 31;
+  auto stage_at = [&](int r, int c) { return stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4); };
+  for (int c0 = half * SC; c0 < cols; c0 += 2 * SC) {
+    const int width = min(SC, cols - c0);  // columns here
+#pragma unroll
+    for (int h = 0; h < SC / 16; ++h) {
+      if (h * 16 >= width) break;
+      float v[16];
+      if (live) {
+        tc::load16(acc + c0 + h * 16, v);
+        if (TERMS == 2) {
+          float u[16];
+          tc::load16(acc + second + c0 + h * 16, u);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+        }
+      }
+      if (!live) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+      } else if (!BACK) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (ACT == GS_ACT_SIGMOID && h * 16 + k * 4 >= width) break;  // 20 instructions each
+          const float4 b = *reinterpret_cast<const float4*>(my_bias + c0 + h * 16 + k * 4);
+          v[k * 4] = activate<ACT>(v[k * 4] + b.x);
+          v[k * 4 + 1] = activate<ACT>(v[k * 4 + 1] + b.y);
+          v[k * 4 + 2] = activate<ACT>(v[k * 4 + 2] + b.z);
+          v[k * 4 + 3] = activate<ACT>(v[k * 4 + 3] + b.w);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 16 / OE; ++c) {
+        char* const to = stage_at(lane, h * (16 / OE) + c);
+        if constexpr (OB == 4)
+          *reinterpret_cast<float4*>(to) =
+              make_float4(v[c * OE], v[c * OE + 1], v[c * OE + 2], v[c * OE + 3]);
+        else
+          *reinterpret_cast<uint4*>(to) = round_chunk<T>(v + c * OE);
+      }
+    }
+    __syncwarp();
+    const int c = lane & 3;
+    if constexpr (MODE == kScatter) {
+      float* const sum = static_cast<float*>(out_rows);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = (lane >> 2) + 8 * i;
+        const int32_t to_row = __shfl_sync(0xffffffffu, into, r);
+        if (to_row < 0 || c * 4 >= width) continue;
+        float* const to = sum + (int64_t)to_row * pitch + n0 + c0 + c * 4;
+        const float4 v = *reinterpret_cast<const float4*>(stage_at(r, c));
+        if (wide_out) {
+          asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
+                       ::"l"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+        } else {
+          atomicAdd(to, v.x);
+          if (c * 4 + 1 < width) atomicAdd(to + 1, v.y);
+          if (c * 4 + 2 < width) atomicAdd(to + 2, v.z);
+          if (c * 4 + 3 < width) atomicAdd(to + 3, v.w);
+        }
+      }
+    } else {
+      T* const out = static_cast<T*>(out_rows) + (int64_t)row * pitch + n0 + c0;
+      if (wide_out) {
+        if (c * OE < width) {
+          T* to = out + (int64_t)(lane >> 2) * pitch + c * OE;
+          const int64_t down = (int64_t)8 * pitch;
+#pragma unroll
+          for (int i = 0; i < 4; ++i, to += down)
+            if ((lane >> 2) + 8 * i < rows)
+              *reinterpret_cast<uint4*>(to) =
+                  *reinterpret_cast<const uint4*>(stage_at((lane >> 2) + 8 * i, c));
+        }
+      } else if (pitch <= SC) {  // whole rows: one run of memory
+        const int total = rows * width;
+        for (int i = lane; i < total; i += 32) {
+          const int r = i / width, e = i - r * width;
+          out[i] = reinterpret_cast<const T*>(stage_at(r, e / OE))[e % OE];
+        }
+      } else {
+        constexpr int LR = 32 / SC;  // rows that the lanes cover
+        const int e = lane & (SC - 1);
+        if (e < width)
+          for (int r = lane / SC; r < rows; r += LR)
+            out[(int64_t)r * pitch + e] =
+                reinterpret_cast<const T*>(stage_at(r, e / OE))[e % OE];
+      }
+    }
+    __syncwarp();
+  }
+}
+
 // out[row] = f(rows a, weights of the row's group): the forward, and v_x.
 //
 // One CTA an SM streams consecutive 128-row tiles, a panel (128 bytes of
@@ -597,13 +703,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     const int bw = warp - 8, row0 = (bw & 3) * 32;  // lanes of the accumulator
     float* const my_bias = s_bias[bw];
     int biased = -1, t = 0;
-    // 32 rows x 64 bytes at a time: out of the accumulator, through the warp's
-    // own piece of shared memory, and in pieces of rows to `out`
-    constexpr int OB = MODE == kScatter ? 4 : sizeof(T);  // bytes of a result
-    constexpr int OE = 16 / OB, SC = 64 / OB;             // results in 16 and in 64 bytes
-    char* const stage = s_stage + bw * 2048;
-    auto stage_at = [&](int r, int c) { return stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4); };
-
     for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
       const bool live = cur.g >= 0 && cur.g < p.s.G;
       const int rows = min(32, cur.n - row0);
@@ -622,96 +721,10 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         tc::fence_after_sync();
       }
       if (into >= p.s.n) into = -1;
-      for (int c0 = (bw >> 2) * SC; c0 < cols; c0 += 2 * SC) {
-        const int width = min(SC, cols - c0);  // columns here
-#pragma unroll
-        for (int h = 0; h < SC / 16; ++h) {
-          if (h * 16 >= width) break;
-          float v[16];
-          if (live) {
-            tc::load16(acc + c0 + h * 16, v);
-            if (L::kTerms == 2) {
-              float u[16];
-              tc::load16(acc + p.nt + c0 + h * 16, u);
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (fabsf(v[i]) < INFINITY) v[i] += u[i];
-            }
-          }
-          if (!live) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-          } else if (!BACK) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (ACT == GS_ACT_SIGMOID && h * 16 + k * 4 >= width) break;  // 20 instructions each
-              const float4 b = *reinterpret_cast<const float4*>(my_bias + c0 + h * 16 + k * 4);
-              v[k * 4] = activate<ACT>(v[k * 4] + b.x);
-              v[k * 4 + 1] = activate<ACT>(v[k * 4 + 1] + b.y);
-              v[k * 4 + 2] = activate<ACT>(v[k * 4 + 2] + b.z);
-              v[k * 4 + 3] = activate<ACT>(v[k * 4 + 3] + b.w);
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < 16 / OE; ++c) {
-            char* const to = stage_at(lane, h * (16 / OE) + c);
-            if constexpr (OB == 4)
-              *reinterpret_cast<float4*>(to) =
-                  make_float4(v[c * OE], v[c * OE + 1], v[c * OE + 2], v[c * OE + 3]);
-            else
-              *reinterpret_cast<uint4*>(to) = round_chunk<T>(v + c * OE);
-          }
-        }
-        __syncwarp();
-        const int c = lane & 3;
-        if constexpr (MODE == kScatter) {
-          float* const sum = static_cast<float*>(p.out);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = (lane >> 2) + 8 * i;
-            const int32_t to_row = __shfl_sync(0xffffffffu, into, r);
-            if (to_row < 0 || c * 4 >= width) continue;
-            float* const to = sum + (int64_t)to_row * p.width + n0 + c0 + c * 4;
-            const float4 v = *reinterpret_cast<const float4*>(stage_at(r, c));
-            if (p.wide_out) {
-              asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
-                           ::"l"(to), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
-            } else {
-              atomicAdd(to, v.x);
-              if (c * 4 + 1 < width) atomicAdd(to + 1, v.y);
-              if (c * 4 + 2 < width) atomicAdd(to + 2, v.z);
-              if (c * 4 + 3 < width) atomicAdd(to + 3, v.w);
-            }
-          }
-        } else {
-          T* const out = static_cast<T*>(p.out) + (int64_t)(cur.row + row0) * p.width + n0 + c0;
-          if (p.wide_out) {
-            if (c * OE < width) {
-              T* to = out + (int64_t)(lane >> 2) * p.width + c * OE;
-              const int64_t down = (int64_t)8 * p.width;
-#pragma unroll
-              for (int i = 0; i < 4; ++i, to += down)
-                if ((lane >> 2) + 8 * i < rows)
-                  *reinterpret_cast<uint4*>(to) =
-                      *reinterpret_cast<const uint4*>(stage_at((lane >> 2) + 8 * i, c));
-            }
-          } else if (p.width <= SC) {  // whole rows: one run of memory
-            const int total = rows * width;
-            for (int i = lane; i < total; i += 32) {
-              const int r = i / width, e = i - r * width;
-              out[i] = reinterpret_cast<const T*>(stage_at(r, e / OE))[e % OE];
-            }
-          } else {
-            constexpr int LR = 32 / SC;  // rows that the lanes cover
-            const int e = lane & (SC - 1);
-            if (e < width)
-              for (int r = lane / SC; r < rows; r += LR)
-                out[(int64_t)r * p.width + e] =
-                    reinterpret_cast<const T*>(stage_at(r, e / OE))[e % OE];
-          }
-        }
-        __syncwarp();
-      }
+      take_results<T, ACT, MODE, L::kTerms>(live, acc, p.nt, bw >> 2, rows, cols, my_bias, into,
+                                            s_stage + bw * 2048, p.out,
+                                            BACK && MODE == kScatter ? 0 : cur.row + row0, p.width,
+                                            n0, p.wide_out);
       if (live) {
         tc::fence_before_sync();
         __syncwarp();
@@ -1000,6 +1013,402 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
   if (warp == 0) tc::dealloc(tmem, columns);
 }
 
+// ------------------------------------------------- the whole backward, 16 bits
+struct BothArgs {
+  Shape s;
+  const void* x;
+  const int32_t* ids;
+  const int32_t* off;
+  const void* w;
+  void* vx;          // v_x, its fp32 sums with SHARED, or NULL: not wanted
+  float* part;       // as in WeightArgs
+  int pk, pm;        // panels (64 columns) of K and M: 1 or 2
+  int slots, ys;     // tiles of v_y and x, and of y, in shared memory
+  int biases;
+};
+
+// Rows of K and M of up to 128 features, on 16-byte boundaries: v_y, y and x
+// are read once for v_x, v_W and v_b together.  A tile is 128 rows; v_y's
+// panels are rewritten as v_z and multiplied twice from where they lie: with
+// rows as lanes and the weights (v_x), and with rows as depth and x (v_W: both
+// operands are "MN-major" then, as the weights are in the first product), so
+// nothing is transposed.  The roles of the warps are those of the rows kernel.
+//
+// v_W's accumulator is added to the CTA's place in `part` at the end of a
+// group, and every kPiece tiles: the tensor core cuts sums to fp32 instead of
+// rounding them, 2^-24 of the sum at each of a tile's 8 additions.
+constexpr int kPiece = 32;
+
+template <typename T, int ACT, bool SHARED>
+__global__ void __launch_bounds__(2 * kThreads + 64, 1)
+    both_mma_kernel(BothArgs p, int columns, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ CUtensorMap map_y,
+                    const __grid_constant__ CUtensorMap map_x) {
+  constexpr int TERMS = ACT == GS_ACT_SIGMOID ? 2 : 1;  // parts of v_z
+  constexpr int NBUF = TERMS == 2 ? 1 : 2;              // accumulators of v_x
+  constexpr bool HAS_Y = ACT != GS_ACT_NONE;
+  extern __shared__ char smem_raw[];
+  __shared__ uint64_t s_bars[3 * 4 + 2 * 4 + 2 * 2 + 3];
+  __shared__ uint32_t s_tmem;
+  __shared__ float s_db[8][128];
+  const int lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int K = p.s.K, M = p.s.M;
+  const int nk = (K + 31) / 32 * 32, nm = (M + 31) / 32 * 32;
+  const int tile_bytes = (p.pm + p.pk) * kPanel;
+  char* const s_stage = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
+  char* const s_w = s_stage + 8 * 2048;
+  char* const s_tiles = s_w + p.pk * kPanel;   // v_z's panels, then x's
+  char* const s_y = s_tiles + p.slots * tile_bytes;
+  const uint32_t bar0 = tc::smem_addr(s_bars);
+  auto full = [&](int i) { return bar0 + 8 * i; };
+  auto free_ = [&](int i) { return bar0 + 8 * (4 + i); };
+  auto ready = [&](int i) { return bar0 + 8 * (8 + i); };
+  auto y_full = [&](int i) { return bar0 + 8 * (12 + i); };
+  auto y_free = [&](int i) { return bar0 + 8 * (16 + i); };
+  auto made = [&](int i) { return bar0 + 8 * (20 + i); };
+  auto taken = [&](int i) { return bar0 + 8 * (22 + i); };
+  const uint32_t weighed = bar0 + 8 * 24, sum_made = bar0 + 8 * 25, sum_taken = bar0 + 8 * 26;
+
+  if (warp == 0) tc::alloc(&s_tmem, columns);
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < 4; ++i) {
+      tc::bar_init(full(i), 1);
+      tc::bar_init(free_(i), 1);
+      tc::bar_init(ready(i), 8);
+      tc::bar_init(y_full(i), 1);
+      tc::bar_init(y_free(i), TERMS == 2 ? 1 : 8);  // the low parts of v_z lie there
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::bar_init(made(i), 1);
+      tc::bar_init(taken(i), 8);
+    }
+    tc::bar_init(weighed, 8);
+    tc::bar_init(sum_made, 1);
+    tc::bar_init(sum_taken, 8);
+    tc::bar_init_done();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = s_tmem, sum_acc = tmem + NBUF * TERMS * nk;
+  uint32_t limit = kWaitLimit;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (!tc::bar_wait(bar, parity & 1, limit)) {
+      limit = 0;
+      g_wait_gave_up = 1;
+    }
+  };
+
+  const int64_t tiles = (p.s.R + kTile - 1) / kTile;
+  const int end = (int)min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
+  Run none;
+  none.row = (int)(first_tile(tiles, gridDim.x, blockIdx.x) * kTile);
+  none.n = 0, none.g = -1, none.group_end = 0;
+  auto after = [&](const Run& t) { return run_from(p.off, p.s.G, t.row + t.n, end, kTile, t); };
+  auto after_live = [&](Run t) {
+    t = after(t);
+    while (t.n > 0 && (t.g < 0 || t.g >= p.s.G)) {
+      t.n = t.group_end - t.row;
+      t = after(t);
+    }
+    return t;
+  };
+
+  if (warp == 17) {
+    // ------------------------------------------------------------- TMA
+    int slot = 0, ys = 0, t = 0;
+    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur), ++t) {
+      if (t >= p.slots) wait(free_(slot), t / p.slots - 1);
+      if (tc::elected()) {
+        const uint32_t to = tc::smem_addr(s_tiles + slot * tile_bytes);
+        tc::expect(full(slot), SHARED ? p.pm * kPanel : tile_bytes);
+        for (int j = 0; j < p.pm; ++j)
+          tc::load_box(to + j * kPanel, &map_v, j * 64, cur.row, full(slot));
+        if (!SHARED)
+          for (int j = 0; j < p.pk; ++j)
+            tc::load_box(to + (p.pm + j) * kPanel, &map_x, j * 64, cur.row, full(slot));
+      }
+      __syncwarp();
+      if (HAS_Y) {
+        if (t >= p.ys) wait(y_free(ys), t / p.ys - 1);
+        if (tc::elected()) {
+          const uint32_t to = tc::smem_addr(s_y + ys * p.pm * kPanel);
+          tc::expect(y_full(ys), p.pm * kPanel);
+          for (int j = 0; j < p.pm; ++j)
+            tc::load_box(to + j * kPanel, &map_y, j * 64, cur.row, y_full(ys));
+        }
+        __syncwarp();
+      }
+      slot = slot + 1 == p.slots ? 0 : slot + 1;
+      ys = ys + 1 == p.ys ? 0 : ys + 1;
+    }
+  } else if (warp == 16) {
+    // ------------------------------------------------------------- MMAs
+    const uint32_t by_rows = tc::instr_desc(Mma<T>::format, (K + 15) / 16 * 16) | tc::kMnMajorB;
+    const uint32_t by_sums = tc::instr_desc(Mma<T>::format, (M + 15) / 16 * 16) |
+                             tc::kMnMajorA | tc::kMnMajorB;
+    const uint32_t leader = tc::elected();
+    const uint32_t k_blocks = p.pk > 1 ? kPanel : 0;  // to the next 64 columns
+    const int steps = (M + 15) / 16;
+    int staged = -1, stagings = 0, slot = 0, ys = 0, t = 0, piece = 0, sums = 0;
+    Run cur = after_live(none);
+    while (cur.n > 0) {
+      const Run nxt = after_live(cur);
+      char* const vz = s_tiles + slot * tile_bytes;
+      const uint32_t v_at = tc::smem_addr(vz), x_at = v_at + p.pm * kPanel;
+      const uint32_t low_at = tc::smem_addr(s_y + ys * p.pm * kPanel);
+      wait(ready(slot), t / p.slots);
+      if (p.vx) {
+        if (cur.g != staged) wait(weighed, stagings++);
+        staged = cur.g;
+        const int buf = NBUF == 2 ? t & 1 : 0;
+        if (t >= NBUF) wait(taken(buf), t / NBUF - 1);
+        tc::fence_after_sync();
+        const uint32_t acc = tmem + buf * TERMS * nk;
+        for (int i = 0; i < steps; ++i) {  // 16 of M: 32 bytes of a row, 16 rows of weights
+          const uint32_t at = (i >> 2) * kPanel + (i & 3) * 32;
+          const uint64_t dw = tc::smem_desc_mn(tc::smem_addr(s_w) + i * 2048, k_blocks);
+          tc::mma<false>(leader, acc, tc::smem_desc(v_at + at), dw, by_rows, i > 0);
+          if (TERMS == 2)
+            tc::mma<false>(leader, acc + nk, tc::smem_desc(low_at + at), dw, by_rows, i > 0);
+        }
+        tc::commit(leader, made(buf));
+      }
+      if (piece == 0 && sums > 0) wait(sum_taken, sums - 1);
+      tc::fence_after_sync();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {        // 16 rows
+        const uint64_t dx = tc::smem_desc_mn(x_at + i * 2048, k_blocks);
+        tc::mma<false>(leader, sum_acc, dx, tc::smem_desc_mn(v_at + i * 2048, kPanel), by_sums,
+                       piece > 0 || i > 0);
+        if (TERMS == 2)
+          tc::mma<false>(leader, sum_acc + nm, dx, tc::smem_desc_mn(low_at + i * 2048, kPanel),
+                         by_sums, piece > 0 || i > 0);
+      }
+      tc::commit(leader, free_(slot));
+      if (TERMS == 2) tc::commit(leader, y_free(ys));
+      if (++piece == kPiece || nxt.n == 0 || nxt.g != cur.g) {
+        tc::commit(leader, sum_made);
+        ++sums;
+        piece = 0;
+      }
+      slot = slot + 1 == p.slots ? 0 : slot + 1;
+      ys = ys + 1 == p.ys ? 0 : ys + 1;
+      ++t;
+      cur = nxt;
+    }
+    if (t > 0) wait(free_(slot > 0 ? slot - 1 : p.slots - 1), (t - 1) / p.slots);
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ front warps
+    const int tid = threadIdx.x;
+    const T* const x = static_cast<const T*>(p.x);
+    const T* const w = static_cast<const T*>(p.w);
+    const int c16 = tid & 7, r16 = tid >> 3;
+    const uint32_t o16 = chunk_at(r16, c16);
+    auto stage_weights = [&](int g) {  // rows of M, as they are
+      const T* const wg = w + (int64_t)g * M * K;
+      for (int m = r16; m < (M + 15) / 16 * 16; m += 32)
+        for (int j = 0; j < p.pk; ++j) {
+          const int c = j * 64 + c16 * 8;
+          const uint4 q = get_chunk<T, true>(m < M && c < K ? wg + (int64_t)m * K + c : wg,
+                                             m < M && c < K ? 1 : 0);
+          *reinterpret_cast<uint4*>(s_w + j * kPanel + chunk_at(m, c16)) = q;
+        }
+    };
+    // gathered rows of x: tile `ahead` into slot `ahead_s`
+    Run ahead = none, behind = none;
+    int ahead_s = 0, id[4];
+    auto read_ids = [&](const Run& t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        id[i] = p.ids && r16 + 32 * i < t.n ? __ldg(p.ids + t.row + r16 + 32 * i) : -1;
+    };
+    auto send = [&]() {
+      if (ahead.n > 0) {
+        char* const to = s_tiles + ahead_s * tile_bytes + p.pm * kPanel + o16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t from = (int64_t)id[i] * K + c16 * 8;
+          const bool ok = id[i] >= 0 && id[i] < p.s.n;
+          for (int j = 0; j < p.pk; ++j)
+            send_chunk<T, true>(to + j * kPanel + 4096 * i, x + from + j * 64,
+                                ok ? K - j * 64 - c16 * 8 : 0);
+        }
+        ahead_s = ahead_s + 1 == p.slots ? 0 : ahead_s + 1;
+        ahead = behind;
+        read_ids(ahead);
+        behind = after_live(ahead);
+      }
+      send_done();
+    };
+    if (SHARED) {
+      ahead = after_live(none);
+      read_ids(ahead);
+      behind = after_live(ahead);
+      for (int i = 1; i < p.slots; ++i) send();
+    }
+    float db[2][8];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
+    int staged = -1, slot = 0, ys = 0, t = 0;
+    Run cur = after_live(none);
+    while (cur.n > 0) {
+      const Run nxt = after_live(cur);
+      const int before = slot > 0 ? slot - 1 : p.slots - 1;
+      if (p.vx && cur.g != staged) {
+        if (t > 0) wait(free_(before), (t - 1) / p.slots);
+        stage_weights(cur.g);
+        tc::fence_smem();
+        __syncwarp();
+        if (lane == 0) tc::arrive(weighed);
+        staged = cur.g;
+      }
+      if (SHARED) {
+        if (t > 0) wait(free_(before), (t - 1) / p.slots);
+        send();
+        arrived(p.slots - 1);
+      }
+      wait(full(slot), t / p.slots);
+      if (HAS_Y) wait(y_full(ys), t / p.ys);
+      char* const vz = s_tiles + slot * tile_bytes;
+      char* const yt = s_y + ys * p.pm * kPanel;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (j >= p.pm) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t o = j * kPanel + o16 + 4096 * i;
+          const bool in = r16 + 32 * i < cur.n;  // rows behind are another group's
+          Chunk<T> v, z;
+          v.q = *reinterpret_cast<const uint4*>(vz + o);
+          if (HAS_Y) z.q = *reinterpret_cast<const uint4*>(yt + o);
+          float f[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[e] = in ? through<ACT>(to_f(v.v[e]), HAS_Y ? to_f(z.v[e]) : 0.0f) : 0.0f;
+            db[j][e] += f[e];
+          }
+          if (TERMS == 2) {
+            put_chunk<T, true>(vz + o, yt - vz, f);
+          } else if (HAS_Y || !in) {  // exact: v_y or 0
+            *reinterpret_cast<uint4*>(vz + o) = round_chunk<T>(f);
+          }
+        }
+      }
+      if (!SHARED && cur.n < kTile) {  // nor may what x has there be multiplied, even by zeros
+        for (int i = 0; i < 4; ++i)
+          if (r16 + 32 * i >= cur.n)
+            for (int j = 0; j < p.pk; ++j)
+              *reinterpret_cast<uint4*>(vz + (p.pm + j) * kPanel + o16 + 4096 * i) =
+                  make_uint4(0, 0, 0, 0);
+      }
+      tc::fence_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tc::arrive(ready(slot));
+        if (HAS_Y && TERMS == 1) tc::arrive(y_free(ys));
+      }
+      if (nxt.n == 0 || nxt.g != cur.g) {  // the group's v_b, summed in a fixed order
+        if (p.biases) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float b = db[j][e];
+              b += __shfl_xor_sync(0xffffffffu, b, 8);
+              b += __shfl_xor_sync(0xffffffffu, b, 16);
+              if (lane < 8) s_db[warp][j * 64 + lane * 8 + e] = b;
+            }
+          tc::bar_sync(1, kThreads);
+          if (tid < M) {
+            float b = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b += s_db[i][tid];
+            p.part[(int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1)) + (int64_t)M * K + tid] = b;
+          }
+          tc::bar_sync(1, kThreads);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
+      }
+      slot = slot + 1 == p.slots ? 0 : slot + 1;
+      ys = ys + 1 == p.ys ? 0 : ys + 1;
+      ++t;
+      cur = nxt;
+    }
+    if (SHARED) arrived(0);
+  } else {
+    // ------------------------------------------------------------- back warps
+    constexpr int MODE = SHARED ? kScatter : kBackward;
+    const int bw = warp - 8, row0 = (bw & 3) * 32;
+    int t = 0, piece = 0, sums = 0;
+    bool first = true;  // of the group
+    Run cur = after(none);
+    while (cur.n > 0) {
+      const Run nxt = after(cur);
+      const bool live = cur.g >= 0 && cur.g < p.s.G;
+      const int rows = min(32, cur.n - row0), buf = NBUF == 2 ? t & 1 : 0;
+      if (p.vx) {
+        int into = -1;
+        if (SHARED && live && lane < rows) into = __ldg(p.ids + cur.row + row0 + lane);
+        if (live) {
+          wait(made(buf), t / NBUF);
+          tc::fence_after_sync();
+        }
+        if (into >= p.s.n) into = -1;
+        if (!SHARED || live)
+          take_results<T, ACT, MODE, TERMS>(live, tmem + buf * TERMS * nk + ((uint32_t)row0 << 16),
+                                            nk, bw >> 2, rows, K, nullptr, into,
+                                            s_stage + bw * 2048, p.vx,
+                                            SHARED ? 0 : cur.row + row0, K, 0, 1);
+        if (live) {
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::arrive(taken(buf));
+        }
+      }
+      if (live) {
+        ++t;
+        const bool last = nxt.n == 0 || nxt.g != cur.g;
+        if (++piece == kPiece || last) {
+          wait(sum_made, sums);
+          tc::fence_after_sync();
+          float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1));
+          const int kk = row0 + lane;
+          for (int c0 = (bw >> 2) * 16; c0 < M; c0 += 32) {
+            float v[16];
+            tc::load16(sum_acc + ((uint32_t)row0 << 16) + c0, v);
+            if (TERMS == 2) {
+              float u[16];
+              tc::load16(sum_acc + nm + ((uint32_t)row0 << 16) + c0, u);
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (kk < K && c0 + i < M) {
+                float* const at = to + (int64_t)(c0 + i) * K + kk;
+                *at = first ? v[i] : *at + v[i];
+              }
+          }
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::arrive(sum_taken);
+          ++sums;
+          piece = 0;
+          first = last;
+        }
+      }
+      cur = nxt;
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) tc::dealloc(tmem, columns);
+}
+
 // v_W and v_b of a group: the places of the CTAs that had rows of it, in
 // order.  Eight warps take an eighth of the places each, for 32 values.
 template <typename T>
@@ -1180,6 +1589,8 @@ int run_fwd(const Shape& s, const void* x, const int32_t* ids, const int32_t* of
   return launch_rows<T, ACT, kForward, false>(p, st);
 }
 
+bool dims_fit_both(int K, int M) { return K <= 128 && M <= 128 && K % 8 == 0 && M % 8 == 0; }
+
 // The backward's launches and its scratch: parts of the weight sums, then
 // the fp32 sums of shared rows for the 16-bit types.
 struct Plan {
@@ -1187,13 +1598,14 @@ struct Plan {
   size_t part_floats, sum_floats;
 };
 
-Plan plan_of(const gs_grouped_params* p) {
+Plan plan_of(const gs_grouped_params* p) {  // one CTA an SM, or two
   Plan q;
   q.nt = p->out_features > 64 ? 128 : 64;
   q.kt = (int)ceil_div(p->in_features, 128);
   q.mt = (int)ceil_div(p->out_features, q.nt);
   const int64_t tiles = ceil_div(p->rows, kTile);
-  int64_t n = (int64_t)sm_count() * (p->dtype == GS_F32 ? 1 : 2) / ((int64_t)q.kt * q.mt);
+  const bool two = p->dtype != GS_F32 && !(dims_fit_both(p->in_features, p->out_features));
+  int64_t n = (int64_t)sm_count() * (two ? 2 : 1) / ((int64_t)q.kt * q.mt);
   n = n < 1 ? 1 : n > tiles ? tiles : n;
   q.parts = (int)n;
   q.part_floats = ((size_t)q.parts + p->groups) * p->out_features * ((size_t)p->in_features + 1);
@@ -1213,6 +1625,43 @@ int launch_weights(const WeightArgs& p, const Plan& q, cudaStream_t st) {
   return launch_status("grouped_linear_bwd");
 }
 
+// Whether one kernel can do the whole backward of 16-bit rows.
+template <typename T>
+bool fits_both(const Shape& s, const void* x, const void* w, const void* y, const void* vy,
+               const void* vx) {
+  return sizeof(T) == 2 && dims_fit_both(s.K, s.M) && s.R > 0 && on16(x) && on16(w) && on16(vy) && (!y || on16(y)) && (!vx || on16(vx));
+}
+
+template <typename T, int ACT, bool SHARED>
+int launch_both(BothArgs p, const void* vy, const void* y, const Plan& q, cudaStream_t st) {
+  constexpr auto kernel = both_mma_kernel<T, ACT, SHARED>;
+  if (int rc = allow_smem<kernel>()) return rc;
+  p.pk = p.s.K > 64 ? 2 : 1, p.pm = p.s.M > 64 ? 2 : 1;
+  p.slots = 2, p.ys = ACT ? 1 : 0;
+  auto smem = [&]() {
+    return 1024 + 8 * 2048 + kPanel * (p.pk + p.slots * (p.pm + p.pk) + p.ys * p.pm);
+  };
+  // first another tile of y, then one more of everything, while there is room
+  if (ACT && smem() + p.pm * kPanel <= kSmemMost) ++p.ys;
+  while (p.slots < 4 && smem() + (2 * p.pm + p.pk) * kPanel <= kSmemMost) {
+    ++p.slots;
+    if (ACT && p.ys < 4) ++p.ys;
+  }
+  if (p.ys == 0) p.ys = 1;  // not used
+  const int nk = (p.s.K + 31) / 32 * 32, nm = (p.s.M + 31) / 32 * 32;
+  const int terms = ACT == GS_ACT_SIGMOID ? 2 : 1;
+  int columns = 32;
+  while (columns < 2 * nk + terms * nm) columns *= 2;
+  CUtensorMap map_v{}, map_y{}, map_x{};
+  if (int rc = make_map(&map_v, vy, dtype_of<T>, p.s.R, p.s.M)) return rc;
+  if (ACT)
+    if (int rc = make_map(&map_y, y, dtype_of<T>, p.s.R, p.s.M)) return rc;
+  if (!SHARED)
+    if (int rc = make_map(&map_x, p.x, dtype_of<T>, p.s.R, p.s.K)) return rc;
+  kernel<<<(unsigned)q.parts, 2 * kThreads + 64, smem(), st>>>(p, columns, map_v, map_y, map_x);
+  return launch_status("grouped_linear_bwd");
+}
+
 template <typename T, int ACT>
 int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const int32_t* ids,
             const int32_t* off, const void* w, const void* y, const void* vy, void* vx, void* vw,
@@ -1220,9 +1669,27 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
   constexpr bool kSplit = sizeof(T) == 2 && ACT == GS_ACT_SIGMOID;
   const Plan q = plan_of(prm);
   if (ACT == GS_ACT_NONE) y = nullptr;
-  if (vx) {
-    const bool shared = prm->use_row_ids != 0;
-    float* sum = sizeof(T) == 4 ? static_cast<float*>(vx) : ws + q.part_floats;
+  const bool shared = prm->use_row_ids != 0;
+  float* const sum = sizeof(T) == 4 ? static_cast<float*>(vx) : ws + q.part_floats;
+  const bool both = (vw || vb) && fits_both<T>(s, x, w, y, vy, vx);
+  if constexpr (sizeof(T) == 2) {
+    if (both) {
+      if (vx && shared && cudaMemsetAsync(sum, 0, sizeof(float) * s.n * s.K, st) != cudaSuccess)
+        return launch_status("grouped_linear_bwd");
+      BothArgs p{};
+      p.s = s;
+      p.x = x, p.ids = ids, p.off = off, p.w = w, p.part = ws;
+      p.vx = !vx ? nullptr : shared ? sum : vx;
+      p.biases = vb != nullptr;
+      const int rc = shared ? launch_both<T, ACT, true>(p, vy, y, q, st)
+                            : launch_both<T, ACT, false>(p, vy, y, q, st);
+      if (rc) return rc;
+      if (vx && shared && s.n > 0)
+        round_kernel<T><<<grid_for(s.n * s.K, 256), 256, 0, st>>>(s.n * s.K, sum,
+                                                                  static_cast<T*>(vx));
+    }
+  }
+  if (vx && !both) {
     if (shared && cudaMemsetAsync(sum, 0, sizeof(float) * s.n * s.K, st) != cudaSuccess)
       return launch_status("grouped_linear_bwd");
     if (s.R > 0) {
@@ -1241,7 +1708,7 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
                                                                 static_cast<T*>(vx));
   }
   if (vw || vb) {
-    if (s.R > 0) {
+    if (s.R > 0 && !both) {
       WeightArgs p{};
       p.s = s;
       p.x = x, p.y = y, p.vy = vy, p.ids = ids, p.off = off, p.part = ws;

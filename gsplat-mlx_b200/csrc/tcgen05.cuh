@@ -22,10 +22,20 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
          (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 
+// The same panel as an operand whose rows are the depth (MN-major): 64
+// columns of 16-bit values to a row, the next 64 `blocks` bytes on, 8 rows to
+// 1024 bytes.  A step of 16 rows adds 2048 to the start.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t blocks) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3FFF) | (uint64_t(blocks >> 4) << 16) |
+         (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
 enum Format : uint32_t { kF16 = 0, kBF16 = 1, kTF32 = 2 };
 
 // Instruction descriptor: fp32 accumulators, A and B of one format, both
-// K-major, M = 128 lanes, N columns (a multiple of 16).
+// K-major unless the flags say MN-major, M = 128 lanes, N columns (a multiple
+// of 16).
+constexpr uint32_t kMnMajorA = 1u << 15, kMnMajorB = 1u << 16;
 __device__ __forceinline__ uint32_t instr_desc(uint32_t format, uint32_t n) {
   return (1u << 4) | (format << 7) | (format << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
