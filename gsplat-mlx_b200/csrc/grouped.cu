@@ -1023,7 +1023,7 @@ struct BothArgs {
   void* vx;          // v_x, its fp32 sums with SHARED, or NULL: not wanted
   float* part;       // as in WeightArgs
   int pk, pm;        // panels (64 columns) of K and M: 1 or 2
-  int slots, ys;     // tiles of v_y and x, and of y, in shared memory
+  int slots, ys;     // tiles of v_y and x, and panels of y, in shared memory
   int biases;
 };
 
@@ -1047,19 +1047,20 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   constexpr int TERMS = ACT == GS_ACT_SIGMOID ? 2 : 1;  // parts of v_z
   constexpr int NBUF = TERMS == 2 ? 1 : 2;              // accumulators of v_x
   constexpr bool HAS_Y = ACT != GS_ACT_NONE;
-  extern __shared__ char smem_raw[];
-  __shared__ uint64_t s_bars[3 * 4 + 2 * 4 + 2 * 2 + 3];
-  __shared__ uint32_t s_tmem;
-  __shared__ float s_db[8][128];
+  // all of it dynamic: the panels have to start on 1024 bytes, with nothing lost
+  extern __shared__ __align__(1024) char smem_raw[];
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int K = p.s.K, M = p.s.M;
   const int nk = (K + 31) / 32 * 32, nm = (M + 31) / 32 * 32;
   const int tile_bytes = (p.pm + p.pk) * kPanel;
-  char* const s_stage = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
-  char* const s_w = s_stage + 8 * 2048;
-  char* const s_tiles = s_w + p.pk * kPanel;   // v_z's panels, then x's
+  char* const s_tiles = smem_raw;              // v_z's panels, then x's
   char* const s_y = s_tiles + p.slots * tile_bytes;
+  char* const s_w = s_y + p.ys * kPanel;
+  char* const s_stage = s_w + p.pk * kPanel;
+  float (*const s_db)[64] = reinterpret_cast<float (*)[64]>(s_stage + 8 * 2048);
+  uint64_t* const s_bars = reinterpret_cast<uint64_t*>(s_db + 8);
+  uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + 27);
   const uint32_t bar0 = tc::smem_addr(s_bars);
   auto full = [&](int i) { return bar0 + 8 * i; };
   auto free_ = [&](int i) { return bar0 + 8 * (4 + i); };
@@ -1117,7 +1118,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
-    int slot = 0, ys = 0, t = 0;
+    int slot = 0, ys = 0, yq = 0, t = 0;
     for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur), ++t) {
       if (t >= p.slots) wait(free_(slot), t / p.slots - 1);
       if (tc::elected()) {
@@ -1130,18 +1131,16 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
             tc::load_box(to + (p.pm + j) * kPanel, &map_x, j * 64, cur.row, full(slot));
       }
       __syncwarp();
-      if (HAS_Y) {
-        if (t >= p.ys) wait(y_free(ys), t / p.ys - 1);
+      for (int j = 0; HAS_Y && j < p.pm; ++j, ++yq) {
+        if (yq >= p.ys) wait(y_free(ys), yq / p.ys - 1);
         if (tc::elected()) {
-          const uint32_t to = tc::smem_addr(s_y + ys * p.pm * kPanel);
-          tc::expect(y_full(ys), p.pm * kPanel);
-          for (int j = 0; j < p.pm; ++j)
-            tc::load_box(to + j * kPanel, &map_y, j * 64, cur.row, y_full(ys));
+          tc::expect(y_full(ys), kPanel);
+          tc::load_box(tc::smem_addr(s_y + ys * kPanel), &map_y, j * 64, cur.row, y_full(ys));
         }
         __syncwarp();
+        ys = ys + 1 == p.ys ? 0 : ys + 1;
       }
       slot = slot + 1 == p.slots ? 0 : slot + 1;
-      ys = ys + 1 == p.ys ? 0 : ys + 1;
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
@@ -1157,7 +1156,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       const Run nxt = after_live(cur);
       char* const vz = s_tiles + slot * tile_bytes;
       const uint32_t v_at = tc::smem_addr(vz), x_at = v_at + p.pm * kPanel;
-      const uint32_t low_at = tc::smem_addr(s_y + ys * p.pm * kPanel);
+      const uint32_t low_at = tc::smem_addr(s_y + ys * kPanel);  // whole tiles: ys % pm == 0
       wait(ready(slot), t / p.slots);
       if (p.vx) {
         if (cur.g != staged) wait(weighed, stagings++);
@@ -1187,14 +1186,14 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
                          by_sums, piece > 0 || i > 0);
       }
       tc::commit(leader, free_(slot));
-      if (TERMS == 2) tc::commit(leader, y_free(ys));
+      for (int j = 0; TERMS == 2 && j < p.pm; ++j) tc::commit(leader, y_free(ys + j));
       if (++piece == kPiece || nxt.n == 0 || nxt.g != cur.g) {
         tc::commit(leader, sum_made);
         ++sums;
         piece = 0;
       }
       slot = slot + 1 == p.slots ? 0 : slot + 1;
-      ys = ys + 1 == p.ys ? 0 : ys + 1;
+      ys = ys + p.pm >= p.ys ? 0 : ys + p.pm;
       ++t;
       cur = nxt;
     }
@@ -1251,7 +1250,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     float db[2][8];
 #pragma unroll
     for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
-    int staged = -1, slot = 0, ys = 0, t = 0;
+    int staged = -1, slot = 0, ys = 0, yq = 0, t = 0;
     Run cur = after_live(none);
     while (cur.n > 0) {
       const Run nxt = after_live(cur);
@@ -1270,12 +1269,12 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         arrived(p.slots - 1);
       }
       wait(full(slot), t / p.slots);
-      if (HAS_Y) wait(y_full(ys), t / p.ys);
       char* const vz = s_tiles + slot * tile_bytes;
-      char* const yt = s_y + ys * p.pm * kPanel;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (j >= p.pm) break;
+        char* const yt = s_y + ys * kPanel - j * kPanel;
+        if (HAS_Y) wait(y_full(ys), yq / p.ys);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t o = j * kPanel + o16 + 4096 * i;
@@ -1295,6 +1294,15 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
             *reinterpret_cast<uint4*>(vz + o) = round_chunk<T>(f);
           }
         }
+        if (HAS_Y) {
+          if (TERMS == 1) {
+            tc::fence_smem();  // read before TMA writes there again
+            __syncwarp();
+            if (lane == 0) tc::arrive(y_free(ys));
+          }
+          ++yq;
+          ys = ys + 1 == p.ys ? 0 : ys + 1;
+        }
       }
       if (!SHARED && cur.n < kTile) {  // nor may what x has there be multiplied, even by zeros
         for (int i = 0; i < 4; ++i)
@@ -1305,35 +1313,34 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       }
       tc::fence_smem();
       __syncwarp();
-      if (lane == 0) {
-        tc::arrive(ready(slot));
-        if (HAS_Y && TERMS == 1) tc::arrive(y_free(ys));
-      }
+      if (lane == 0) tc::arrive(ready(slot));
       if (nxt.n == 0 || nxt.g != cur.g) {  // the group's v_b, summed in a fixed order
         if (p.biases) {
+          float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1)) +
+                            (int64_t)M * K;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               float b = db[j][e];
               b += __shfl_xor_sync(0xffffffffu, b, 8);
               b += __shfl_xor_sync(0xffffffffu, b, 16);
-              if (lane < 8) s_db[warp][j * 64 + lane * 8 + e] = b;
+              if (lane < 8) s_db[warp][lane * 8 + e] = b;
             }
-          tc::bar_sync(1, kThreads);
-          if (tid < M) {
-            float b = 0.0f;
+            tc::bar_sync(1, kThreads);
+            if (tid < 64 && j * 64 + tid < M) {
+              float b = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) b += s_db[i][tid];
-            p.part[(int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1)) + (int64_t)M * K + tid] = b;
+              for (int i = 0; i < 8; ++i) b += s_db[i][tid];
+              to[j * 64 + tid] = b;
+            }
+            tc::bar_sync(1, kThreads);
           }
-          tc::bar_sync(1, kThreads);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
       }
       slot = slot + 1 == p.slots ? 0 : slot + 1;
-      ys = ys + 1 == p.ys ? 0 : ys + 1;
       ++t;
       cur = nxt;
     }
@@ -1472,16 +1479,16 @@ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // arrays.
 constexpr int kSmemMost = 227 * 1024 - 5120;
 
-// Lets a kernel use kSmemMost bytes on the current device; asked once for
+// Lets a kernel use `bytes` of dynamic shared memory on the current device; asked once for
 // each kernel (the instantiation is the kernel's own) and device.
-template <auto kernel>
+template <auto kernel, int bytes = kSmemMost>
 int allow_smem() {
   static bool done[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
     return launch_status("grouped_linear");
   if (!done[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost) !=
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
         cudaSuccess)
       return launch_status("grouped_linear");
     done[dev] = true;
@@ -1635,21 +1642,20 @@ bool fits_both(const Shape& s, const void* x, const void* w, const void* y, cons
 template <typename T, int ACT, bool SHARED>
 int launch_both(BothArgs p, const void* vy, const void* y, const Plan& q, cudaStream_t st) {
   constexpr auto kernel = both_mma_kernel<T, ACT, SHARED>;
-  if (int rc = allow_smem<kernel>()) return rc;
+  constexpr int kAll = 227 * 1024;  // this kernel has no static shared memory
+  if (int rc = allow_smem<kernel, kAll>()) return rc;
   p.pk = p.s.K > 64 ? 2 : 1, p.pm = p.s.M > 64 ? 2 : 1;
-  p.slots = 2, p.ys = ACT ? 1 : 0;
-  auto smem = [&]() {
-    return 1024 + 8 * 2048 + kPanel * (p.pk + p.slots * (p.pm + p.pk) + p.ys * p.pm);
-  };
-  // first another tile of y, then one more of everything, while there is room
-  if (ACT && smem() + p.pm * kPanel <= kSmemMost) ++p.ys;
-  while (p.slots < 4 && smem() + (2 * p.pm + p.pk) * kPanel <= kSmemMost) {
-    ++p.slots;
-    if (ACT && p.ys < 4) ++p.ys;
-  }
-  if (p.ys == 0) p.ys = 1;  // not used
-  const int nk = (p.s.K + 31) / 32 * 32, nm = (p.s.M + 31) / 32 * 32;
   const int terms = ACT == GS_ACT_SIGMOID ? 2 : 1;
+  // As many tiles as there is room for beside one tile of y, then as many
+  // panels of y (whole tiles where the low parts of v_z lie in them).
+  p.slots = 2, p.ys = ACT ? p.pm : 0;
+  auto smem = [&]() {
+    return 8 * 2048 + 2048 + 27 * 8 + 8 + kPanel * (p.pk + p.slots * (p.pm + p.pk) + p.ys);
+  };
+  while (p.slots < 4 && smem() + (p.pm + p.pk) * kPanel <= kAll) ++p.slots;
+  const int more = terms == 2 ? p.pm : 1;
+  while (ACT && p.ys + more <= 4 && smem() + more * kPanel <= kAll) p.ys += more;
+  const int nk = (p.s.K + 31) / 32 * 32, nm = (p.s.M + 31) / 32 * 32;
   int columns = 32;
   while (columns < 2 * nk + terms * nm) columns *= 2;
   CUtensorMap map_v{}, map_y{}, map_x{};
