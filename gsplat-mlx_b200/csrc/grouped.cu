@@ -5,9 +5,10 @@
 //   v_z[r] = v_y[r] act'(y[r])
 //   v_x[id(r)] += W[g]^T v_z[r],  v_W[g] = sum v_z[r] x[id(r)]^T,  v_b[g] = sum v_z[r]
 //
-// A row's group is found by binary search over the offsets; the search's
-// invariant off[g] <= r < off[g + 1] holds for the pair that it ends at even
-// where the offsets do not ascend, so no index leaves its buffer.
+// A row's group is found by a search over the offsets whose invariant
+// off[g] <= r < off[g + 1] holds for the pair that it ends at even where the
+// offsets do not ascend, so every run of rows has one row at least and no
+// index leaves its buffer.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,16 +36,21 @@ struct Shape {
   int G, K, M;
 };
 
-// The group of row r: -1 in front of the first, G behind the last.
-__device__ __forceinline__ int group_of(const int32_t* __restrict__ off, int G, int64_t r) {
-  if (r < __ldg(off)) return -1;
-  if (r >= __ldg(off + G)) return G;
+// The group of row r: -1 in front of the first, G behind the last.  Called by
+// whole warps with the same r: a step of the search looks at 32 places.
+__device__ __forceinline__ int group_of(const int32_t* __restrict__ off, int G, int r) {
+  const int lane = threadIdx.x & 31;
+  const int first = __ldg(off), last = __ldg(off + G);
   int lo = 0, hi = G;  // off[lo] <= r < off[hi]
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(off + mid) <= r) lo = mid; else hi = mid;
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const uint32_t below = __ballot_sync(0xffffffffu, at < hi && __ldg(off + at) <= r);
+    // the places where the row is above one and below the next
+    const int i = below == 0xffffffffu ? 31 : max(__ffs(~below) - 2, 0);
+    lo += i * step;
+    hi = min(hi, lo + step);
   }
-  return lo;
+  return r < first ? -1 : r >= last ? G : lo;
 }
 
 template <int ACT>
@@ -1207,13 +1213,17 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     const uint32_t o16 = chunk_at(r16, c16);
     auto stage_weights = [&](int g) {  // rows of M, as they are
       const T* const wg = w + (int64_t)g * M * K;
-      for (int m = r16; m < (M + 15) / 16 * 16; m += 32)
-        for (int j = 0; j < p.pk; ++j) {
-          const int c = j * 64 + c16 * 8;
-          const uint4 q = get_chunk<T, true>(m < M && c < K ? wg + (int64_t)m * K + c : wg,
-                                             m < M && c < K ? 1 : 0);
-          *reinterpret_cast<uint4*>(s_w + j * kPanel + chunk_at(m, c16)) = q;
-        }
+      uint4 q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int m = r16 + 32 * (i & 3), c = (i >> 2) * 64 + c16 * 8;
+        const bool in = m < M && c < K;
+        q[i] = get_chunk<T, true>(in ? wg + (int64_t)m * K + c : wg, in);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >> 2 < p.pk)
+          *reinterpret_cast<uint4*>(s_w + (i >> 2) * kPanel + o16 + 4096 * (i & 3)) = q[i];
     };
     // gathered rows of x: tile `ahead` into slot `ahead_s`
     Run ahead = none, behind = none;
@@ -1393,12 +1403,17 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
               for (int i = 0; i < 16; ++i)
                 if (fabsf(v[i]) < INFINITY) v[i] += u[i];
             }
+            float* const at = to + (int64_t)c0 * K + kk;
+            if (!first && kk < K) {  // all read before the first is written
+              float u[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) u[i] = c0 + i < M ? at[(int64_t)i * K] : 0.0f;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] += u[i];
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (kk < K && c0 + i < M) {
-                float* const at = to + (int64_t)(c0 + i) * K + kk;
-                *at = first ? v[i] : *at + v[i];
-              }
+              if (kk < K && c0 + i < M) at[(int64_t)i * K] = v[i];
           }
           tc::fence_before_sync();
           __syncwarp();
@@ -1417,16 +1432,18 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 }
 
 // v_W and v_b of a group: the places of the CTAs that had rows of it, in
-// order.  Eight warps take an eighth of the places each, for 32 values.
-template <typename T>
+// order.  A block takes 256 / SHARES values; its warps take a share of the
+// places each, and the shares are added in order.
+template <typename T, int SHARES>
 __global__ void __launch_bounds__(256) join_kernel(Shape s, int parts,
                                                    const int32_t* __restrict__ off,
                                                    const float* __restrict__ part,
                                                    T* __restrict__ vw, T* __restrict__ vb) {
-  __shared__ float s_sum[8][32];
-  const int g = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int VALUES = 256 / SHARES;
+  __shared__ float s_sum[SHARES][VALUES];
+  const int g = blockIdx.y, share = threadIdx.x / VALUES, at = threadIdx.x % VALUES;
   const int64_t mk = (int64_t)s.M * s.K, each = mk + s.M;
-  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t i = (int64_t)blockIdx.x * VALUES + at;
   const int64_t r0 = max((int64_t)__ldg(off + g), (int64_t)0);
   const int64_t r1 = min((int64_t)__ldg(off + g + 1), s.R);
   float sum = 0.0f;
@@ -1434,21 +1451,22 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int parts,
     const int64_t tiles = (s.R + kTile - 1) / kTile;
     auto part_of = [&](int64_t r) { return (int)(((r / kTile + 1) * parts - 1) / tiles); };
     const int b0 = part_of(r0), n = part_of(r1 - 1) - b0 + 1;
-    const int from = n * warp / 8, to = n * (warp + 1) / 8;
+    const int from = n * share / SHARES, to = n * (share + 1) / SHARES;
     const float* p = part + (int64_t)(b0 + g + from) * each + i;
 #pragma unroll 8
     for (int b = from; b < to; ++b, p += each) sum += __ldg(p);
   }
-  s_sum[warp][lane] = sum;
-  __syncthreads();
-  if (warp == 0 && i < each) {
+  if (SHARES > 1) {
+    s_sum[share][at] = sum;
+    __syncthreads();
+    if (share > 0) return;
 #pragma unroll
-    for (int w = 1; w < 8; ++w) sum += s_sum[w][lane];
-    if (i < mk) {
-      if (vw) vw[g * mk + i] = from_f<T>(sum);
-    } else if (vb) {
-      vb[(int64_t)g * s.M + (i - mk)] = from_f<T>(sum);
-    }
+    for (int w = 1; w < SHARES; ++w) sum += s_sum[w][at];
+  }
+  if (i < mk) {
+    if (vw) vw[g * mk + i] = from_f<T>(sum);
+  } else if (i < each && vb) {
+    vb[(int64_t)g * s.M + (i - mk)] = from_f<T>(sum);
   }
 }
 
@@ -1727,8 +1745,13 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
     }
     const int64_t each = (int64_t)s.M * (s.K + 1);
     if (s.G > 65535) return invalid("grouped_linear: more than 65535 groups");
-    join_kernel<T><<<dim3((unsigned)ceil_div(each, 32), (unsigned)s.G), 256, 0, st>>>(
-        s, q.parts, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
+    // about parts / G places a group: few are not worth sharing out
+    if (q.parts < 16 * (int64_t)s.G)
+      join_kernel<T, 1><<<dim3((unsigned)ceil_div(each, 256), (unsigned)s.G), 256, 0, st>>>(
+          s, q.parts, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
+    else
+      join_kernel<T, 8><<<dim3((unsigned)ceil_div(each, 32), (unsigned)s.G), 256, 0, st>>>(
+          s, q.parts, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
   }
   return launch_status("grouped_linear_bwd");
 }
