@@ -752,40 +752,36 @@ struct WeightArgs {
   const void* vy;
   const int32_t* ids;
   const int32_t* off;
-  float* part;       // [parts + G][M * K + M]
+  float* part;       // [parts + G][M * K + M x copies of v_b]
   int kt, mt;        // tiles of K (128) and M (NT)
   int wide_x, wide_y;
   int biases;
 };
 
-// v_W[g] (as K lanes x M columns) = sum over g's rows of x[r]^T v_z[r].
+// v_W[g] (as K lanes x M columns) = sum over g's rows of x[r]^T v_z[r], of
+// 16-bit rows that the kernel for the whole backward does not take: off the 16-byte
+// boundary, or more than 128 features.
 //
-// The rows are the depth here, so both operands are staged transposed: a
-// thread takes a few rows' chunks of the same columns (4 x 4 fp32, 8 x 8 in
-// 16 bits) and writes their columns as chunks.  A CTA sums the rows of its
-// consecutive tiles; what it has at the end of a group goes to its own place
-// in `part` (CTA b and group g: place b + g; both only ever grow), and the
-// places of a group are added in order by another kernel, so the sums have a
-// fixed order.  In fp32 the accumulators are moved to registers every
-// kFlush panels: the tensor core cuts a sum to fp32 rather than rounding it,
-// which a few thousand additions would make visible.
-constexpr int kFlush = 8;
-
+// The rows are the depth here, and both operands are staged transposed: a
+// thread takes eight rows' chunks of the same eight columns and writes their
+// columns as chunks.  A CTA sums the rows of its consecutive tiles; what it
+// has at the end of a group goes to its own place in `part` (CTA b and group
+// g: place b + g; both only ever grow), and the places of a group are added
+// in order by another kernel, so the sums have a fixed order.
 template <typename T, int ACT, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
     weights_mma_kernel(WeightArgs p, int columns) {
   constexpr int E = Chunk<T>::E;
   constexpr int DP = 128 / sizeof(T);
   constexpr int STEP = 32 / sizeof(T);
-  constexpr bool F32 = sizeof(T) == 4;
-  constexpr int XTERMS = F32 ? 2 : 1, VTERMS = F32 || SPLIT ? 2 : 1;
+  constexpr int VTERMS = SPLIT ? 2 : 1;
   constexpr int VPANEL = NT * 128;
   extern __shared__ char smem_raw[];
   __shared__ uint64_t s_bar;
   __shared__ uint32_t s_tmem;
   __shared__ int32_t s_ids[4][DP];
   char* const s_x = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
-  char* const s_v = s_x + XTERMS * kPanel;
+  char* const s_v = s_x + kPanel;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int k0 = (blockIdx.y % p.kt) * 128, m0 = (blockIdx.y / p.kt) * NT;
@@ -822,12 +818,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
   const bool has_x = tid < x_units, has_v = vu < v_units;
   const int rb = (tid & 7) * E;                 // first row of either block
   const int xc = (tid >> 3) * E, vc = (vu >> 3) * E;
-  // in 16 bits a thread has a block of x or one of v_y: they share registers
-  uint4 rx[E], rv_own[F32 ? E : 1], ry[ACT ? E : 1];
-  auto rv = [&](int i) -> uint4& {
-    if constexpr (F32) return rv_own[i];
-    else return rx[i];
-  };
+  uint4 rx[E], ry[ACT ? E : 1];  // a thread has a block of x or one of v_y
   float bsum[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) bsum[e] = 0.0f;
@@ -866,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
       if (has_v) {
         const int64_t from = in ? (int64_t)(t.row + rb + i) * p.s.M + m0 + vc : 0;
         const int there = in ? mn - vc : 0;
-        rv(i) = p.wide_y ? get_chunk<T, true>(vy + from, there) : get_chunk<T, false>(vy + from, there);
+        rx[i] = p.wide_y ? get_chunk<T, true>(vy + from, there) : get_chunk<T, false>(vy + from, there);
         if (ACT)
           ry[ACT ? i : 0] = p.wide_y ? get_chunk<T, true>(y + from, there)
                                      : get_chunk<T, false>(y + from, there);
@@ -875,27 +866,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
   };
 
   constexpr int HALF = NT / 2;  // columns of a warp's half of the accumulators
-  float acc[F32 ? HALF : 1];
-  bool held = false;            // acc has a part of the sum
-  // adds the accumulators to acc (fp32 only)
-  auto flush = [&]() {
-    if constexpr (F32) {
-#pragma unroll
-      for (int c = 0; c < HALF; c += 16) {
-        float v[16], u[16];
-        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * HALF + c;
-        tc::load16(from, v);
-        tc::load16(from + NT, u);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (fabsf(v[i]) < INFINITY) v[i] += u[i];
-          acc[c + i] = held ? acc[c + i] + v[i] : v[i];
-        }
-      }
-      held = true;
-    }
-  };
-
   if (tid < DP) s_ids[0][tid] = id_of(cur, tid);
   int next_id = tid < DP ? id_of(nxt, tid) : -1;
   __syncthreads();
@@ -904,25 +874,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
 
   for (int k = 0; cur.n > 0; ++k) {
     if (pending > 0) wait_mma();  // the panels' memory is free again
-    if (F32 && pending == kFlush) {
-      flush();
-      pending = 0;
-    }
     if (has_x) {
 #pragma unroll
       for (int c = 0; c < E; ++c) {
-        float f[E];
         Chunk<T> raw;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           Chunk<T> q;
           q.q = rx[i];
-          f[i] = to_f(q.v[c]);
           raw.v[i] = q.v[c];
         }
-        char* const to = s_x + chunk_at(xc + c, tid & 7);
-        if (F32) put_chunk<T, false>(to, kPanel, f);
-        else *reinterpret_cast<uint4*>(to) = raw.q;
+        *reinterpret_cast<uint4*>(s_x + chunk_at(xc + c, tid & 7)) = raw.q;
       }
     }
     if (has_v) {
@@ -932,7 +894,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           Chunk<T> q, o;
-          q.q = rv(i);
+          q.q = rx[i];
           if (ACT) o.q = ry[ACT ? i : 0];
           f[i] = through<ACT>(to_f(q.v[c]), ACT ? to_f(o.v[c]) : 0.0f);
           bsum[c] += f[i];
@@ -954,15 +916,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
         if (i >= steps) break;
         const uint64_t at = 2 * i;
         const bool more = pending > 0 || i > 0;
-        if (VTERMS == 2) {
-          tc::mma<Mma<T>::TF32>(leader, tmem + NT, dx + at, dv + (VPANEL >> 4) + at, idesc, more);
-          if (XTERMS == 2) {
-            tc::mma<Mma<T>::TF32>(leader, tmem + NT, dx + (kPanel >> 4) + at, dv + at, idesc, true);
-            tc::mma<Mma<T>::TF32>(leader, tmem + NT, dx + (kPanel >> 4) + at, dv + (VPANEL >> 4) + at,
-                                  idesc, true);
-          }
-        }
-        tc::mma<Mma<T>::TF32>(leader, tmem, dx + at, dv + at, idesc, more);
+        if (VTERMS == 2)
+          tc::mma<false>(leader, tmem + NT, dx + at, dv + (VPANEL >> 4) + at, idesc, more);
+        tc::mma<false>(leader, tmem, dx + at, dv + at, idesc, more);
       }
       tc::commit(leader, bar);
     }
@@ -977,26 +933,23 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
       wait_mma();
       float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)p.s.M * (p.s.K + 1));
       const int kk = (warp & 3) * 32 + lane;
-      if (F32) flush();
 #pragma unroll
       for (int c = 0; c < HALF; c += 16) {
         float v[16];
-        if (!F32) {
-          const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * HALF + c;
-          tc::load16(from, v);
-          if (SPLIT) {
-            float u[16];
-            tc::load16(from + NT, u);
+        const uint32_t from = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (warp >> 2) * HALF + c;
+        tc::load16(from, v);
+        if (SPLIT) {
+          float u[16];
+          tc::load16(from + NT, u);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (fabsf(v[i]) < INFINITY) v[i] += u[i];
-          }
+          for (int i = 0; i < 16; ++i)
+            if (fabsf(v[i]) < INFINITY) v[i] += u[i];
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int m = (warp >> 2) * HALF + c + i;
           if (kk < kn && m < mn)
-            to[(int64_t)(m0 + m) * p.s.K + k0 + kk] = F32 ? acc[F32 ? c + i : 0] : v[i];
+            to[(int64_t)(m0 + m) * p.s.K + k0 + kk] = v[i];
         }
       }
 #pragma unroll
@@ -1009,7 +962,6 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
         bsum[e] = 0.0f;
       }
       pending = 0;
-      held = false;
       tc::fence_before_sync();
       __syncthreads();
     }
@@ -1017,6 +969,381 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 1 : 2)
     nxt = after;
   }
   if (warp == 0) tc::dealloc(tmem, columns);
+}
+
+// v_W and v_b of fp32 rows.
+//
+// Depth runs over rows here and tf32 operands are K-major, so what arrives as
+// 32 rows x 32 columns boxes (TMA; copies where rows are gathered or off the
+// boundary) is transposed on its way to the operands: a thread reads a 4 x 4
+// block as four chunks and writes its columns as chunks of the values (of
+// which the tensor core takes the upper part) and of their low parts.  The
+// eight lanes of an access take the diagonal blocks (column block l, row
+// block l ^ p), which keeps both the reads and the writes free of conflicts in
+// the swizzled panels.  Two groups of four front warps take every second
+// panel of 32 rows, each with operand memory of its own.
+//
+// The tensor core cuts a sum to fp32 at each addition; left to itself that
+// was 2e-5 of the result after 8000 rows.  So every kFlush panels the MMAs
+// change accumulators, and the back warps add the finished one to sums that
+// they hold in registers.
+constexpr int kFlush = 4;
+constexpr int kRows32 = 32;
+constexpr int kBox = kRows32 * 128;
+constexpr int kBiasCopies32 = 4;  // partial sums of v_b: front groups x halves
+
+struct Weight32Args {
+  Shape s;
+  const float* x;
+  const float* y;
+  const float* vy;
+  const int32_t* ids;
+  const int32_t* off;
+  float* part;         // as in WeightArgs, with kBiasCopies32 rows of v_b
+  int kt;              // tiles of K (128)
+  int kx, mx;          // boxes of a K tile and of an M tile
+  int slots;           // panels of boxes; even with copies
+  int x_mode, v_mode;  // 0: TMA, 1: copies of 16 bytes, 2: of 4
+  int biases;
+};
+
+template <int ACT, int NT>
+__global__ void __launch_bounds__(2 * kThreads + 64, 1)
+    weights32_kernel(Weight32Args p, const __grid_constant__ CUtensorMap map_x,
+                     const __grid_constant__ CUtensorMap map_v,
+                     const __grid_constant__ CUtensorMap map_y) {
+  constexpr bool HAS_Y = ACT != GS_ACT_NONE;
+  extern __shared__ __align__(1024) char smem_raw[];
+  const int lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int K = p.s.K, M = p.s.M;
+  const int k0 = (blockIdx.y % p.kt) * 128, m0 = (blockIdx.y / p.kt) * NT;
+  const int kn = min(128, K - k0), mn = min(NT, M - m0);
+  const int boxes = p.kx + p.mx;                          // x's, then v_y's
+  const int slot_bytes = (boxes + (HAS_Y ? p.mx : 0)) * kBox;  // then y's
+  // operands: two sets of values and low parts of x, of v_z.  An MMA reads
+  // 128 rows of x's whatever kn is: what lies behind goes to unused lanes.
+  const int set_bytes = 2 * boxes * kBox;
+  char* const s_sets = smem_raw;
+  char* const s_slots = s_sets + 2 * set_bytes;
+  uint64_t* const s_bars = reinterpret_cast<uint64_t*>(s_slots + p.slots * slot_bytes);
+  uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + 24);
+  const uint32_t bar0 = tc::smem_addr(s_bars);
+  auto full = [&](int i) { return bar0 + 8 * i; };          // TMA's boxes are there
+  auto free_ = [&](int i) { return bar0 + 8 * (8 + i); };   // and have been read
+  auto ready = [&](int i) { return bar0 + 8 * (16 + i); };  // operands
+  auto spent = [&](int i) { return bar0 + 8 * (18 + i); };
+  auto made = [&](int i) { return bar0 + 8 * (20 + i); };   // accumulators
+  auto taken = [&](int i) { return bar0 + 8 * (22 + i); };
+  if (warp == 0) tc::alloc(&s_tmem, 4 * NT);
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < 8; ++i) {
+      tc::bar_init(full(i), 1);
+      tc::bar_init(free_(i), 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::bar_init(ready(i), 4);
+      tc::bar_init(spent(i), 1);
+      tc::bar_init(made(i), 1);
+      tc::bar_init(taken(i), 8);
+    }
+    tc::bar_init_done();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  uint32_t limit = kWaitLimit;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (!tc::bar_wait(bar, parity & 1, limit)) {
+      limit = 0;
+      g_wait_gave_up = 1;
+    }
+  };
+
+  const int64_t tiles = (p.s.R + kTile - 1) / kTile;
+  const int end = (int)min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
+  Run none;
+  none.row = (int)(first_tile(tiles, gridDim.x, blockIdx.x) * kTile);
+  none.n = 0, none.g = -1, none.group_end = 0;
+  auto after = [&](Run t) {  // skips rows outside every group
+    t = run_from(p.off, p.s.G, t.row + t.n, end, kRows32, t);
+    while (t.n > 0 && (t.g < 0 || t.g >= p.s.G))
+      t = run_from(p.off, p.s.G, t.group_end, end, kRows32, t);
+    return t;
+  };
+  const int tma_boxes = (p.x_mode == 0 ? p.kx : 0) + (p.v_mode == 0 ? p.mx * (HAS_Y ? 2 : 1) : 0);
+
+  if (warp == 17) {
+    // ------------------------------------------------------------- TMA
+    if (tma_boxes > 0) {
+      int slot = 0, q = 0;
+      for (Run cur = after(none); cur.n > 0; cur = after(cur), ++q) {
+        if (q >= p.slots) wait(free_(slot), q / p.slots - 1);
+        if (tc::elected()) {
+          const uint32_t to = tc::smem_addr(s_slots + slot * slot_bytes);
+          tc::expect(full(slot), tma_boxes * kBox);
+          if (p.x_mode == 0)
+            for (int j = 0; j < p.kx; ++j)
+              tc::load_box(to + j * kBox, &map_x, k0 + j * 32, cur.row, full(slot));
+          if (p.v_mode == 0)
+            for (int j = 0; j < p.mx; ++j) {
+              tc::load_box(to + (p.kx + j) * kBox, &map_v, m0 + j * 32, cur.row, full(slot));
+              if (HAS_Y)
+                tc::load_box(to + (boxes + j) * kBox, &map_y, m0 + j * 32, cur.row, full(slot));
+            }
+        }
+        __syncwarp();
+        slot = slot + 1 == p.slots ? 0 : slot + 1;
+      }
+    }
+  } else if (warp == 16) {
+    // ------------------------------------------------------------- MMAs
+    const uint32_t idesc = tc::instr_desc(tc::kTF32, (mn + 15) / 16 * 16);
+    const uint32_t leader = tc::elected();
+    int q = 0, held = 0, sums = 0;
+    Run cur = after(none);
+    while (cur.n > 0) {
+      const Run nxt = after(cur);
+      const int set = q & 1, buf = sums & 1;
+      wait(ready(set), q >> 1);
+      if (held == 0 && sums > 1) wait(taken(buf), (sums >> 1) - 1);
+      tc::fence_after_sync();
+      const uint32_t x_at = tc::smem_addr(s_sets + set * set_bytes);
+      const uint64_t xh = tc::smem_desc(x_at), xl = tc::smem_desc(x_at + p.kx * kBox);
+      const uint32_t v_at = x_at + 2 * p.kx * kBox;
+      const uint64_t vh = tc::smem_desc(v_at), vl = tc::smem_desc(v_at + p.mx * kBox);
+      const uint32_t acc = tmem + buf * 2 * NT;
+      const int steps = (cur.n + 7) / 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= steps) break;
+        const uint64_t at = 2 * i;
+        const bool more = held > 0 || i > 0;
+        tc::mma<true>(leader, acc + NT, xl + at, vl + at, idesc, more);
+        tc::mma<true>(leader, acc + NT, xl + at, vh + at, idesc, true);
+        tc::mma<true>(leader, acc + NT, xh + at, vl + at, idesc, true);
+        tc::mma<true>(leader, acc, xh + at, vh + at, idesc, more);
+      }
+      tc::commit(leader, spent(set));
+      if (++held == kFlush || nxt.n == 0 || nxt.g != cur.g) {
+        tc::commit(leader, made(buf));
+        ++sums;
+        held = 0;
+      }
+      ++q;
+      cur = nxt;
+    }
+    if (q > 0) wait(spent((q - 1) & 1), (q - 1) >> 1);
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ front warps
+    const int fg = warp >> 2, tid = threadIdx.x & 127;
+    const bool copies = p.x_mode != 0 || p.v_mode != 0;
+    const int own = p.slots / 2;  // with copies: this group's slots
+    auto second = [&](const Run& t) { return after(after(t)); };
+    // copies: rows r16 and r16 + 16, chunk c16, of every box
+    const int r16 = tid >> 3, c16 = tid & 7;
+    Run ahead = none;
+    int ahead_i = 0, id[2];
+    auto read_ids = [&](const Run& t) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = r16 + 16 * i;
+        id[i] = row >= t.n ? -1 : p.ids ? __ldg(p.ids + t.row + row) : t.row + row;
+      }
+    };
+    auto send = [&]() {
+      if (ahead.n > 0) {
+        char* const to = s_slots + (2 * ahead_i + fg) * slot_bytes;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = r16 + 16 * i;
+          const uint32_t o = chunk_at(row, c16);
+          if (p.x_mode != 0) {
+            const bool ok = id[i] >= 0 && id[i] < p.s.n;
+            const float* const from = p.x + (ok ? (int64_t)id[i] * K + k0 + c16 * 4 : 0);
+            for (int j = 0; j < p.kx; ++j) {
+              const int there = ok ? kn - j * 32 - c16 * 4 : 0;
+              if (p.x_mode == 1) send_chunk<float, true>(to + j * kBox + o, from + j * 32, there);
+              else send_chunk<float, false>(to + j * kBox + o, from + j * 32, there);
+            }
+          }
+          if (p.v_mode != 0) {
+            const bool ok = row < ahead.n;
+            const int64_t from = ok ? (int64_t)(ahead.row + row) * M + m0 + c16 * 4 : 0;
+            for (int j = 0; j < p.mx; ++j) {
+              const int there = ok ? mn - j * 32 - c16 * 4 : 0;
+              send_chunk<float, false>(to + (p.kx + j) * kBox + o, p.vy + from + j * 32, there);
+              if (HAS_Y)
+                send_chunk<float, false>(to + (boxes + j) * kBox + o, p.y + from + j * 32, there);
+            }
+          }
+        }
+        ahead_i = ahead_i + 1 == own ? 0 : ahead_i + 1;
+        ahead = second(ahead);
+        read_ids(ahead);
+      }
+      send_done();
+    };
+    Run cur = after(none);
+    if (copies) {
+      ahead = fg ? after(cur) : cur;
+      read_ids(ahead);
+      for (int i = 1; i < own; ++i) send();
+    }
+    // this thread's 4 x 4 blocks: of boxes 2 it + (tid >> 6)
+    const int l = tid & 7, c = l, rg = l ^ ((tid >> 3) & 7);
+    constexpr int ITS = (4 + NT / 32) / 2;
+    float db[ITS][4];
+#pragma unroll
+    for (int it = 0; it < ITS; ++it)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) db[it][j] = 0.0f;
+    int slot = 0, q = 0;
+    while (cur.n > 0) {
+      const Run nxt = after(cur);
+      if ((q & 1) == fg) {
+        if (copies) {
+          if (own > 1) {
+            arrived(own - 2);
+            tc::bar_sync(1 + fg, 128);  // everyone's copies, and nobody in the panel before
+            send();
+          } else {
+            tc::bar_sync(1 + fg, 128);
+            send();
+            arrived(0);
+            tc::bar_sync(1 + fg, 128);
+          }
+        }
+        // (first: it says that every panel before has been through its slot, so
+        // that the slot's barrier is at this panel)
+        if (q > 1) wait(spent(fg), (q >> 1) - 1);
+        if (tma_boxes > 0) wait(full(slot), q / p.slots);
+        const char* const from = s_slots + slot * slot_bytes;
+        char* const set = s_sets + fg * set_bytes;
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const int b = 2 * it + (tid >> 6);
+          if (b < boxes) {
+            const bool is_v = b >= p.kx;
+            Chunk<float> v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = 4 * rg + i;
+              v[i].q = row < cur.n
+                           ? *reinterpret_cast<const uint4*>(from + b * kBox + chunk_at(row, c))
+                           : make_uint4(0, 0, 0, 0);
+            }
+            if (is_v) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int row = 4 * rg + i;
+                if (HAS_Y) {
+                  Chunk<float> z;
+                  z.q = *reinterpret_cast<const uint4*>(from + (b + p.mx) * kBox + chunk_at(row, c));
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    v[i].v[j] = row < cur.n ? through<ACT>(v[i].v[j], z.v[j]) : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) db[it][j] += v[i].v[j];
+              }
+            }
+            // values, and as many bytes behind all of them their low parts
+            char* const to = set + (is_v ? (p.kx + b) * kBox : b * kBox);
+            const int low = (is_v ? p.mx : p.kx) * kBox;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              Chunk<float> t;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) t.v[i] = v[i].v[j];
+              char* const at = to + chunk_at(4 * c + j, rg);
+              *reinterpret_cast<uint4*>(at) = t.q;
+              put_low(at + low, t);
+            }
+          }
+        }
+        tc::fence_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tc::arrive(ready(fg));
+          if (tma_boxes > 0) tc::arrive(free_(slot));
+        }
+      }
+      if (nxt.n == 0 || nxt.g != cur.g) {  // v_b: this group's and half's share
+        if (p.biases && k0 == 0) {
+          float* const to = p.part +
+                            (int64_t)(blockIdx.x + cur.g) * M * (K + kBiasCopies32) +
+                            (int64_t)M * K + (int64_t)(2 * fg + ((tid >> 5) & 1)) * M + m0;
+#pragma unroll
+          for (int it = 0; it < ITS; ++it) {
+            const int col = (2 * it + (tid >> 6) - p.kx) * 32 + c * 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float b = db[it][j];
+              b += __shfl_xor_sync(0xffffffffu, b, 8);
+              b += __shfl_xor_sync(0xffffffffu, b, 16);
+              if (lane < 8 && col >= 0 && col + j < mn) to[col + j] = b;
+            }
+          }
+        }
+#pragma unroll
+        for (int it = 0; it < ITS; ++it)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) db[it][j] = 0.0f;
+      }
+      slot = slot + 1 == p.slots ? 0 : slot + 1;
+      ++q;
+      cur = nxt;
+    }
+    if (copies) arrived(0);
+  } else {
+    // ------------------------------------------------------------- back warps
+    constexpr int HALF = NT / 2;
+    const int bw = warp - 8, row0 = (bw & 3) * 32, c0 = (bw >> 2) * HALF;
+    float acc[HALF];
+#pragma unroll
+    for (int i = 0; i < HALF; ++i) acc[i] = 0.0f;
+    int held = 0, sums = 0;
+    Run cur = after(none);
+    while (cur.n > 0) {
+      const Run nxt = after(cur);
+      const bool last = nxt.n == 0 || nxt.g != cur.g;
+      if (++held == kFlush || last) {
+        const int buf = sums & 1;
+        wait(made(buf), sums >> 1);
+        tc::fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < HALF; c += 16) {
+          if (c0 + c >= mn) break;
+          float v[16], u[16];
+          const uint32_t from = tmem + buf * 2 * NT + ((uint32_t)row0 << 16) + c0 + c;
+          tc::load16(from, v);
+          tc::load16(from + NT, u);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[c + i] += fabsf(v[i]) < INFINITY ? v[i] + u[i] : v[i];
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) tc::arrive(taken(buf));
+        ++sums;
+        held = 0;
+        if (last) {
+          float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * M * (K + kBiasCopies32) +
+                            (int64_t)(m0 + c0) * K + k0 + row0 + lane;
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) {
+            if (row0 + lane < kn && c0 + i < mn) to[(int64_t)i * K] = acc[i];
+            acc[i] = 0.0f;
+          }
+        }
+      }
+      cur = nxt;
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 0) tc::dealloc(tmem, 4 * NT);
 }
 
 // ------------------------------------------------- the whole backward, 16 bits
@@ -1432,17 +1759,17 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 }
 
 // v_W and v_b of a group: the places of the CTAs that had rows of it, in
-// order.  A block takes 256 / SHARES values; its warps take a share of the
+// order; a place has M x K sums and `copies` rows of M sums.  A block takes 256 / SHARES values; its warps take a share of the
 // places each, and the shares are added in order.
 template <typename T, int SHARES>
-__global__ void __launch_bounds__(256) join_kernel(Shape s, int parts,
+__global__ void __launch_bounds__(256) join_kernel(Shape s, int parts, int copies,
                                                    const int32_t* __restrict__ off,
                                                    const float* __restrict__ part,
                                                    T* __restrict__ vw, T* __restrict__ vb) {
   constexpr int VALUES = 256 / SHARES;
   __shared__ float s_sum[SHARES][VALUES];
   const int g = blockIdx.y, share = threadIdx.x / VALUES, at = threadIdx.x % VALUES;
-  const int64_t mk = (int64_t)s.M * s.K, each = mk + s.M;
+  const int64_t mk = (int64_t)s.M * s.K, each = mk + s.M, place = mk + (int64_t)copies * s.M;
   const int64_t i = (int64_t)blockIdx.x * VALUES + at;
   const int64_t r0 = max((int64_t)__ldg(off + g), (int64_t)0);
   const int64_t r1 = min((int64_t)__ldg(off + g + 1), s.R);
@@ -1452,9 +1779,14 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int parts,
     auto part_of = [&](int64_t r) { return (int)(((r / kTile + 1) * parts - 1) / tiles); };
     const int b0 = part_of(r0), n = part_of(r1 - 1) - b0 + 1;
     const int from = n * share / SHARES, to = n * (share + 1) / SHARES;
-    const float* p = part + (int64_t)(b0 + g + from) * each + i;
+    const float* p = part + (int64_t)(b0 + g + from) * place + i;
+    if (i < mk) {
 #pragma unroll 8
-    for (int b = from; b < to; ++b, p += each) sum += __ldg(p);
+      for (int b = from; b < to; ++b, p += place) sum += __ldg(p);
+    } else {
+      for (int b = from; b < to; ++b, p += place)
+        for (int c = 0; c < copies; ++c) sum += __ldg(p + (int64_t)c * s.M);
+    }
   }
   if (SHARES > 1) {
     s_sum[share][at] = sum;
@@ -1514,9 +1846,10 @@ int allow_smem() {
   return GS_OK;
 }
 
-// A map of rows [n, depth] in boxes of 128 rows x 128 bytes, swizzled as the
-// operands are; what lies outside reads as zeros.
-int make_map(CUtensorMap* map, const void* rows, int dtype, int64_t n, int depth) {
+// A map of rows [n, depth] in boxes of `tall` rows x 128 bytes, swizzled as
+// the operands are; what lies outside reads as zeros.
+int make_map(CUtensorMap* map, const void* rows, int dtype, int64_t n, int depth,
+             int tall = kTile) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                               const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -1536,7 +1869,7 @@ int make_map(CUtensorMap* map, const void* rows, int dtype, int64_t n, int depth
   }
   const cuuint64_t es = dtype == GS_F32 ? 4 : 2;
   const cuuint64_t dims[2] = {(cuuint64_t)depth, (cuuint64_t)n}, pitch[1] = {depth * es};
-  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), kTile}, ones[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)tall}, ones[2] = {1, 1};
   const CUtensorMapDataType type = dtype == GS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : dtype == GS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -1620,6 +1953,7 @@ bool dims_fit_both(int K, int M) { return K <= 128 && M <= 128 && K % 8 == 0 && 
 // the fp32 sums of shared rows for the 16-bit types.
 struct Plan {
   int nt, kt, mt, parts;
+  int copies;  // of v_b's sums in a place
   size_t part_floats, sum_floats;
 };
 
@@ -1633,18 +1967,57 @@ Plan plan_of(const gs_grouped_params* p) {  // one CTA an SM, or two
   int64_t n = (int64_t)sm_count() * (two ? 2 : 1) / ((int64_t)q.kt * q.mt);
   n = n < 1 ? 1 : n > tiles ? tiles : n;
   q.parts = (int)n;
-  q.part_floats = ((size_t)q.parts + p->groups) * p->out_features * ((size_t)p->in_features + 1);
+  q.copies = p->dtype == GS_F32 ? kBiasCopies32 : 1;
+  q.part_floats =
+      ((size_t)q.parts + p->groups) * p->out_features * ((size_t)p->in_features + q.copies);
   q.sum_floats = p->use_row_ids && p->dtype != GS_F32 ? (size_t)p->n * p->in_features : 0;
   q.part_floats = (q.part_floats + 63) / 64 * 64;  // the sums start on 256 bytes
   return q;
+}
+
+template <int ACT, int NT>
+int launch_weights32(const Shape& s, const void* x, const void* y, const void* vy,
+                     const int32_t* ids, const int32_t* off, float* part, const void* vb,
+                     const Plan& q, cudaStream_t st) {
+  constexpr auto kernel = weights32_kernel<ACT, NT>;
+  constexpr int kAll = 227 * 1024;  // this kernel has no static shared memory
+  if (int rc = allow_smem<kernel, kAll>()) return rc;
+  if ((int64_t)q.kt * q.mt > 65535) return invalid("grouped_linear: too many features");
+  Weight32Args p{};
+  p.s = s;
+  p.x = static_cast<const float*>(x), p.y = static_cast<const float*>(y);
+  p.vy = static_cast<const float*>(vy), p.ids = ids, p.off = off, p.part = part;
+  p.kt = q.kt, p.biases = vb != nullptr;
+  p.kx = ((s.K < 128 ? s.K : 128) + 31) / 32, p.mx = ((s.M < NT ? s.M : NT) + 31) / 32;
+  const bool wide_x = s.K % 4 == 0 && on16(x);
+  p.x_mode = wide_x ? (ids ? 1 : 0) : 2;
+  p.v_mode = s.M % 4 == 0 && on16(vy) && (!y || on16(y)) ? 0 : 2;
+  const int set = 2 * (p.kx + p.mx) * kBox, slot = (p.kx + p.mx * (ACT ? 2 : 1)) * kBox;
+  const int fixed = 2 * set + 24 * 8 + 8;
+  // an x operand's MMA reads 128 rows from its start on: they lie in the sets
+  // and slots behind it
+  p.slots = (kAll - fixed) / slot;
+  p.slots = p.slots > 8 ? 8 : p.slots;
+  if (p.x_mode || p.v_mode) p.slots = p.slots / 2 * 2;
+  CUtensorMap map_x{}, map_v{}, map_y{};
+  if (p.x_mode == 0)
+    if (int rc = make_map(&map_x, x, GS_F32, s.R, s.K, kRows32)) return rc;
+  if (p.v_mode == 0) {
+    if (int rc = make_map(&map_v, vy, GS_F32, s.R, s.M, kRows32)) return rc;
+    if (ACT)
+      if (int rc = make_map(&map_y, y, GS_F32, s.R, s.M, kRows32)) return rc;
+  }
+  kernel<<<dim3((unsigned)q.parts, (unsigned)(q.kt * q.mt)), 2 * kThreads + 64,
+           fixed + p.slots * slot, st>>>(p, map_x, map_v, map_y);
+  return launch_status("grouped_linear_bwd");
 }
 
 template <typename T, int ACT, int NT, bool SPLIT>
 int launch_weights(const WeightArgs& p, const Plan& q, cudaStream_t st) {
   constexpr auto kernel = weights_mma_kernel<T, ACT, NT, SPLIT>;
   if (int rc = allow_smem<kernel>()) return rc;
-  const int xt = sizeof(T) == 4 ? 2 : 1, vt = sizeof(T) == 4 || SPLIT ? 2 : 1;
-  const int smem = 1024 + xt * kPanel + vt * NT * 128, columns = NT * vt;
+  const int vt = SPLIT ? 2 : 1;
+  const int smem = 1024 + kPanel + vt * NT * 128, columns = NT * vt;
   if ((int64_t)q.kt * q.mt > 65535) return invalid("grouped_linear: too many features");
   kernel<<<dim3((unsigned)q.parts, (unsigned)(q.kt * q.mt)), kThreads, smem, st>>>(p, columns);
   return launch_status("grouped_linear_bwd");
@@ -1732,7 +2105,13 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
                                                                 static_cast<T*>(vx));
   }
   if (vw || vb) {
-    if (s.R > 0 && !both) {
+    if constexpr (sizeof(T) == 4) {
+      if (s.R > 0) {
+        const int rc = q.nt == 64 ? launch_weights32<ACT, 64>(s, x, y, vy, ids, off, ws, vb, q, st)
+                                  : launch_weights32<ACT, 128>(s, x, y, vy, ids, off, ws, vb, q, st);
+        if (rc) return rc;
+      }
+    } else if (s.R > 0 && !both) {
       WeightArgs p{};
       p.s = s;
       p.x = x, p.y = y, p.vy = vy, p.ids = ids, p.off = off, p.part = ws;
@@ -1746,12 +2125,12 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
     const int64_t each = (int64_t)s.M * (s.K + 1);
     if (s.G > 65535) return invalid("grouped_linear: more than 65535 groups");
     // about parts / G places a group: few are not worth sharing out
-    if (q.parts < 16 * (int64_t)s.G)
+    if (q.parts < 8 * (int64_t)s.G)
       join_kernel<T, 1><<<dim3((unsigned)ceil_div(each, 256), (unsigned)s.G), 256, 0, st>>>(
-          s, q.parts, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
+          s, q.parts, q.copies, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
     else
       join_kernel<T, 8><<<dim3((unsigned)ceil_div(each, 32), (unsigned)s.G), 256, 0, st>>>(
-          s, q.parts, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
+          s, q.parts, q.copies, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
   }
   return launch_status("grouped_linear_bwd");
 }
