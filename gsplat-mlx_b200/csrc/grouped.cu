@@ -13,6 +13,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <climits>
 #include <type_traits>
 
 #include "common.cuh"
@@ -1066,10 +1067,12 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   Run none;
   none.row = (int)(first_tile(tiles, gridDim.x, blockIdx.x) * kTile);
   none.n = 0, none.g = -1, none.group_end = 0;
-  auto after = [&](Run t) {  // skips rows outside every group
-    t = run_from(p.off, p.s.G, t.row + t.n, end, kRows32, t);
+  // all of this CTA's rows of the next group; rows outside every group are
+  // skipped
+  auto after = [&](Run t) {
+    t = run_from(p.off, p.s.G, t.row + t.n, end, INT_MAX, t);
     while (t.n > 0 && (t.g < 0 || t.g >= p.s.G))
-      t = run_from(p.off, p.s.G, t.group_end, end, kRows32, t);
+      t = run_from(p.off, p.s.G, t.group_end, end, INT_MAX, t);
     return t;
   };
   const int tma_boxes = (p.x_mode == 0 ? p.kx : 0) + (p.v_mode == 0 ? p.mx * (HAS_Y ? 2 : 1) : 0);
@@ -1078,33 +1081,33 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     // ------------------------------------------------------------- TMA
     if (tma_boxes > 0) {
       int slot = 0, q = 0;
-      for (Run cur = after(none); cur.n > 0; cur = after(cur), ++q) {
-        if (q >= p.slots) wait(free_(slot), q / p.slots - 1);
-        if (tc::elected()) {
-          const uint32_t to = tc::smem_addr(s_slots + slot * slot_bytes);
-          tc::expect(full(slot), tma_boxes * kBox);
-          if (p.x_mode == 0)
-            for (int j = 0; j < p.kx; ++j)
-              tc::load_box(to + j * kBox, &map_x, k0 + j * 32, cur.row, full(slot));
-          if (p.v_mode == 0)
-            for (int j = 0; j < p.mx; ++j) {
-              tc::load_box(to + (p.kx + j) * kBox, &map_v, m0 + j * 32, cur.row, full(slot));
-              if (HAS_Y)
-                tc::load_box(to + (boxes + j) * kBox, &map_y, m0 + j * 32, cur.row, full(slot));
-            }
+      for (Run cur = after(none); cur.n > 0; cur = after(cur))
+        for (int row = cur.row; row < cur.row + cur.n; row += kRows32, ++q) {
+          if (q >= p.slots) wait(free_(slot), q / p.slots - 1);
+          if (tc::elected()) {
+            const uint32_t to = tc::smem_addr(s_slots + slot * slot_bytes);
+            tc::expect(full(slot), tma_boxes * kBox);
+            if (p.x_mode == 0)
+              for (int j = 0; j < p.kx; ++j)
+                tc::load_box(to + j * kBox, &map_x, k0 + j * 32, row, full(slot));
+            if (p.v_mode == 0)
+              for (int j = 0; j < p.mx; ++j) {
+                tc::load_box(to + (p.kx + j) * kBox, &map_v, m0 + j * 32, row, full(slot));
+                if (HAS_Y)
+                  tc::load_box(to + (boxes + j) * kBox, &map_y, m0 + j * 32, row, full(slot));
+              }
+          }
+          __syncwarp();
+          slot = slot + 1 == p.slots ? 0 : slot + 1;
         }
-        __syncwarp();
-        slot = slot + 1 == p.slots ? 0 : slot + 1;
-      }
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
     const uint32_t idesc = tc::instr_desc(tc::kTF32, (mn + 15) / 16 * 16);
     const uint32_t leader = tc::elected();
     int q = 0, held = 0, sums = 0;
-    Run cur = after(none);
-    while (cur.n > 0) {
-      const Run nxt = after(cur);
+    for (Run cur = after(none); cur.n > 0; cur = after(cur))
+    for (int left = cur.n; left > 0; left -= kRows32, ++q) {
       const int set = q & 1, buf = sums & 1;
       wait(ready(set), q >> 1);
       if (held == 0 && sums > 1) wait(taken(buf), (sums >> 1) - 1);
@@ -1114,7 +1117,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       const uint32_t v_at = x_at + 2 * p.kx * kBox;
       const uint64_t vh = tc::smem_desc(v_at), vl = tc::smem_desc(v_at + p.mx * kBox);
       const uint32_t acc = tmem + buf * 2 * NT;
-      const int steps = (cur.n + 7) / 8;
+      const int steps = (left + 7) / 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i >= steps) break;
@@ -1126,13 +1129,11 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         tc::mma<true>(leader, acc, xh + at, vh + at, idesc, more);
       }
       tc::commit(leader, spent(set));
-      if (++held == kFlush || nxt.n == 0 || nxt.g != cur.g) {
+      if (++held == kFlush || left <= kRows32) {
         tc::commit(leader, made(buf));
         ++sums;
         held = 0;
       }
-      ++q;
-      cur = nxt;
     }
     if (q > 0) wait(spent((q - 1) & 1), (q - 1) >> 1);
   } else if (warp < 8) {
@@ -1140,16 +1141,27 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     const int fg = warp >> 2, tid = threadIdx.x & 127;
     const bool copies = p.x_mode != 0 || p.v_mode != 0;
     const int own = p.slots / 2;  // with copies: this group's slots
-    auto second = [&](const Run& t) { return after(after(t)); };
     // copies: rows r16 and r16 + 16, chunk c16, of every box
     const int r16 = tid >> 3, c16 = tid & 7;
-    Run ahead = none;
-    int ahead_i = 0, id[2];
-    auto read_ids = [&](const Run& t) {
+    Run ahead = none;           // the rows that are copied next: from ahead_row on
+    int ahead_row = 0, ahead_i = 0, id[2];
+    auto forward = [&](int panels) {  // moves on, to this group's next panel
+      for (; panels > 0 && ahead.n > 0; --panels) {
+        ahead_row += kRows32;
+        if (ahead_row >= ahead.row + ahead.n) {
+          ahead = after(ahead);
+          ahead_row = ahead.row;
+        }
+      }
+      // (no use of what is read here: it is on its way until the next copies)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int row = r16 + 16 * i;
-        id[i] = row >= t.n ? -1 : p.ids ? __ldg(p.ids + t.row + row) : t.row + row;
+        const int row = ahead_row + r16 + 16 * i;
+        id[i] = -1;
+        if (row < ahead.row + ahead.n) {
+          if (p.ids) id[i] = __ldg(p.ids + row);
+          else id[i] = row;
+        }
       }
     };
     auto send = [&]() {
@@ -1169,8 +1181,8 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
             }
           }
           if (p.v_mode != 0) {
-            const bool ok = row < ahead.n;
-            const int64_t from = ok ? (int64_t)(ahead.row + row) * M + m0 + c16 * 4 : 0;
+            const bool ok = ahead_row + row < ahead.row + ahead.n;
+            const int64_t from = ok ? (int64_t)(ahead_row + row) * M + m0 + c16 * 4 : 0;
             for (int j = 0; j < p.mx; ++j) {
               const int there = ok ? mn - j * 32 - c16 * 4 : 0;
               send_chunk<float, false>(to + (p.kx + j) * kBox + o, p.vy + from + j * 32, there);
@@ -1180,15 +1192,14 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
           }
         }
         ahead_i = ahead_i + 1 == own ? 0 : ahead_i + 1;
-        ahead = second(ahead);
-        read_ids(ahead);
+        forward(2);
       }
       send_done();
     };
-    Run cur = after(none);
     if (copies) {
-      ahead = fg ? after(cur) : cur;
-      read_ids(ahead);
+      ahead = after(none);
+      ahead_row = ahead.row;
+      forward(fg);
       for (int i = 1; i < own; ++i) send();
     }
     // this thread's 4 x 4 blocks: of boxes 2 it + (tid >> 6)
@@ -1200,9 +1211,10 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j) db[it][j] = 0.0f;
     int slot = 0, q = 0;
-    while (cur.n > 0) {
-      const Run nxt = after(cur);
-      if ((q & 1) == fg) {
+    for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
+      for (int left = cur.n; left > 0;
+           left -= kRows32, ++q, slot = slot + 1 == p.slots ? 0 : slot + 1) {
+        if ((q & 1) != fg) continue;
         if (copies) {
           if (own > 1) {
             arrived(own - 2);
@@ -1230,7 +1242,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int row = 4 * rg + i;
-              v[i].q = row < cur.n
+              v[i].q = row < left
                            ? *reinterpret_cast<const uint4*>(from + b * kBox + chunk_at(row, c))
                            : make_uint4(0, 0, 0, 0);
             }
@@ -1243,7 +1255,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
                   z.q = *reinterpret_cast<const uint4*>(from + (b + p.mx) * kBox + chunk_at(row, c));
 #pragma unroll
                   for (int j = 0; j < 4; ++j)
-                    v[i].v[j] = row < cur.n ? through<ACT>(v[i].v[j], z.v[j]) : 0.0f;
+                    v[i].v[j] = row < left ? through<ACT>(v[i].v[j], z.v[j]) : 0.0f;
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) db[it][j] += v[i].v[j];
@@ -1270,31 +1282,25 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
           if (tma_boxes > 0) tc::arrive(free_(slot));
         }
       }
-      if (nxt.n == 0 || nxt.g != cur.g) {  // v_b: this group's and half's share
-        if (p.biases && k0 == 0) {
-          float* const to = p.part +
-                            (int64_t)(blockIdx.x + cur.g) * M * (K + kBiasCopies32) +
-                            (int64_t)M * K + (int64_t)(2 * fg + ((tid >> 5) & 1)) * M + m0;
+      if (p.biases && k0 == 0) {  // v_b: this front group's and half's share
+        float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * M * (K + kBiasCopies32) +
+                          (int64_t)M * K + (int64_t)(2 * fg + ((tid >> 5) & 1)) * M + m0;
 #pragma unroll
-          for (int it = 0; it < ITS; ++it) {
-            const int col = (2 * it + (tid >> 6) - p.kx) * 32 + c * 4;
+        for (int it = 0; it < ITS; ++it) {
+          const int col = (2 * it + (tid >> 6) - p.kx) * 32 + c * 4;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float b = db[it][j];
-              b += __shfl_xor_sync(0xffffffffu, b, 8);
-              b += __shfl_xor_sync(0xffffffffu, b, 16);
-              if (lane < 8 && col >= 0 && col + j < mn) to[col + j] = b;
-            }
+          for (int j = 0; j < 4; ++j) {
+            float b = db[it][j];
+            b += __shfl_xor_sync(0xffffffffu, b, 8);
+            b += __shfl_xor_sync(0xffffffffu, b, 16);
+            if (lane < 8 && col >= 0 && col + j < mn) to[col + j] = b;
           }
         }
-#pragma unroll
-        for (int it = 0; it < ITS; ++it)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) db[it][j] = 0.0f;
       }
-      slot = slot + 1 == p.slots ? 0 : slot + 1;
-      ++q;
-      cur = nxt;
+#pragma unroll
+      for (int it = 0; it < ITS; ++it)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) db[it][j] = 0.0f;
     }
     if (copies) arrived(0);
   } else {
@@ -1304,12 +1310,9 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     float acc[HALF];
 #pragma unroll
     for (int i = 0; i < HALF; ++i) acc[i] = 0.0f;
-    int held = 0, sums = 0;
-    Run cur = after(none);
-    while (cur.n > 0) {
-      const Run nxt = after(cur);
-      const bool last = nxt.n == 0 || nxt.g != cur.g;
-      if (++held == kFlush || last) {
+    int sums = 0;
+    for (Run cur = after(none); cur.n > 0; cur = after(cur))
+      for (int left = cur.n; left > 0; left -= kFlush * kRows32) {
         const int buf = sums & 1;
         wait(made(buf), sums >> 1);
         tc::fence_after_sync();
@@ -1327,8 +1330,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         __syncwarp();
         if (lane == 0) tc::arrive(taken(buf));
         ++sums;
-        held = 0;
-        if (last) {
+        if (left <= kFlush * kRows32) {
           float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * M * (K + kBiasCopies32) +
                             (int64_t)(m0 + c0) * K + k0 + row0 + lane;
 #pragma unroll
@@ -1338,8 +1340,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
           }
         }
       }
-      cur = nxt;
-    }
   }
   tc::fence_before_sync();
   __syncthreads();
