@@ -1802,6 +1802,271 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int parts, int copie
   }
 }
 
+// --------------------------------------------------------- few outputs (colours)
+//
+// Up to 8 outputs (a colour has 3) and rows of up to 512 bytes: a tensor-core
+// tile would be nearly all padding (32-3 fp32: 16 MMAs of 128 x 16 a panel took
+// 1000 cycles, the panel's 16 KB come in 370).  Here `lpr` neighbouring lanes
+// take a row, 16 bytes each; a lane keeps its columns of the group's weights
+// in registers, and of v_W's sums in the backward, which does all of its parts
+// in the one pass.  A warp has 16 / MP rows per lane in flight.
+struct NarrowArgs {
+  Shape s;
+  const void* x;
+  const int32_t* ids;
+  const int32_t* off;
+  const void* w;
+  const void* bias;
+  void* y;             // written by the forward, read by the backward
+  const void* vy;
+  void* vx;            // v_x, its fp32 sums with row ids, or NULL
+  float* part;         // as in WeightArgs, or NULL
+  int lpr;             // a power of two
+  int act;
+};
+
+__device__ __forceinline__ float activate_as(int act, float z) {
+  return act == GS_ACT_RELU ? activate<GS_ACT_RELU>(z)
+                            : act == GS_ACT_SIGMOID ? activate<GS_ACT_SIGMOID>(z) : z;
+}
+__device__ __forceinline__ float through_as(int act, float v, float y) {
+  return act == GS_ACT_RELU ? through<GS_ACT_RELU>(v, y)
+                            : act == GS_ACT_SIGMOID ? through<GS_ACT_SIGMOID>(v, y) : v;
+}
+
+// The spans of this CTA's rows that belong together, and this lane's place.
+#define NARROW_SETUP                                                                        \
+  constexpr int E = Chunk<T>::E, U = 16 / MP;                                               \
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;                               \
+  const int K = p.s.K, M = p.s.M;                                                           \
+  const int c = lane & (p.lpr - 1), rg = lane / p.lpr, set = 32 / p.lpr; /* rows at once */ \
+  const T* const x = static_cast<const T*>(p.x);                                            \
+  const T* const w = static_cast<const T*>(p.w);                                            \
+  const int there = K - c * E; /* columns of this lane: none, some or E */                  \
+  const int64_t tiles = (p.s.R + kTile - 1) / kTile;                                        \
+  const int end = (int)min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);    \
+  Run none;                                                                                 \
+  none.row = (int)(first_tile(tiles, gridDim.x, blockIdx.x) * kTile);                       \
+  none.n = 0, none.g = -1, none.group_end = 0;                                              \
+  auto after = [&](const Run& t) {                                                          \
+    return run_from(p.off, p.s.G, t.row + t.n, end, INT_MAX, t);                            \
+  };                                                                                        \
+  float wk[MP][E];                                                                          \
+  auto read_weights = [&](int g) {                                                          \
+    _Pragma("unroll") for (int m = 0; m < MP; ++m) {                                        \
+      Chunk<T> q;                                                                           \
+      q.q = get_chunk<T, WIDE>(w + ((int64_t)g * M + (m < M ? m : 0)) * K +                 \
+                                   (there > 0 ? c * E : 0), m < M ? there : 0);             \
+      _Pragma("unroll") for (int e = 0; e < E; ++e) wk[m][e] = to_f(q.v[e]);                \
+    }                                                                                       \
+  };                                                                                        \
+  int id[U];                                                                                \
+  auto read_ids = [&](int r, int stop) { /* no use of what is read yet */                   \
+    _Pragma("unroll") for (int u = 0; u < U; ++u) {                                         \
+      const int row = r + u * set + rg;                                                     \
+      id[u] = -1;                                                                           \
+      if (row < stop) {                                                                     \
+        if (p.ids) id[u] = __ldg(p.ids + row);                                              \
+        else id[u] = row;                                                                   \
+      }                                                                                     \
+    }                                                                                       \
+  };
+
+// A lane keeps H of its 2 H values, with the partner's share of them.
+template <int H>
+__device__ __forceinline__ void hand_over(float (&v)[16], int lane, int o, int& n, int& first) {
+  const bool up = lane & o;
+#pragma unroll
+  for (int i = 0; i < H; ++i) {
+    const float mine = up ? v[i + H] : v[i];
+    v[i] = mine + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + H], o);
+  }
+  n = H;
+  first += up ? H : 0;
+}
+
+template <typename T, int MP, bool WIDE>
+__global__ void __launch_bounds__(256, MP == 4 && sizeof(T) == 4 ? 4 : 2) narrow_fwd_kernel(NarrowArgs p) {
+  NARROW_SETUP
+  const T* const bias = static_cast<const T*>(p.bias);
+  T* const y = static_cast<T*>(p.y);
+  for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
+    const int stop = cur.row + cur.n;
+    if (cur.g < 0 || cur.g >= p.s.G) {
+      for (int64_t i = (int64_t)cur.row * M + threadIdx.x; i < (int64_t)stop * M; i += 256)
+        y[i] = from_f<T>(0.0f);
+      continue;
+    }
+    read_weights(cur.g);
+    int r = cur.row + warp * U * set;
+    read_ids(r, stop);
+    for (; r < stop; r += 8 * U * set) {
+      Chunk<T> q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool ok = id[u] >= 0 && id[u] < p.s.n && there > 0;
+        q[u].q = get_chunk<T, WIDE>(x + (ok ? (int64_t)id[u] * K + c * E : 0), ok ? there : 0);
+      }
+      read_ids(r + 8 * U * set, stop);
+      float v[16];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int m = 0; m < MP; ++m) {
+          float a = 0.0f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) a = fmaf(to_f(q[u].v[e]), wk[m][e], a);
+          v[u * MP + m] = a;
+        }
+      // The row's lanes add up their parts; each step a lane hands half of its
+      // values to the partner and adds the partner's other half, until lane
+      // c has the 16 / lpr values from c 16 / lpr on (one, twice, for 32).
+      int n = 16, first = 0;
+      if (p.lpr > 1) hand_over<8>(v, lane, p.lpr >> 1, n, first);
+      if (p.lpr > 2) hand_over<4>(v, lane, p.lpr >> 2, n, first);
+      if (p.lpr > 4) hand_over<2>(v, lane, p.lpr >> 3, n, first);
+      if (p.lpr > 8) hand_over<1>(v, lane, p.lpr >> 4, n, first);
+      if (p.lpr > 16) {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
+        if (lane & 1) n = 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (i >= n) break;
+        const int m = (first + i) % MP, row = r + (first + i) / MP * set + rg;
+        if (m < M && row < stop) {
+          const float b = bias ? to_f(__ldg(bias + (int64_t)cur.g * M + m)) : 0.0f;
+          y[(int64_t)row * M + m] = from_f<T>(activate_as(p.act, v[i] + b));
+        }
+      }
+    }
+  }
+}
+
+// E values to p, `there` of them.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void set_chunk(T* p, const float* f, int there) {
+  constexpr int E = Chunk<T>::E;
+  if (WIDE) {
+    if (there > 0) {
+      if constexpr (E == 4)
+        *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+      else
+        *reinterpret_cast<uint4*>(p) = round_chunk<T>(f);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e < there) p[e] = from_f<T>(f[e]);
+  }
+}
+
+template <typename T, int MP, bool WIDE>
+__global__ void __launch_bounds__(256, 2) narrow_bwd_kernel(NarrowArgs p) {
+  NARROW_SETUP
+  __shared__ float s_part[8][32];
+  const T* const y = static_cast<const T*>(p.y);
+  const T* const vy = static_cast<const T*>(p.vy);
+  for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
+    const int stop = cur.row + cur.n;
+    if (cur.g < 0 || cur.g >= p.s.G) {
+      if (p.vx && !p.ids)
+        for (int64_t i = (int64_t)cur.row * K + threadIdx.x; i < (int64_t)stop * K; i += 256)
+          static_cast<T*>(p.vx)[i] = from_f<T>(0.0f);
+      continue;
+    }
+    read_weights(cur.g);
+    float sum[MP][E], db[MP];
+#pragma unroll
+    for (int m = 0; m < MP; ++m) {
+      db[m] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum[m][e] = 0.0f;
+    }
+    int r = cur.row + warp * U * set;
+    read_ids(r, stop);
+    for (; r < stop; r += 8 * U * set) {
+      Chunk<T> q[U];
+      float vz[U][MP];
+      bool ok[U];
+      int64_t to[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int row = r + u * set + rg;
+        ok[u] = id[u] >= 0 && id[u] < p.s.n && there > 0;
+        to[u] = ok[u] ? (int64_t)id[u] * K + c * E : 0;
+        if (p.part) q[u].q = get_chunk<T, WIDE>(x + to[u], ok[u] ? there : 0);
+#pragma unroll
+        for (int m = 0; m < MP; ++m) {
+          const bool in = m < M && row < stop;
+          const int64_t at = in ? (int64_t)row * M + m : 0;
+          vz[u][m] = in ? to_f(vy[at]) : 0.0f;
+          if (p.act) vz[u][m] = in ? through_as(p.act, vz[u][m], to_f(y[at])) : 0.0f;
+        }
+      }
+      read_ids(r + 8 * U * set, stop);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (p.vx && ok[u]) {
+          float f[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            f[e] = 0.0f;
+#pragma unroll
+            for (int m = 0; m < MP; ++m) f[e] = fmaf(vz[u][m], wk[m][e], f[e]);
+          }
+          if (!p.ids) {
+            set_chunk<T, WIDE>(static_cast<T*>(p.vx) + to[u], f, there);
+          } else {
+            float* const at = static_cast<float*>(p.vx) + to[u];
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+              if (WIDE) {  // 16 bytes of T: K is a multiple of 4, and the sums are aligned
+                asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};"
+                             ::"l"(at + e), "f"(f[e]), "f"(f[e + 1]), "f"(f[e + 2]), "f"(f[e + 3])
+                             : "memory");
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (e + i < there) atomicAdd(at + e + i, f[e + i]);
+              }
+            }
+          }
+        }
+        if (p.part) {
+#pragma unroll
+          for (int m = 0; m < MP; ++m) {
+            db[m] += vz[u][m];
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum[m][e] = fmaf(vz[u][m], to_f(q[u].v[e]), sum[m][e]);
+          }
+        }
+      }
+    }
+    if (!p.part) continue;
+    // over the warp's rows, then over the warps, in order
+    float* const place = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1));
+#pragma unroll
+    for (int m = 0; m < MP; ++m) {
+      if (m >= M) break;
+#pragma unroll
+      for (int e = 0; e <= E; ++e) {  // E: v_b
+        float a = e < E ? sum[m][e < E ? e : 0] : db[m];
+        for (int o = p.lpr; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        __syncthreads();
+        s_part[warp][lane] = a;
+        __syncthreads();
+        if (warp == 0 && rg == 0) {
+#pragma unroll
+          for (int i = 1; i < 8; ++i) a += s_part[i][lane];
+          if (e < E && e < there) place[(int64_t)m * K + c * E + e] = a;
+          if (e == E && c == 0) place[(int64_t)M * K + m] = a;
+        }
+      }
+    }
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) round_kernel(int64_t n, const float* __restrict__ a,
                                                     T* __restrict__ b) {
@@ -1935,9 +2200,49 @@ int launch_rows(const RowsArgs& p, cudaStream_t st) {
   return launch_rows<T, ACT, MODE, kTma, true, SPLIT>(p, st);
 }
 
+// Few outputs of rows of up to 32 chunks; the backward has to hold a lane's
+// weights and sums in registers.
+bool is_narrow(int K, int M, int dtype, bool backward) {
+  const int e = dtype == GS_F32 ? 4 : 8;
+  return M <= (backward && dtype != GS_F32 ? 4 : 8) && K <= 32 * e;
+}
+
+template <typename T>
+int launch_narrow(NarrowArgs p, bool backward, int parts, cudaStream_t st) {
+  const int chunks = (int)ceil_div(p.s.K, 16 / (int)sizeof(T));
+  p.lpr = 1;
+  while (p.lpr < chunks) p.lpr *= 2;
+  const bool wide = p.s.K * sizeof(T) % 16 == 0 && on16(p.x) && on16(p.w) && (!p.vx || on16(p.vx));
+  const dim3 grid((unsigned)parts);
+  if (backward) {
+    if (p.s.M <= 4) {
+      if (wide) narrow_bwd_kernel<T, 4, true><<<grid, 256, 0, st>>>(p);
+      else narrow_bwd_kernel<T, 4, false><<<grid, 256, 0, st>>>(p);
+    } else if constexpr (sizeof(T) == 4) {
+      if (wide) narrow_bwd_kernel<T, 8, true><<<grid, 256, 0, st>>>(p);
+      else narrow_bwd_kernel<T, 8, false><<<grid, 256, 0, st>>>(p);
+    }
+  } else if (p.s.M <= 4) {
+    if (wide) narrow_fwd_kernel<T, 4, true><<<grid, 256, 0, st>>>(p);
+    else narrow_fwd_kernel<T, 4, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (wide) narrow_fwd_kernel<T, 8, true><<<grid, 256, 0, st>>>(p);
+    else narrow_fwd_kernel<T, 8, false><<<grid, 256, 0, st>>>(p);
+  }
+  return launch_status("grouped_linear");
+}
+
 template <typename T, int ACT>
 int run_fwd(const Shape& s, const void* x, const int32_t* ids, const int32_t* off, const void* w,
             const void* b, void* y, cudaStream_t st) {
+  if (is_narrow(s.K, s.M, dtype_of<T>, false)) {
+    NarrowArgs p{};
+    p.s = s;
+    p.x = x, p.ids = ids, p.off = off, p.w = w, p.bias = b, p.y = y, p.act = ACT;
+    const int64_t tiles = ceil_div(s.R, kTile), most =
+        (int64_t)sm_count() * (s.M <= 4 && sizeof(T) == 4 ? 4 : 2);
+    return launch_narrow<T>(p, false, (int)(tiles < most ? tiles : most), st);
+  }
   RowsArgs p{};
   p.s = s;
   p.a = x, p.ids = ids, p.off = off, p.w = w, p.bias = b, p.out = y;
@@ -1954,6 +2259,7 @@ bool dims_fit_both(int K, int M) { return K <= 128 && M <= 128 && K % 8 == 0 && 
 struct Plan {
   int nt, kt, mt, parts;
   int copies;  // of v_b's sums in a place
+  bool narrow;
   size_t part_floats, sum_floats;
 };
 
@@ -1963,11 +2269,13 @@ Plan plan_of(const gs_grouped_params* p) {  // one CTA an SM, or two
   q.kt = (int)ceil_div(p->in_features, 128);
   q.mt = (int)ceil_div(p->out_features, q.nt);
   const int64_t tiles = ceil_div(p->rows, kTile);
-  const bool two = p->dtype != GS_F32 && !(dims_fit_both(p->in_features, p->out_features));
+  q.narrow = is_narrow(p->in_features, p->out_features, p->dtype, true);
+  const bool two = q.narrow || (p->dtype != GS_F32 &&
+                                !dims_fit_both(p->in_features, p->out_features));
   int64_t n = (int64_t)sm_count() * (two ? 2 : 1) / ((int64_t)q.kt * q.mt);
   n = n < 1 ? 1 : n > tiles ? tiles : n;
   q.parts = (int)n;
-  q.copies = p->dtype == GS_F32 ? kBiasCopies32 : 1;
+  q.copies = p->dtype == GS_F32 && !q.narrow ? kBiasCopies32 : 1;
   q.part_floats =
       ((size_t)q.parts + p->groups) * p->out_features * ((size_t)p->in_features + q.copies);
   q.sum_floats = p->use_row_ids && p->dtype != GS_F32 ? (size_t)p->n * p->in_features : 0;
@@ -2068,7 +2376,23 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
   if (ACT == GS_ACT_NONE) y = nullptr;
   const bool shared = prm->use_row_ids != 0;
   float* const sum = sizeof(T) == 4 ? static_cast<float*>(vx) : ws + q.part_floats;
-  const bool both = (vw || vb) && fits_both<T>(s, x, w, y, vy, vx);
+  const bool both = !q.narrow && (vw || vb) && fits_both<T>(s, x, w, y, vy, vx);
+  if (q.narrow) {
+    if (vx && shared && cudaMemsetAsync(sum, 0, sizeof(float) * s.n * s.K, st) != cudaSuccess)
+      return launch_status("grouped_linear_bwd");
+    if (s.R > 0) {
+      NarrowArgs p{};
+      p.s = s;
+      p.x = x, p.ids = ids, p.off = off, p.w = w, p.act = ACT, p.vy = vy;
+      p.y = const_cast<void*>(y);
+      p.vx = !vx ? nullptr : shared ? sum : vx;
+      p.part = vw || vb ? ws : nullptr;
+      if (int rc = launch_narrow<T>(p, true, q.parts, st)) return rc;
+    }
+    if (vx && shared && sizeof(T) == 2 && s.n > 0)
+      round_kernel<T><<<grid_for(s.n * s.K, 256), 256, 0, st>>>(s.n * s.K, sum,
+                                                                static_cast<T*>(vx));
+  }
   if constexpr (sizeof(T) == 2) {
     if (both) {
       if (vx && shared && cudaMemsetAsync(sum, 0, sizeof(float) * s.n * s.K, st) != cudaSuccess)
@@ -2086,7 +2410,7 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
                                                                   static_cast<T*>(vx));
     }
   }
-  if (vx && !both) {
+  if (vx && !both && !q.narrow) {
     if (shared && cudaMemsetAsync(sum, 0, sizeof(float) * s.n * s.K, st) != cudaSuccess)
       return launch_status("grouped_linear_bwd");
     if (s.R > 0) {
@@ -2105,7 +2429,8 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
                                                                 static_cast<T*>(vx));
   }
   if (vw || vb) {
-    if constexpr (sizeof(T) == 4) {
+    if (q.narrow) {
+    } else if constexpr (sizeof(T) == 4) {
       if (s.R > 0) {
         const int rc = q.nt == 64 ? launch_weights32<ACT, 64>(s, x, y, vy, ids, off, ws, vb, q, st)
                                   : launch_weights32<ACT, 128>(s, x, y, vy, ids, off, ws, vb, q, st);
@@ -2149,12 +2474,15 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
     default: return f<__half, GS_ACT_SIGMOID>(__VA_ARGS__);                            \
   }
 
+// Rows are counted in 32 bits, some tiles past the last.
+constexpr int64_t kRowsMost = INT32_MAX - 4096;
+
 int bad_params(const gs_grouped_params* p) {
   if (!p || p->rows < 0 || p->n < 0 || p->groups < 1 || p->in_features < 1 ||
       p->out_features < 1)
     return invalid("grouped_linear: bad params");
-  if (p->rows >= INT32_MAX || p->n >= INT32_MAX)
-    return invalid("grouped_linear: 2^31 rows or more");
+  if (p->rows > kRowsMost || p->n > kRowsMost)
+    return invalid("grouped_linear: 2^31 - 4096 rows or more");
   if (!p->use_row_ids && p->n != p->rows)
     return invalid("grouped_linear: x has another number of rows");
   if (p->dtype < GS_F32 || p->dtype > GS_F16) return invalid("grouped_linear: unknown dtype");

@@ -77,8 +77,8 @@ def _validated(inputs, activation):
     if any(t is not None and t.device != x.device for t in ts):
         raise RuntimeError("grouped_linear: inputs on different devices.")
     R = x.shape[0] if ids is None else ids.shape[0]
-    if max(R, x.shape[0]) >= 2 ** 31 - 1:
-        raise RuntimeError("grouped_linear: 2^31 rows or more.")
+    if max(R, x.shape[0]) >= 2 ** 31 - 4096:
+        raise RuntimeError("grouped_linear: 2^31 - 4096 rows or more.")
     p = GroupedParams(R, x.shape[0], G, K, M, _DTYPES[x.dtype], _ACTIVATIONS[activation],
                       int(ids is not None))
     return p, [None if t is None else t.contiguous() for t in ts]

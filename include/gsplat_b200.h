@@ -675,8 +675,8 @@ int gs_group_offsets(int64_t n, const int32_t* sorted_ids, int32_t groups,
 enum gs_activation { GS_ACT_NONE = 0, GS_ACT_RELU = 1, GS_ACT_SIGMOID = 2 };
 
 typedef struct {
-  int64_t rows;         /* R, below 2^31                                    */
-  int64_t n;            /* rows of x: R without row_ids; below 2^31         */
+  int64_t rows;         /* R, below 2^31 - 4096                             */
+  int64_t n;            /* rows of x: R without row_ids; below 2^31 - 4096  */
   int32_t groups;       /* G                                                */
   int32_t in_features;  /* K                                                */
   int32_t out_features; /* M                                                */
