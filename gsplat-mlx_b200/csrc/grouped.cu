@@ -160,6 +160,21 @@ __device__ __forceinline__ uint4 get_chunk(const T* __restrict__ p, int there) {
   return c.q;
 }
 
+// The place of a ring of buffers that is next, and how often it went round:
+// the phase of the place's barriers.
+struct Ring {
+  int slots, slot, turn;
+  __device__ __forceinline__ explicit Ring(int n) : slots(n), slot(0), turn(0) {}
+  __device__ __forceinline__ void next() {
+    if (++slot == slots) slot = 0, ++turn;
+  }
+  // the place `n` <= slots before, and its last phase
+  __device__ __forceinline__ int slot_before(int n) const {
+    return slot >= n ? slot - n : slot - n + slots;
+  }
+  __device__ __forceinline__ int turn_before(int n) const { return slot >= n ? turn : turn - 1; }
+};
+
 // Consecutive rows of one group, at most `most` of them, up to `end`.
 struct Run {
   int row;
@@ -463,51 +478,48 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   Run none;
   none.row = (int)(first_tile(tiles, gridDim.x, blockIdx.x) * kTile);
   none.n = 0, none.g = -1, none.group_end = 0;
-  auto after = [&](const Run& t) { return run_from(p.off, p.s.G, t.row + t.n, end, kTile, t); };
-
+  // the rows behind t that belong together
+  auto after = [&](const Run& t) { return run_from(p.off, p.s.G, t.row + t.n, end, INT_MAX, t); };
   auto after_live = [&](Run t) {  // rows outside every group are the back's alone
     t = after(t);
-    while (t.n > 0 && (t.g < 0 || t.g >= p.s.G)) {
-      t.n = t.group_end - t.row;
-      t = after(t);
-    }
+    while (t.n > 0 && (t.g < 0 || t.g >= p.s.G)) t = after(t);
     return t;
   };
   auto steps_of = [&](int j) { return (min(DP, p.depth - j * DP) + STEP - 1) / STEP; };
-  // the slot of the panel `back` panels before the one in `slot`
-  auto slot_before = [&](int slot, int back) {
-    return slot >= back ? slot - back : slot + p.slots - back;
-  };
   // the front makes operands of the panels; else they are multiplied as they are
   constexpr bool kWork = LOAD == kCopy || L::kTerms == 2 || L::kY;
 
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
     if (LOAD == kTma) {
-      int slot = 0, q = 0;
+      Ring ring(p.slots);
       for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
-        for (int j = 0; j < p.panels; ++j, ++q) {
-          if (q >= p.slots) wait(free_(slot), q / p.slots - 1);
-          if (tc::elected()) {
-            const uint32_t to = tc::smem_addr(s_rows + slot * kPanel);
-            tc::expect(full(slot), kPanel * (L::kY ? 2 : 1));
-            tc::load_box(to, &map_a, j * DP, cur.row, full(slot));
-            if (L::kY) tc::load_box(to + p.slots * kPanel, &map_y, j * DP, cur.row, full(slot));
+        for (int i = 0; i < cur.n; i += kTile)
+          for (int j = 0; j < p.panels; ++j, ring.next()) {
+            const int slot = ring.slot;
+            if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+            if (tc::elected()) {
+              const uint32_t to = tc::smem_addr(s_rows + slot * kPanel);
+              tc::expect(full(slot), kPanel * (L::kY ? 2 : 1));
+              tc::load_box(to, &map_a, j * DP, cur.row + i, full(slot));
+              if (L::kY)
+                tc::load_box(to + p.slots * kPanel, &map_y, j * DP, cur.row + i, full(slot));
+            }
+            __syncwarp();
           }
-          __syncwarp();
-          slot = slot + 1 == p.slots ? 0 : slot + 1;
-        }
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
     const uint32_t idesc = tc::instr_desc(Mma<T>::format, (cols + 15) / 16 * 16);
     const uint32_t leader = tc::elected();
-    int staged = -1, stagings = 0, slot = 0, q = 0, t = 0;
-    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur), ++t) {
-      for (int j = 0; j < p.panels; ++j, ++q) {
-        if (cur.g != staged || !p.resident) wait(weighed, stagings++);
-        staged = cur.g;
-        wait(kWork ? ready(slot) : full(slot), q / p.slots);
+    Ring ring(p.slots);
+    int stagings = 0, q = 0, t = 0;
+    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
+    for (int row = 0; row < cur.n; row += kTile, ++t) {
+      for (int j = 0; j < p.panels; ++j, ++q, ring.next()) {
+        const int slot = ring.slot;
+        if (row + j == 0 || !p.resident) wait(weighed, stagings++);
+        wait(kWork ? ready(slot) : full(slot), ring.turn);
         if (j == 0 && t > 1) wait(taken(t & 1), (t >> 1) - 1);
         tc::fence_after_sync();
         const int steps = steps_of(j);
@@ -534,11 +546,10 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         }
         tc::commit(leader, free_(slot));
         if (j + 1 == p.panels) tc::commit(leader, made(t & 1));
-        slot = slot + 1 == p.slots ? 0 : slot + 1;
       }
     }
     // every MMA is done before the memory goes
-    if (q > 0) wait(free_(slot_before(slot, 1)), (q - 1) / p.slots);
+    if (q > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
   } else if (warp < 8) {
     // ------------------------------------------------------------ front warps
     const int tid = threadIdx.x;
@@ -548,26 +559,34 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     const int c16 = tid & 7, r16 = tid >> 3;  // this thread's chunk, and its rows r16 + 32 i
     const uint32_t o16 = chunk_at(r16, c16);  // + 4096 i in a panel
 
-    // The panel that is copied next: panel ahead_j of the tile `ahead`, into
-    // slot `ahead_s`.
-    Run ahead = none, behind = none;
-    int ahead_j = 0, ahead_s = 0;
-    int at[4], id[4];  // rows of x, gathered: validated, and as read for the tile after
-    auto read_ids = [&](const Run& t) {
+    // The panel that is copied next: panel ahead_j of the rows at[], into slot
+    // `ahead_s`; id[] are the rows of the tile after, from `behind_row` of
+    // `behind` on, as they were read.
+    Run behind = none;
+    int behind_row = 0, ahead_j = 0, ahead_s = 0, at[4], id[4];
+    bool ahead = false;  // there is something to copy
+    auto move_on = [&]() {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        id[i] = p.ids && !BACK && r16 + 32 * i < t.n ? __ldg(p.ids + t.row + r16 + 32 * i) : -1;
-    };
-    auto settle = [&]() {  // of the tile that is copied now
+      for (int i = 0; i < 4; ++i) at[i] = id[i] < p.s.n || BACK ? id[i] : -1;
+      ahead = behind.n > 0;
+      behind_row += kTile;
+      if (behind_row >= behind.n) {
+        behind = after_live(behind);
+        behind_row = 0;
+      }
+      // (no use of what is read here: it is on its way for a tile's time)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = r16 + 32 * i;
-        if (p.ids && !BACK) at[i] = id[i] < p.s.n ? id[i] : -1;
-        else at[i] = row < ahead.n ? ahead.row + row : -1;
+        const int row = behind_row + r16 + 32 * i;
+        id[i] = -1;
+        if (row < behind.n) {
+          if (p.ids && !BACK) id[i] = __ldg(p.ids + behind.row + row);
+          else id[i] = behind.row + row;
+        }
       }
     };
     auto send = [&]() {
-      if (ahead.n > 0) {
+      if (ahead) {
         if (c16 < 2 * steps_of(ahead_j)) {
           const int d = ahead_j * DP + c16 * E;
           const uint32_t to = ahead_s * kPanel + o16;
@@ -584,10 +603,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         ahead_s = ahead_s + 1 == p.slots ? 0 : ahead_s + 1;
         if (++ahead_j == p.panels) {
           ahead_j = 0;
-          ahead = behind;
-          settle();
-          behind = after_live(ahead);
-          read_ids(behind);
+          move_on();
         }
       }
       send_done();  // also where nothing is left, to keep the count
@@ -637,27 +653,28 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     // long done.
     const int lag = p.slots > 2 ? 2 : 1;
     if (LOAD == kCopy) {
-      ahead = after_live(none);
-      read_ids(ahead);
-      settle();
-      behind = after_live(ahead);
-      read_ids(behind);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) id[i] = -1;
+      move_on();
+      move_on();
       for (int i = lag; i < p.slots; ++i) send();
     }
-    int staged = -1, slot = 0, q = 0;
+    Ring ring(p.slots);
+    int q = 0;
     for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur)) {
-      if (cur.g != staged && p.resident) {
+      if (p.resident) {
         // every MMA of the group before is done
-        if (q > 0) wait(free_(slot_before(slot, 1)), (q - 1) / p.slots);
+        if (q > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
         stage_weights(cur.g, 0, p.panels);
         tc::fence_smem();
         __syncwarp();
         if (lane == 0) tc::arrive(weighed);
-        staged = cur.g;
       }
-      for (int j = 0; j < p.panels; ++j, ++q) {
+      for (int row = 0; row < cur.n; row += kTile)
+      for (int j = 0; j < p.panels; ++j, ++q, ring.next()) {
+        const int slot = ring.slot;
         if (!p.resident) {
-          if (q > 0) wait(free_(slot_before(slot, 1)), (q - 1) / p.slots);
+          if (q > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
           stage_weights(cur.g, j, j + 1);
           tc::fence_smem();
           __syncwarp();
@@ -665,12 +682,12 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         }
         if (kWork) {
           // the panel `lag` before is done with: its slot, and its low parts
-          if (q >= lag) wait(free_(slot_before(slot, lag)), (q - lag) / p.slots);
+          if (q >= lag) wait(free_(ring.slot_before(lag)), ring.turn_before(lag));
           if (LOAD == kCopy) {
             send();
             arrived(p.slots - lag);
           } else {
-            wait(full(slot), q / p.slots);
+            wait(full(slot), ring.turn);
           }
           if ((L::kTerms == 2 || L::kY) && c16 < 2 * steps_of(j)) {
             char* const here = s_rows + slot * kPanel;
@@ -698,9 +715,8 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         } else {
           // keeps pace: a barrier says whether its last phase is over, not
           // which one that is
-          wait(free_(slot), q / p.slots);
+          wait(free_(slot), ring.turn);
         }
-        slot = slot + 1 == p.slots ? 0 : slot + 1;
       }
     }
     if (LOAD == kCopy) arrived(0);
@@ -710,11 +726,12 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     const int bw = warp - 8, row0 = (bw & 3) * 32;  // lanes of the accumulator
     float* const my_bias = s_bias[bw];
     int biased = -1, t = 0;
-    for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
+    for (Run cur = after(none); cur.n > 0; cur = after(cur))
+    for (int row = cur.row; row < cur.row + cur.n; row += kTile) {
       const bool live = cur.g >= 0 && cur.g < p.s.G;
-      const int rows = min(32, cur.n - row0);
+      const int rows = min(32, cur.row + cur.n - row - row0);
       int32_t into = -1;  // where lane's row is added up
-      if (MODE == kScatter && live && lane < rows) into = __ldg(p.ids + cur.row + row0 + lane);
+      if (MODE == kScatter && live && lane < rows) into = __ldg(p.ids + row + row0 + lane);
       const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms + ((uint32_t)row0 << 16);
       if (live) {
         if (!BACK && cur.g != biased) {
@@ -730,7 +747,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       if (into >= p.s.n) into = -1;
       take_results<T, ACT, MODE, L::kTerms>(live, acc, p.nt, bw >> 2, rows, cols, my_bias, into,
                                             s_stage + bw * 2048, p.out,
-                                            BACK && MODE == kScatter ? 0 : cur.row + row0, p.width,
+                                            MODE == kScatter ? 0 : row + row0, p.width,
                                             n0, p.wide_out);
       if (live) {
         tc::fence_before_sync();
@@ -1080,10 +1097,11 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
     if (tma_boxes > 0) {
-      int slot = 0, q = 0;
+      Ring ring(p.slots);
       for (Run cur = after(none); cur.n > 0; cur = after(cur))
-        for (int row = cur.row; row < cur.row + cur.n; row += kRows32, ++q) {
-          if (q >= p.slots) wait(free_(slot), q / p.slots - 1);
+        for (int row = cur.row; row < cur.row + cur.n; row += kRows32, ring.next()) {
+          const int slot = ring.slot;
+          if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
           if (tc::elected()) {
             const uint32_t to = tc::smem_addr(s_slots + slot * slot_bytes);
             tc::expect(full(slot), tma_boxes * kBox);
@@ -1098,7 +1116,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
               }
           }
           __syncwarp();
-          slot = slot + 1 == p.slots ? 0 : slot + 1;
         }
     }
   } else if (warp == 16) {
@@ -1210,11 +1227,12 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     for (int it = 0; it < ITS; ++it)
 #pragma unroll
       for (int j = 0; j < 4; ++j) db[it][j] = 0.0f;
-    int slot = 0, q = 0;
+    Ring ring(p.slots);
+    int q = 0;
     for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
-      for (int left = cur.n; left > 0;
-           left -= kRows32, ++q, slot = slot + 1 == p.slots ? 0 : slot + 1) {
+      for (int left = cur.n; left > 0; left -= kRows32, ++q, ring.next()) {
         if ((q & 1) != fg) continue;
+        const int slot = ring.slot;
         if (copies) {
           if (own > 1) {
             arrived(own - 2);
@@ -1230,7 +1248,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         // (first: it says that every panel before has been through its slot, so
         // that the slot's barrier is at this panel)
         if (q > 1) wait(spent(fg), (q >> 1) - 1);
-        if (tma_boxes > 0) wait(full(slot), q / p.slots);
+        if (tma_boxes > 0) wait(full(slot), ring.turn);
         const char* const from = s_slots + slot * slot_bytes;
         char* const set = s_sets + fg * set_bytes;
 #pragma unroll
@@ -1439,41 +1457,39 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   Run none;
   none.row = (int)(first_tile(tiles, gridDim.x, blockIdx.x) * kTile);
   none.n = 0, none.g = -1, none.group_end = 0;
-  auto after = [&](const Run& t) { return run_from(p.off, p.s.G, t.row + t.n, end, kTile, t); };
+  auto after = [&](const Run& t) { return run_from(p.off, p.s.G, t.row + t.n, end, INT_MAX, t); };
   auto after_live = [&](Run t) {
     t = after(t);
-    while (t.n > 0 && (t.g < 0 || t.g >= p.s.G)) {
-      t.n = t.group_end - t.row;
-      t = after(t);
-    }
+    while (t.n > 0 && (t.g < 0 || t.g >= p.s.G)) t = after(t);
     return t;
   };
 
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
-    int slot = 0, ys = 0, yq = 0, t = 0;
-    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur), ++t) {
-      if (t >= p.slots) wait(free_(slot), t / p.slots - 1);
+    Ring ring(p.slots), y_ring(p.ys);
+    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
+    for (int row = cur.row; row < cur.row + cur.n; row += kTile, ring.next()) {
+      const int slot = ring.slot;
+      if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
       if (tc::elected()) {
         const uint32_t to = tc::smem_addr(s_tiles + slot * tile_bytes);
         tc::expect(full(slot), SHARED ? p.pm * kPanel : tile_bytes);
         for (int j = 0; j < p.pm; ++j)
-          tc::load_box(to + j * kPanel, &map_v, j * 64, cur.row, full(slot));
+          tc::load_box(to + j * kPanel, &map_v, j * 64, row, full(slot));
         if (!SHARED)
           for (int j = 0; j < p.pk; ++j)
-            tc::load_box(to + (p.pm + j) * kPanel, &map_x, j * 64, cur.row, full(slot));
+            tc::load_box(to + (p.pm + j) * kPanel, &map_x, j * 64, row, full(slot));
       }
       __syncwarp();
-      for (int j = 0; HAS_Y && j < p.pm; ++j, ++yq) {
-        if (yq >= p.ys) wait(y_free(ys), yq / p.ys - 1);
+      for (int j = 0; HAS_Y && j < p.pm; ++j, y_ring.next()) {
+        const int ys = y_ring.slot;
+        if (y_ring.turn > 0) wait(y_free(ys), y_ring.turn - 1);
         if (tc::elected()) {
           tc::expect(y_full(ys), kPanel);
-          tc::load_box(tc::smem_addr(s_y + ys * kPanel), &map_y, j * 64, cur.row, y_full(ys));
+          tc::load_box(tc::smem_addr(s_y + ys * kPanel), &map_y, j * 64, row, y_full(ys));
         }
         __syncwarp();
-        ys = ys + 1 == p.ys ? 0 : ys + 1;
       }
-      slot = slot + 1 == p.slots ? 0 : slot + 1;
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
@@ -1483,17 +1499,17 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     const uint32_t leader = tc::elected();
     const uint32_t k_blocks = p.pk > 1 ? kPanel : 0;  // to the next 64 columns
     const int steps = (M + 15) / 16;
-    int staged = -1, stagings = 0, slot = 0, ys = 0, t = 0, piece = 0, sums = 0;
-    Run cur = after_live(none);
-    while (cur.n > 0) {
-      const Run nxt = after_live(cur);
+    Ring ring(p.slots);
+    int stagings = 0, ys = 0, t = 0, piece = 0, sums = 0;
+    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
+    for (int left = cur.n; left > 0; left -= kTile, ++t, ring.next()) {
+      const int slot = ring.slot;
       char* const vz = s_tiles + slot * tile_bytes;
       const uint32_t v_at = tc::smem_addr(vz), x_at = v_at + p.pm * kPanel;
       const uint32_t low_at = tc::smem_addr(s_y + ys * kPanel);  // whole tiles: ys % pm == 0
-      wait(ready(slot), t / p.slots);
+      wait(ready(slot), ring.turn);
       if (p.vx) {
-        if (cur.g != staged) wait(weighed, stagings++);
-        staged = cur.g;
+        if (left == cur.n) wait(weighed, stagings++);
         const int buf = NBUF == 2 ? t & 1 : 0;
         if (t >= NBUF) wait(taken(buf), t / NBUF - 1);
         tc::fence_after_sync();
@@ -1520,17 +1536,14 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       }
       tc::commit(leader, free_(slot));
       for (int j = 0; TERMS == 2 && j < p.pm; ++j) tc::commit(leader, y_free(ys + j));
-      if (++piece == kPiece || nxt.n == 0 || nxt.g != cur.g) {
+      if (++piece == kPiece || left <= kTile) {
         tc::commit(leader, sum_made);
         ++sums;
         piece = 0;
       }
-      slot = slot + 1 == p.slots ? 0 : slot + 1;
       ys = ys + p.pm >= p.ys ? 0 : ys + p.pm;
-      ++t;
-      cur = nxt;
     }
-    if (t > 0) wait(free_(slot > 0 ? slot - 1 : p.slots - 1), (t - 1) / p.slots);
+    if (t > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
   } else if (warp < 8) {
     // ------------------------------------------------------------ front warps
     const int tid = threadIdx.x;
@@ -1552,13 +1565,20 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         if (i >> 2 < p.pk)
           *reinterpret_cast<uint4*>(s_w + (i >> 2) * kPanel + o16 + 4096 * (i & 3)) = q[i];
     };
-    // gathered rows of x: tile `ahead` into slot `ahead_s`
-    Run ahead = none, behind = none;
-    int ahead_s = 0, id[4];
-    auto read_ids = [&](const Run& t) {
+    // gathered rows of x: those from ahead_row of `ahead` on, into slot `ahead_s`
+    Run ahead = none;
+    int ahead_row = 0, ahead_s = 0, id[4];
+    auto move_on = [&]() {
+      ahead_row += kTile;
+      if (ahead_row >= ahead.n) {
+        ahead = after_live(ahead);
+        ahead_row = 0;
+      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        id[i] = p.ids && r16 + 32 * i < t.n ? __ldg(p.ids + t.row + r16 + 32 * i) : -1;
+      for (int i = 0; i < 4; ++i) {
+        const int row = ahead_row + r16 + 32 * i;
+        id[i] = row < ahead.n ? __ldg(p.ids + ahead.row + row) : -1;
+      }
     };
     auto send = [&]() {
       if (ahead.n > 0) {
@@ -1572,50 +1592,46 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
                                 ok ? K - j * 64 - c16 * 8 : 0);
         }
         ahead_s = ahead_s + 1 == p.slots ? 0 : ahead_s + 1;
-        ahead = behind;
-        read_ids(ahead);
-        behind = after_live(ahead);
+        move_on();
       }
       send_done();
     };
     if (SHARED) {
-      ahead = after_live(none);
-      read_ids(ahead);
-      behind = after_live(ahead);
+      move_on();
       for (int i = 1; i < p.slots; ++i) send();
     }
     float db[2][8];
 #pragma unroll
     for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
-    int staged = -1, slot = 0, ys = 0, yq = 0, t = 0;
-    Run cur = after_live(none);
-    while (cur.n > 0) {
-      const Run nxt = after_live(cur);
-      const int before = slot > 0 ? slot - 1 : p.slots - 1;
-      if (p.vx && cur.g != staged) {
-        if (t > 0) wait(free_(before), (t - 1) / p.slots);
+    Ring ring(p.slots), y_ring(p.ys);
+    int t = 0;
+    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
+    for (int left = cur.n; left > 0; left -= kTile, ++t, ring.next()) {
+      const int slot = ring.slot;
+      if (p.vx && left == cur.n) {
+        if (t > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
         stage_weights(cur.g);
         tc::fence_smem();
         __syncwarp();
         if (lane == 0) tc::arrive(weighed);
-        staged = cur.g;
       }
       if (SHARED) {
-        if (t > 0) wait(free_(before), (t - 1) / p.slots);
+        if (t > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
         send();
         arrived(p.slots - 1);
       }
-      wait(full(slot), t / p.slots);
+      wait(full(slot), ring.turn);
       char* const vz = s_tiles + slot * tile_bytes;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (j >= p.pm) break;
+        const int ys = y_ring.slot;
         char* const yt = s_y + ys * kPanel - j * kPanel;
-        if (HAS_Y) wait(y_full(ys), yq / p.ys);
+        if (HAS_Y) wait(y_full(ys), y_ring.turn);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t o = j * kPanel + o16 + 4096 * i;
-          const bool in = r16 + 32 * i < cur.n;  // rows behind are another group's
+          const bool in = r16 + 32 * i < left;  // rows behind are another group's
           Chunk<T> v, z;
           v.q = *reinterpret_cast<const uint4*>(vz + o);
           if (HAS_Y) z.q = *reinterpret_cast<const uint4*>(yt + o);
@@ -1637,13 +1653,12 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
             __syncwarp();
             if (lane == 0) tc::arrive(y_free(ys));
           }
-          ++yq;
-          ys = ys + 1 == p.ys ? 0 : ys + 1;
+          y_ring.next();
         }
       }
-      if (!SHARED && cur.n < kTile) {  // nor may what x has there be multiplied, even by zeros
+      if (!SHARED && left < kTile) {  // nor may what x has there be multiplied, even by zeros
         for (int i = 0; i < 4; ++i)
-          if (r16 + 32 * i >= cur.n)
+          if (r16 + 32 * i >= left)
             for (int j = 0; j < p.pk; ++j)
               *reinterpret_cast<uint4*>(vz + (p.pm + j) * kPanel + o16 + 4096 * i) =
                   make_uint4(0, 0, 0, 0);
@@ -1651,7 +1666,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       tc::fence_smem();
       __syncwarp();
       if (lane == 0) tc::arrive(ready(slot));
-      if (nxt.n == 0 || nxt.g != cur.g) {  // the group's v_b, summed in a fixed order
+      if (left <= kTile) {  // the group's v_b, summed in a fixed order
         if (p.biases) {
           float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1)) +
                             (int64_t)M * K;
@@ -1677,9 +1692,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
       }
-      slot = slot + 1 == p.slots ? 0 : slot + 1;
-      ++t;
-      cur = nxt;
     }
     if (SHARED) arrived(0);
   } else {
@@ -1688,14 +1700,14 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     const int bw = warp - 8, row0 = (bw & 3) * 32;
     int t = 0, piece = 0, sums = 0;
     bool first = true;  // of the group
-    Run cur = after(none);
-    while (cur.n > 0) {
-      const Run nxt = after(cur);
+    for (Run cur = after(none); cur.n > 0; cur = after(cur))
+    for (int left = cur.n; left > 0; left -= kTile) {
       const bool live = cur.g >= 0 && cur.g < p.s.G;
-      const int rows = min(32, cur.n - row0), buf = NBUF == 2 ? t & 1 : 0;
+      const int row = cur.row + cur.n - left + row0;  // this warp's first
+      const int rows = min(32, left - row0), buf = NBUF == 2 ? t & 1 : 0;
       if (p.vx) {
         int into = -1;
-        if (SHARED && live && lane < rows) into = __ldg(p.ids + cur.row + row0 + lane);
+        if (SHARED && live && lane < rows) into = __ldg(p.ids + row + lane);
         if (live) {
           wait(made(buf), t / NBUF);
           tc::fence_after_sync();
@@ -1705,7 +1717,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
           take_results<T, ACT, MODE, TERMS>(live, tmem + buf * TERMS * nk + ((uint32_t)row0 << 16),
                                             nk, bw >> 2, rows, K, nullptr, into,
                                             s_stage + bw * 2048, p.vx,
-                                            SHARED ? 0 : cur.row + row0, K, 0, 1);
+                                            SHARED ? 0 : row, K, 0, 1);
         if (live) {
           tc::fence_before_sync();
           __syncwarp();
@@ -1714,7 +1726,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       }
       if (live) {
         ++t;
-        const bool last = nxt.n == 0 || nxt.g != cur.g;
+        const bool last = left <= kTile;
         if (++piece == kPiece || last) {
           wait(sum_made, sums);
           tc::fence_after_sync();
@@ -1750,7 +1762,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
           first = last;
         }
       }
-      cur = nxt;
     }
   }
   tc::fence_before_sync();
