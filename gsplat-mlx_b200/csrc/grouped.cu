@@ -405,8 +405,8 @@ __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second
 //
 // One CTA an SM streams consecutive 128-row tiles, a panel (128 bytes of
 // depth) at a time, through a ring of `slots` panels.  One warp has the
-// panels filled by TMA where rows lie together; gathered rows, and fp32 rows
-// off the boundary, the eight front warps copy asynchronously.  These make
+// panels filled by TMA, gathered rows four at a time; rows off the 16-byte
+// boundary the eight front warps copy.  These make
 // operands of the panels, another warp issues the MMAs, and the eight back
 // warps take a tile's accumulator while the next tile's is made.  16-bit rows
 // are multiplied as they arrive; of fp32 rows the tensor core reads the upper
@@ -491,7 +491,40 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
-    if (LOAD == kTma) {
+    if (LOAD == kTma && !BACK && p.ids) {
+      // gathered rows: each lane has four of the tile's 128 fetched
+      Ring ring(p.slots);
+      Run ahead = after_live(none);
+      int ahead_row = 0, id[4];
+      auto read_ids = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = ahead_row + 4 * lane + i;
+          id[i] = -1;
+          if (row < ahead.n) id[i] = __ldg(p.ids + ahead.row + row);
+        }
+      };
+      read_ids();
+      while (ahead.n > 0) {
+        int rows[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rows[i] = id[i];
+        ahead_row += kTile;
+        if (ahead_row >= ahead.n) {
+          ahead = after_live(ahead);
+          ahead_row = 0;
+        }
+        read_ids();  // of the next tile, a tile's time ahead of their use
+        for (int j = 0; j < p.panels; ++j, ring.next()) {
+          const int slot = ring.slot;
+          if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+          if (tc::elected()) tc::expect(full(slot), kPanel);
+          __syncwarp();
+          tc::load_rows4(tc::smem_addr(s_rows + slot * kPanel) + lane * 512, &map_a, j * DP, rows,
+                         full(slot));
+        }
+      }
+    } else if (LOAD == kTma) {
       Ring ring(p.slots);
       for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
         for (int i = 0; i < cur.n; i += kTile)
@@ -1021,7 +1054,7 @@ struct Weight32Args {
   int kt;              // tiles of K (128)
   int kx, mx;          // boxes of a K tile and of an M tile
   int slots;           // panels of boxes; even with copies
-  int x_mode, v_mode;  // 0: TMA, 1: copies of 16 bytes, 2: of 4
+  int x_mode, v_mode;  // 0: TMA, 2: copies of 4 bytes
   int biases;
 };
 
@@ -1098,14 +1131,36 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     // ------------------------------------------------------------- TMA
     if (tma_boxes > 0) {
       Ring ring(p.slots);
-      for (Run cur = after(none); cur.n > 0; cur = after(cur))
+      int id[2][4];
+      auto read_ids = [&](const Run& t, int row, int k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = row + 4 * (lane & 7) + i;
+          id[k][i] = -1;
+          if (at < t.row + t.n) id[k][i] = __ldg(p.ids + at);
+        }
+      };
+      for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
+        if (p.x_mode == 0 && p.ids) {
+          read_ids(cur, cur.row, 0);
+          read_ids(cur, cur.row + kRows32, 1);
+        }
         for (int row = cur.row; row < cur.row + cur.n; row += kRows32, ring.next()) {
           const int slot = ring.slot;
+          // gathered rows of x: lane 8 j + i has four of box j's 32 fetched,
+          // whose ids were read two panels ago
+          int rows[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            rows[i] = id[0][i];
+            id[0][i] = id[1][i];
+          }
+          if (p.x_mode == 0 && p.ids) read_ids(cur, row + 2 * kRows32, 1);
           if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
           if (tc::elected()) {
             const uint32_t to = tc::smem_addr(s_slots + slot * slot_bytes);
             tc::expect(full(slot), tma_boxes * kBox);
-            if (p.x_mode == 0)
+            if (p.x_mode == 0 && !p.ids)
               for (int j = 0; j < p.kx; ++j)
                 tc::load_box(to + j * kBox, &map_x, k0 + j * 32, row, full(slot));
             if (p.v_mode == 0)
@@ -1116,7 +1171,13 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
               }
           }
           __syncwarp();
+          if (p.x_mode == 0 && p.ids && lane < 8 * p.kx)
+            tc::load_rows4(tc::smem_addr(s_slots + slot * slot_bytes) + (lane >> 3) * kBox +
+                               (lane & 7) * 512,
+                           &map_x, k0 + (lane >> 3) * 32, rows, full(slot));
+          __syncwarp();
         }
+      }
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
@@ -1193,8 +1254,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
             const float* const from = p.x + (ok ? (int64_t)id[i] * K + k0 + c16 * 4 : 0);
             for (int j = 0; j < p.kx; ++j) {
               const int there = ok ? kn - j * 32 - c16 * 4 : 0;
-              if (p.x_mode == 1) send_chunk<float, true>(to + j * kBox + o, from + j * 32, there);
-              else send_chunk<float, false>(to + j * kBox + o, from + j * 32, there);
+              send_chunk<float, false>(to + j * kBox + o, from + j * 32, there);
             }
           }
           if (p.v_mode != 0) {
@@ -1367,7 +1427,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 // ------------------------------------------------- the whole backward, 16 bits
 struct BothArgs {
   Shape s;
-  const void* x;
   const int32_t* ids;
   const int32_t* off;
   const void* w;
@@ -1467,19 +1526,38 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
     Ring ring(p.slots), y_ring(p.ys);
+    int id[4];
+    auto read_ids = [&](const Run& t, int row) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        id[i] = -1;
+        if (row + 4 * lane + i < t.row + t.n) id[i] = __ldg(p.ids + row + 4 * lane + i);
+      }
+    };
     for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
     for (int row = cur.row; row < cur.row + cur.n; row += kTile, ring.next()) {
       const int slot = ring.slot;
+      int rows[4];  // gathered rows of x: four a lane, read a tile ahead
+      if (SHARED) {
+        if (row == cur.row) read_ids(cur, row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rows[i] = id[i];
+        read_ids(cur, row + kTile);
+      }
       if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
       if (tc::elected()) {
         const uint32_t to = tc::smem_addr(s_tiles + slot * tile_bytes);
-        tc::expect(full(slot), SHARED ? p.pm * kPanel : tile_bytes);
+        tc::expect(full(slot), tile_bytes);
         for (int j = 0; j < p.pm; ++j)
           tc::load_box(to + j * kPanel, &map_v, j * 64, row, full(slot));
         if (!SHARED)
           for (int j = 0; j < p.pk; ++j)
             tc::load_box(to + (p.pm + j) * kPanel, &map_x, j * 64, row, full(slot));
       }
+      __syncwarp();
+      for (int j = 0; SHARED && j < p.pk; ++j)
+        tc::load_rows4(tc::smem_addr(s_tiles + slot * tile_bytes) + (p.pm + j) * kPanel + lane * 512,
+                       &map_x, j * 64, rows, full(slot));
       __syncwarp();
       for (int j = 0; HAS_Y && j < p.pm; ++j, y_ring.next()) {
         const int ys = y_ring.slot;
@@ -1547,7 +1625,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   } else if (warp < 8) {
     // ------------------------------------------------------------ front warps
     const int tid = threadIdx.x;
-    const T* const x = static_cast<const T*>(p.x);
     const T* const w = static_cast<const T*>(p.w);
     const int c16 = tid & 7, r16 = tid >> 3;
     const uint32_t o16 = chunk_at(r16, c16);
@@ -1565,41 +1642,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         if (i >> 2 < p.pk)
           *reinterpret_cast<uint4*>(s_w + (i >> 2) * kPanel + o16 + 4096 * (i & 3)) = q[i];
     };
-    // gathered rows of x: those from ahead_row of `ahead` on, into slot `ahead_s`
-    Run ahead = none;
-    int ahead_row = 0, ahead_s = 0, id[4];
-    auto move_on = [&]() {
-      ahead_row += kTile;
-      if (ahead_row >= ahead.n) {
-        ahead = after_live(ahead);
-        ahead_row = 0;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = ahead_row + r16 + 32 * i;
-        id[i] = row < ahead.n ? __ldg(p.ids + ahead.row + row) : -1;
-      }
-    };
-    auto send = [&]() {
-      if (ahead.n > 0) {
-        char* const to = s_tiles + ahead_s * tile_bytes + p.pm * kPanel + o16;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t from = (int64_t)id[i] * K + c16 * 8;
-          const bool ok = id[i] >= 0 && id[i] < p.s.n;
-          for (int j = 0; j < p.pk; ++j)
-            send_chunk<T, true>(to + j * kPanel + 4096 * i, x + from + j * 64,
-                                ok ? K - j * 64 - c16 * 8 : 0);
-        }
-        ahead_s = ahead_s + 1 == p.slots ? 0 : ahead_s + 1;
-        move_on();
-      }
-      send_done();
-    };
-    if (SHARED) {
-      move_on();
-      for (int i = 1; i < p.slots; ++i) send();
-    }
     float db[2][8];
 #pragma unroll
     for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
@@ -1614,11 +1656,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         tc::fence_smem();
         __syncwarp();
         if (lane == 0) tc::arrive(weighed);
-      }
-      if (SHARED) {
-        if (t > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
-        send();
-        arrived(p.slots - 1);
       }
       wait(full(slot), ring.turn);
       char* const vz = s_tiles + slot * tile_bytes;
@@ -1693,7 +1730,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
       }
     }
-    if (SHARED) arrived(0);
   } else {
     // ------------------------------------------------------------- back warps
     constexpr int MODE = SHARED ? kScatter : kBackward;
@@ -2193,7 +2229,10 @@ int launch_rows(RowsArgs p, cudaStream_t st) {
   nx = nx < 1 ? 1 : nx > tiles ? tiles : nx;
   CUtensorMap map_a{}, map_y{};
   if (LOAD == kTma) {
-    if (int rc = make_map(&map_a, p.a, dtype_of<T>, p.s.R, p.depth)) return rc;
+    const bool gather = MODE == kForward && p.ids;
+    if (int rc = make_map(&map_a, p.a, dtype_of<T>, gather ? p.s.n : p.s.R, p.depth,
+                          gather ? 1 : kTile))
+      return rc;
     if (L::kY)
       if (int rc = make_map(&map_y, p.y, dtype_of<T>, p.s.R, p.depth)) return rc;
   }
@@ -2204,10 +2243,9 @@ int launch_rows(RowsArgs p, cudaStream_t st) {
 
 template <typename T, int ACT, int MODE, bool SPLIT>
 int launch_rows(const RowsArgs& p, cudaStream_t st) {
-  const bool wide = p.depth * sizeof(T) % 16 == 0 && on16(p.a) && (!p.y || on16(p.y));
+  const bool wide = p.depth * sizeof(T) % 16 == 0 && on16(p.a) && (!p.y || on16(p.y)) &&
+                    p.s.n > 0;  // an empty x cannot be mapped
   if (!wide) return launch_rows<T, ACT, MODE, kCopy, false, SPLIT>(p, st);
-  if constexpr (MODE == kForward)
-    if (p.ids) return launch_rows<T, ACT, MODE, kCopy, true, SPLIT>(p, st);
   return launch_rows<T, ACT, MODE, kTma, true, SPLIT>(p, st);
 }
 
@@ -2309,7 +2347,7 @@ int launch_weights32(const Shape& s, const void* x, const void* y, const void* v
   p.kt = q.kt, p.biases = vb != nullptr;
   p.kx = ((s.K < 128 ? s.K : 128) + 31) / 32, p.mx = ((s.M < NT ? s.M : NT) + 31) / 32;
   const bool wide_x = s.K % 4 == 0 && on16(x);
-  p.x_mode = wide_x ? (ids ? 1 : 0) : 2;
+  p.x_mode = wide_x && s.n > 0 ? 0 : 2;
   p.v_mode = s.M % 4 == 0 && on16(vy) && (!y || on16(y)) ? 0 : 2;
   const int set = 2 * (p.kx + p.mx) * kBox, slot = (p.kx + p.mx * (ACT ? 2 : 1)) * kBox;
   const int fixed = 2 * set + 24 * 8 + 8;
@@ -2320,7 +2358,7 @@ int launch_weights32(const Shape& s, const void* x, const void* y, const void* v
   if (p.x_mode || p.v_mode) p.slots = p.slots / 2 * 2;
   CUtensorMap map_x{}, map_v{}, map_y{};
   if (p.x_mode == 0)
-    if (int rc = make_map(&map_x, x, GS_F32, s.R, s.K, kRows32)) return rc;
+    if (int rc = make_map(&map_x, x, GS_F32, s.n, s.K, ids ? 1 : kRows32)) return rc;
   if (p.v_mode == 0) {
     if (int rc = make_map(&map_v, vy, GS_F32, s.R, s.M, kRows32)) return rc;
     if (ACT)
@@ -2346,11 +2384,12 @@ int launch_weights(const WeightArgs& p, const Plan& q, cudaStream_t st) {
 template <typename T>
 bool fits_both(const Shape& s, const void* x, const void* w, const void* y, const void* vy,
                const void* vx) {
-  return sizeof(T) == 2 && dims_fit_both(s.K, s.M) && s.R > 0 && on16(x) && on16(w) && on16(vy) && (!y || on16(y)) && (!vx || on16(vx));
+  return sizeof(T) == 2 && dims_fit_both(s.K, s.M) && s.R > 0 && s.n > 0 && on16(x) && on16(w) && on16(vy) && (!y || on16(y)) && (!vx || on16(vx));
 }
 
 template <typename T, int ACT, bool SHARED>
-int launch_both(BothArgs p, const void* vy, const void* y, const Plan& q, cudaStream_t st) {
+int launch_both(BothArgs p, const void* x, const void* vy, const void* y, const Plan& q,
+                cudaStream_t st) {
   constexpr auto kernel = both_mma_kernel<T, ACT, SHARED>;
   constexpr int kAll = 227 * 1024;  // this kernel has no static shared memory
   if (int rc = allow_smem<kernel, kAll>()) return rc;
@@ -2372,8 +2411,7 @@ int launch_both(BothArgs p, const void* vy, const void* y, const Plan& q, cudaSt
   if (int rc = make_map(&map_v, vy, dtype_of<T>, p.s.R, p.s.M)) return rc;
   if (ACT)
     if (int rc = make_map(&map_y, y, dtype_of<T>, p.s.R, p.s.M)) return rc;
-  if (!SHARED)
-    if (int rc = make_map(&map_x, p.x, dtype_of<T>, p.s.R, p.s.K)) return rc;
+  if (int rc = make_map(&map_x, x, dtype_of<T>, p.s.n, p.s.K, SHARED ? 1 : kTile)) return rc;
   kernel<<<(unsigned)q.parts, 2 * kThreads + 64, smem(), st>>>(p, columns, map_v, map_y, map_x);
   return launch_status("grouped_linear_bwd");
 }
@@ -2410,11 +2448,11 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
         return launch_status("grouped_linear_bwd");
       BothArgs p{};
       p.s = s;
-      p.x = x, p.ids = ids, p.off = off, p.w = w, p.part = ws;
+      p.ids = ids, p.off = off, p.w = w, p.part = ws;
       p.vx = !vx ? nullptr : shared ? sum : vx;
       p.biases = vb != nullptr;
-      const int rc = shared ? launch_both<T, ACT, true>(p, vy, y, q, st)
-                            : launch_both<T, ACT, false>(p, vy, y, q, st);
+      const int rc = shared ? launch_both<T, ACT, true>(p, x, vy, y, q, st)
+                            : launch_both<T, ACT, false>(p, x, vy, y, q, st);
       if (rc) return rc;
       if (vx && shared && s.n > 0)
         round_kernel<T><<<grid_for(s.n * s.K, 256), 256, 0, st>>>(s.n * s.K, sum,

@@ -133,20 +133,30 @@ __device__ __forceinline__ void load_box(uint32_t to, const void* map, int x, in
       "[%0], [%1, {%2, %3}], [%4];"
       ::"r"(to), "l"(map), "r"(x), "r"(row), "r"(bar) : "memory");
 }
+// Four rows of a map whose box is one row high, from column x on, one behind
+// the other; a row outside the map reads as zeros.
+__device__ __forceinline__ void load_rows4(uint32_t to, const void* map, int x, const int (&row)[4],
+                                           uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+      ::"r"(to), "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+      : "memory");
+}
 // A barrier of `threads` of the CTA's threads.
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
 // Waits for the phase to end, up to `limit` polls of the hardware's own
-// bounded wait; false when it gave up.
+// bounded wait, of 20 us or so each; false when it gave up.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t limit) {
   uint32_t done = 0;
   do {
     asm volatile(
         "{\n .reg .pred p;\n"
-        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
   } while (!done && limit-- > 0);
   return done != 0;
 }
