@@ -285,6 +285,12 @@ __device__ __forceinline__ void send_chunk(char* to, const T* __restrict__ p, in
     *reinterpret_cast<uint4*>(to) = get_chunk<T, false>(p, there);
   }
 }
+// The same for 16 bytes at once, with zeros copied, too: the barrier that counts
+// the copies covers them.
+__device__ __forceinline__ void send_or_zero(char* to, const void* p, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+               ::"r"(tc::smem_addr(to)), "l"(p), "r"(there ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void send_done() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // All but the last `n` groups have arrived.
 __device__ __forceinline__ void arrived(int n) {
@@ -405,8 +411,8 @@ __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second
 //
 // One CTA an SM streams consecutive 128-row tiles, a panel (128 bytes of
 // depth) at a time, through a ring of `slots` panels.  One warp has the
-// panels filled by TMA, gathered rows four at a time; rows off the 16-byte
-// boundary the eight front warps copy.  These make
+// panels filled by TMA, or two gather rows by asynchronous copies; rows off
+// the 16-byte boundary the eight front warps copy.  These make
 // operands of the panels, another warp issues the MMAs, and the eight back
 // warps take a tile's accumulator while the next tile's is made.  16-bit rows
 // are multiplied as they arrive; of fp32 rows the tensor core reads the upper
@@ -414,10 +420,15 @@ __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second
 // the backward through an activation rewrites the panel as v_z.  The group's
 // weights are staged once per group, and stay.
 //
-enum { kTma, kCopy };  // how rows arrive
+// How rows arrive: by TMA; gathered, by two warps' copies; by copies of the
+// front warps.  (TMA's four-row gathers took 19 cycles a 128-byte row, 49 us
+// where the copies take 40: 316 k rows 64-64 fp32.)
+enum { kTma, kGather, kCopy };
+constexpr int kLoaders = 64;                          // threads of the gathering warps
+constexpr int kCta = 2 * kThreads + 64 + kLoaders;    // front, back, MMA, TMA, gathers
 
 template <typename T, int ACT, int MODE, int LOAD, bool WIDE, bool SPLIT>
-__global__ void __launch_bounds__(2 * kThreads + 64, 1)
+__global__ void __launch_bounds__(kCta, 1)
     rows_mma_kernel(RowsArgs p, int columns, const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_y) {
   using L = RowsLayout<T, ACT, MODE, SPLIT>;
@@ -450,7 +461,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   if (warp == 0) tc::alloc(&s_tmem, columns);
   if (threadIdx.x == 32) {
     for (int i = 0; i < p.slots; ++i) {
-      tc::bar_init(full(i), 1);
+      tc::bar_init(full(i), LOAD == kGather ? kLoaders : 1);
       tc::bar_init(free_(i), 1);
       tc::bar_init(ready(i), 8);
     }
@@ -487,44 +498,11 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   };
   auto steps_of = [&](int j) { return (min(DP, p.depth - j * DP) + STEP - 1) / STEP; };
   // the front makes operands of the panels; else they are multiplied as they are
-  constexpr bool kWork = LOAD == kCopy || L::kTerms == 2 || L::kY;
+  constexpr bool kWork = LOAD != kTma || L::kTerms == 2 || L::kY;
 
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
-    if (LOAD == kTma && !BACK && p.ids) {
-      // gathered rows: each lane has four of the tile's 128 fetched
-      Ring ring(p.slots);
-      Run ahead = after_live(none);
-      int ahead_row = 0, id[4];
-      auto read_ids = [&]() {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = ahead_row + 4 * lane + i;
-          id[i] = -1;
-          if (row < ahead.n) id[i] = __ldg(p.ids + ahead.row + row);
-        }
-      };
-      read_ids();
-      while (ahead.n > 0) {
-        int rows[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) rows[i] = id[i];
-        ahead_row += kTile;
-        if (ahead_row >= ahead.n) {
-          ahead = after_live(ahead);
-          ahead_row = 0;
-        }
-        read_ids();  // of the next tile, a tile's time ahead of their use
-        for (int j = 0; j < p.panels; ++j, ring.next()) {
-          const int slot = ring.slot;
-          if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
-          if (tc::elected()) tc::expect(full(slot), kPanel);
-          __syncwarp();
-          tc::load_rows4(tc::smem_addr(s_rows + slot * kPanel) + lane * 512, &map_a, j * DP, rows,
-                         full(slot));
-        }
-      }
-    } else if (LOAD == kTma) {
+    if (LOAD == kTma) {
       Ring ring(p.slots);
       for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
         for (int i = 0; i < cur.n; i += kTile)
@@ -540,6 +518,51 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
             }
             __syncwarp();
           }
+    }
+  } else if (warp >= 18) {
+    // ------------------------------------------------------------- gathers
+    if constexpr (LOAD == kGather) {
+      const T* const a = static_cast<const T*>(p.a);
+      const int lt = threadIdx.x - (kCta - kLoaders), c16 = lt & 7, r8 = lt >> 3;
+      constexpr int N = kTile / 8;  // rows of a thread: r8 + 8 i
+      Ring ring(p.slots);
+      Run ahead = after_live(none);
+      int ahead_row = 0, id[N];
+      auto read_ids = [&]() {  // no use yet of what is read
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int row = ahead_row + r8 + 8 * i;
+          id[i] = -1;
+          if (row < ahead.n) id[i] = __ldg(p.ids + ahead.row + row);
+        }
+      };
+      read_ids();
+      while (ahead.n > 0) {
+        int at[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i] = id[i] < p.s.n ? id[i] : -1;
+        ahead_row += kTile;
+        if (ahead_row >= ahead.n) {
+          ahead = after_live(ahead);
+          ahead_row = 0;
+        }
+        read_ids();  // of the next tile
+        for (int j = 0; j < p.panels; ++j, ring.next()) {
+          const int slot = ring.slot, d = j * DP + c16 * E;
+          if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+          if (c16 < 2 * steps_of(j)) {
+            char* const to = s_rows + slot * kPanel + chunk_at(r8, c16);  // r & 7 is r8
+            const T* const ad = d < p.depth ? a + d : a;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const bool there = at[i] >= 0 && d < p.depth;
+              send_or_zero(to + 1024 * i, there ? ad + (int64_t)at[i] * p.depth : a, there);
+            }
+          }
+          tc::arrive_copied(full(slot));
+        }
+      }
+      arrived(0);
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
@@ -1054,12 +1077,12 @@ struct Weight32Args {
   int kt;              // tiles of K (128)
   int kx, mx;          // boxes of a K tile and of an M tile
   int slots;           // panels of boxes; even with copies
-  int x_mode, v_mode;  // 0: TMA, 2: copies of 4 bytes
+  int x_mode, v_mode;  // 0: TMA, 1: gathered, 2: the front's copies of 4 bytes
   int biases;
 };
 
 template <int ACT, int NT>
-__global__ void __launch_bounds__(2 * kThreads + 64, 1)
+__global__ void __launch_bounds__(kCta, 1)
     weights32_kernel(Weight32Args p, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_v,
                      const __grid_constant__ CUtensorMap map_y) {
@@ -1086,10 +1109,12 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   auto spent = [&](int i) { return bar0 + 8 * (18 + i); };
   auto made = [&](int i) { return bar0 + 8 * (20 + i); };   // accumulators
   auto taken = [&](int i) { return bar0 + 8 * (22 + i); };
+  const int tma_boxes = (p.x_mode == 0 ? p.kx : 0) + (p.v_mode == 0 ? p.mx * (HAS_Y ? 2 : 1) : 0);
+  const bool sent = tma_boxes > 0 || p.x_mode == 1;  // by other than the front warps
   if (warp == 0) tc::alloc(&s_tmem, 4 * NT);
   if (threadIdx.x == 32) {
     for (int i = 0; i < 8; ++i) {
-      tc::bar_init(full(i), 1);
+      tc::bar_init(full(i), max((tma_boxes > 0 ? 1 : 0) + (p.x_mode == 1 ? kLoaders : 0), 1));
       tc::bar_init(free_(i), 4);
     }
     for (int i = 0; i < 2; ++i) {
@@ -1125,42 +1150,19 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       t = run_from(p.off, p.s.G, t.group_end, end, INT_MAX, t);
     return t;
   };
-  const int tma_boxes = (p.x_mode == 0 ? p.kx : 0) + (p.v_mode == 0 ? p.mx * (HAS_Y ? 2 : 1) : 0);
 
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
     if (tma_boxes > 0) {
       Ring ring(p.slots);
-      int id[2][4];
-      auto read_ids = [&](const Run& t, int row, int k) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = row + 4 * (lane & 7) + i;
-          id[k][i] = -1;
-          if (at < t.row + t.n) id[k][i] = __ldg(p.ids + at);
-        }
-      };
-      for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
-        if (p.x_mode == 0 && p.ids) {
-          read_ids(cur, cur.row, 0);
-          read_ids(cur, cur.row + kRows32, 1);
-        }
+      for (Run cur = after(none); cur.n > 0; cur = after(cur))
         for (int row = cur.row; row < cur.row + cur.n; row += kRows32, ring.next()) {
           const int slot = ring.slot;
-          // gathered rows of x: lane 8 j + i has four of box j's 32 fetched,
-          // whose ids were read two panels ago
-          int rows[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            rows[i] = id[0][i];
-            id[0][i] = id[1][i];
-          }
-          if (p.x_mode == 0 && p.ids) read_ids(cur, row + 2 * kRows32, 1);
           if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
           if (tc::elected()) {
             const uint32_t to = tc::smem_addr(s_slots + slot * slot_bytes);
             tc::expect(full(slot), tma_boxes * kBox);
-            if (p.x_mode == 0 && !p.ids)
+            if (p.x_mode == 0)
               for (int j = 0; j < p.kx; ++j)
                 tc::load_box(to + j * kBox, &map_x, k0 + j * 32, row, full(slot));
             if (p.v_mode == 0)
@@ -1171,13 +1173,54 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
               }
           }
           __syncwarp();
-          if (p.x_mode == 0 && p.ids && lane < 8 * p.kx)
-            tc::load_rows4(tc::smem_addr(s_slots + slot * slot_bytes) + (lane >> 3) * kBox +
-                               (lane & 7) * 512,
-                           &map_x, k0 + (lane >> 3) * 32, rows, full(slot));
-          __syncwarp();
         }
-      }
+    }
+  } else if (warp >= 18) {
+    // ------------------------------------------------------------- gathers
+    if (p.x_mode == 1) {
+      const int lt = threadIdx.x - (kCta - kLoaders), c16 = lt & 7, r8 = lt >> 3;
+      Ring ring(p.slots);
+      Run ahead = after(none);
+      int ahead_row = 0, id[2][4];  // rows r8 + 8 i of the next two panels
+      auto read_ids = [&](int (&to)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = ahead_row + r8 + 8 * i;
+          to[i] = -1;
+          if (row < ahead.n) to[i] = __ldg(p.ids + ahead.row + row);
+        }
+        ahead_row += kRows32;
+        if (ahead_row >= ahead.n) {
+          ahead = after(ahead);
+          ahead_row = 0;
+        }
+      };
+      read_ids(id[0]);
+      read_ids(id[1]);
+      for (Run cur = after(none); cur.n > 0; cur = after(cur))
+        for (int left = cur.n; left > 0; left -= kRows32, ring.next()) {
+          const int slot = ring.slot;
+          int at[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            at[i] = id[0][i] < p.s.n ? id[0][i] : -1;
+            id[0][i] = id[1][i];
+          }
+          read_ids(id[1]);
+          if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+          char* const to = s_slots + slot * slot_bytes + chunk_at(r8, c16);
+          for (int j = 0; j < p.kx; ++j) {
+            const int k = j * 32 + c16 * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool there = at[i] >= 0 && k < kn;
+              send_or_zero(to + j * kBox + 1024 * i,
+                           there ? p.x + (int64_t)at[i] * K + k0 + k : p.x, there);
+            }
+          }
+          tc::arrive_copied(full(slot));
+        }
+      arrived(0);
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
@@ -1217,7 +1260,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   } else if (warp < 8) {
     // ------------------------------------------------------------ front warps
     const int fg = warp >> 2, tid = threadIdx.x & 127;
-    const bool copies = p.x_mode != 0 || p.v_mode != 0;
+    const bool copies = p.x_mode == 2 || p.v_mode == 2;
     const int own = p.slots / 2;  // with copies: this group's slots
     // copies: rows r16 and r16 + 16, chunk c16, of every box
     const int r16 = tid >> 3, c16 = tid & 7;
@@ -1249,7 +1292,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         for (int i = 0; i < 2; ++i) {
           const int row = r16 + 16 * i;
           const uint32_t o = chunk_at(row, c16);
-          if (p.x_mode != 0) {
+          if (p.x_mode == 2) {
             const bool ok = id[i] >= 0 && id[i] < p.s.n;
             const float* const from = p.x + (ok ? (int64_t)id[i] * K + k0 + c16 * 4 : 0);
             for (int j = 0; j < p.kx; ++j) {
@@ -1257,7 +1300,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
               send_chunk<float, false>(to + j * kBox + o, from + j * 32, there);
             }
           }
-          if (p.v_mode != 0) {
+          if (p.v_mode == 2) {
             const bool ok = ahead_row + row < ahead.row + ahead.n;
             const int64_t from = ok ? (int64_t)(ahead_row + row) * M + m0 + c16 * 4 : 0;
             for (int j = 0; j < p.mx; ++j) {
@@ -1308,7 +1351,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         // (first: it says that every panel before has been through its slot, so
         // that the slot's barrier is at this panel)
         if (q > 1) wait(spent(fg), (q >> 1) - 1);
-        if (tma_boxes > 0) wait(full(slot), ring.turn);
+        if (sent) wait(full(slot), ring.turn);
         const char* const from = s_slots + slot * slot_bytes;
         char* const set = s_sets + fg * set_bytes;
 #pragma unroll
@@ -1357,7 +1400,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         __syncwarp();
         if (lane == 0) {
           tc::arrive(ready(fg));
-          if (tma_boxes > 0) tc::arrive(free_(slot));
+          if (sent) tc::arrive(free_(slot));
         }
       }
       if (p.biases && k0 == 0) {  // v_b: this front group's and half's share
@@ -2229,14 +2272,11 @@ int launch_rows(RowsArgs p, cudaStream_t st) {
   nx = nx < 1 ? 1 : nx > tiles ? tiles : nx;
   CUtensorMap map_a{}, map_y{};
   if (LOAD == kTma) {
-    const bool gather = MODE == kForward && p.ids;
-    if (int rc = make_map(&map_a, p.a, dtype_of<T>, gather ? p.s.n : p.s.R, p.depth,
-                          gather ? 1 : kTile))
-      return rc;
+    if (int rc = make_map(&map_a, p.a, dtype_of<T>, p.s.R, p.depth)) return rc;
     if (L::kY)
       if (int rc = make_map(&map_y, p.y, dtype_of<T>, p.s.R, p.depth)) return rc;
   }
-  kernel<<<dim3((unsigned)nx, (unsigned)ny), 2 * kThreads + 64, L::smem(p), st>>>(
+  kernel<<<dim3((unsigned)nx, (unsigned)ny), kCta, L::smem(p), st>>>(
       p, L::columns(p.nt), map_a, map_y);
   return launch_status("grouped_linear");
 }
@@ -2244,8 +2284,10 @@ int launch_rows(RowsArgs p, cudaStream_t st) {
 template <typename T, int ACT, int MODE, bool SPLIT>
 int launch_rows(const RowsArgs& p, cudaStream_t st) {
   const bool wide = p.depth * sizeof(T) % 16 == 0 && on16(p.a) && (!p.y || on16(p.y)) &&
-                    p.s.n > 0;  // an empty x cannot be mapped
+                    p.s.n > 0;  // there is no address in an empty x
   if (!wide) return launch_rows<T, ACT, MODE, kCopy, false, SPLIT>(p, st);
+  if constexpr (MODE == kForward)
+    if (p.ids) return launch_rows<T, ACT, MODE, kGather, true, SPLIT>(p, st);
   return launch_rows<T, ACT, MODE, kTma, true, SPLIT>(p, st);
 }
 
@@ -2347,7 +2389,7 @@ int launch_weights32(const Shape& s, const void* x, const void* y, const void* v
   p.kt = q.kt, p.biases = vb != nullptr;
   p.kx = ((s.K < 128 ? s.K : 128) + 31) / 32, p.mx = ((s.M < NT ? s.M : NT) + 31) / 32;
   const bool wide_x = s.K % 4 == 0 && on16(x);
-  p.x_mode = wide_x && s.n > 0 ? 0 : 2;
+  p.x_mode = wide_x && s.n > 0 ? (ids ? 1 : 0) : 2;
   p.v_mode = s.M % 4 == 0 && on16(vy) && (!y || on16(y)) ? 0 : 2;
   const int set = 2 * (p.kx + p.mx) * kBox, slot = (p.kx + p.mx * (ACT ? 2 : 1)) * kBox;
   const int fixed = 2 * set + 24 * 8 + 8;
@@ -2355,16 +2397,16 @@ int launch_weights32(const Shape& s, const void* x, const void* y, const void* v
   // and slots behind it
   p.slots = (kAll - fixed) / slot;
   p.slots = p.slots > 8 ? 8 : p.slots;
-  if (p.x_mode || p.v_mode) p.slots = p.slots / 2 * 2;
+  if (p.x_mode == 2 || p.v_mode == 2) p.slots = p.slots / 2 * 2;
   CUtensorMap map_x{}, map_v{}, map_y{};
   if (p.x_mode == 0)
-    if (int rc = make_map(&map_x, x, GS_F32, s.n, s.K, ids ? 1 : kRows32)) return rc;
+    if (int rc = make_map(&map_x, x, GS_F32, s.n, s.K, kRows32)) return rc;
   if (p.v_mode == 0) {
     if (int rc = make_map(&map_v, vy, GS_F32, s.R, s.M, kRows32)) return rc;
     if (ACT)
       if (int rc = make_map(&map_y, y, GS_F32, s.R, s.M, kRows32)) return rc;
   }
-  kernel<<<dim3((unsigned)q.parts, (unsigned)(q.kt * q.mt)), 2 * kThreads + 64,
+  kernel<<<dim3((unsigned)q.parts, (unsigned)(q.kt * q.mt)), kCta,
            fixed + p.slots * slot, st>>>(p, map_x, map_v, map_y);
   return launch_status("grouped_linear_bwd");
 }

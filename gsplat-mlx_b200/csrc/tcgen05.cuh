@@ -120,6 +120,10 @@ __device__ __forceinline__ void bar_init_done() {
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Arrives when the asynchronous copies that this thread has sent are there.
+__device__ __forceinline__ void arrive_copied(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 // Arrives, and has the phase wait for `bytes` of bulk copies.
 __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
