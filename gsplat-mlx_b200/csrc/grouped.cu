@@ -1395,6 +1395,7 @@ __global__ void __launch_bounds__(kCta, 1)
               put_low(at + low, t);
             }
           }
+          asm volatile("" ::: "memory");  // one block at a time: registers
         }
         tc::fence_smem();
         __syncwarp();
@@ -1858,37 +1859,41 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int parts, int copie
                                                    T* __restrict__ vw, T* __restrict__ vb) {
   constexpr int VALUES = 256 / SHARES;
   __shared__ float s_sum[SHARES][VALUES];
-  const int g = blockIdx.y, share = threadIdx.x / VALUES, at = threadIdx.x % VALUES;
+  const int share = threadIdx.x / VALUES, at = threadIdx.x % VALUES;
   const int64_t mk = (int64_t)s.M * s.K, each = mk + s.M, place = mk + (int64_t)copies * s.M;
   const int64_t i = (int64_t)blockIdx.x * VALUES + at;
-  const int64_t r0 = max((int64_t)__ldg(off + g), (int64_t)0);
-  const int64_t r1 = min((int64_t)__ldg(off + g + 1), s.R);
-  float sum = 0.0f;
-  if (r0 < r1 && i < each) {
-    const int64_t tiles = (s.R + kTile - 1) / kTile;
-    auto part_of = [&](int64_t r) { return (int)(((r / kTile + 1) * parts - 1) / tiles); };
-    const int b0 = part_of(r0), n = part_of(r1 - 1) - b0 + 1;
-    const int from = n * share / SHARES, to = n * (share + 1) / SHARES;
-    const float* p = part + (int64_t)(b0 + g + from) * place + i;
-    if (i < mk) {
+  const int64_t tiles = (s.R + kTile - 1) / kTile;
+  auto part_of = [&](int64_t r) { return (int)(((r / kTile + 1) * parts - 1) / tiles); };
+  for (int g = blockIdx.y; g < s.G; g += gridDim.y) {
+    const int64_t r0 = max((int64_t)__ldg(off + g), (int64_t)0);
+    const int64_t r1 = min((int64_t)__ldg(off + g + 1), s.R);
+    float sum = 0.0f;
+    if (r0 < r1 && i < each) {
+      const int b0 = part_of(r0), n = part_of(r1 - 1) - b0 + 1;
+      const int from = n * share / SHARES, to = n * (share + 1) / SHARES;
+      const float* p = part + (int64_t)(b0 + g + from) * place + i;
+      if (i < mk) {
 #pragma unroll 8
-      for (int b = from; b < to; ++b, p += place) sum += __ldg(p);
-    } else {
-      for (int b = from; b < to; ++b, p += place)
-        for (int c = 0; c < copies; ++c) sum += __ldg(p + (int64_t)c * s.M);
+        for (int b = from; b < to; ++b, p += place) sum += __ldg(p);
+      } else {
+        for (int b = from; b < to; ++b, p += place)
+          for (int c = 0; c < copies; ++c) sum += __ldg(p + (int64_t)c * s.M);
+      }
     }
-  }
-  if (SHARES > 1) {
-    s_sum[share][at] = sum;
-    __syncthreads();
-    if (share > 0) return;
+    if (SHARES > 1) {
+      __syncthreads();
+      s_sum[share][at] = sum;
+      __syncthreads();
 #pragma unroll
-    for (int w = 1; w < SHARES; ++w) sum += s_sum[w][at];
-  }
-  if (i < mk) {
-    if (vw) vw[g * mk + i] = from_f<T>(sum);
-  } else if (i < each && vb) {
-    vb[(int64_t)g * s.M + (i - mk)] = from_f<T>(sum);
+      for (int w = 1; w < SHARES; ++w) sum += share == 0 ? s_sum[w][at] : 0.0f;
+    }
+    if (share == 0 && i < each) {
+      if (i < mk) {
+        if (vw) vw[g * mk + i] = from_f<T>(sum);
+      } else if (vb) {
+        vb[(int64_t)g * s.M + (i - mk)] = from_f<T>(sum);
+      }
+    }
   }
 }
 
@@ -2266,7 +2271,6 @@ int launch_rows(RowsArgs p, cudaStream_t st) {
     }
   }
   const int64_t ny = ceil_div(p.width, p.nt);
-  if (ny > 65535) return invalid("grouped_linear: too many features");
   const int64_t tiles = ceil_div(p.s.R, kTile);
   int64_t nx = sm_count() / ny;
   nx = nx < 1 ? 1 : nx > tiles ? tiles : nx;
@@ -2381,7 +2385,6 @@ int launch_weights32(const Shape& s, const void* x, const void* y, const void* v
   constexpr auto kernel = weights32_kernel<ACT, NT>;
   constexpr int kAll = 227 * 1024;  // this kernel has no static shared memory
   if (int rc = allow_smem<kernel, kAll>()) return rc;
-  if ((int64_t)q.kt * q.mt > 65535) return invalid("grouped_linear: too many features");
   Weight32Args p{};
   p.s = s;
   p.x = static_cast<const float*>(x), p.y = static_cast<const float*>(y);
@@ -2417,7 +2420,6 @@ int launch_weights(const WeightArgs& p, const Plan& q, cudaStream_t st) {
   if (int rc = allow_smem<kernel>()) return rc;
   const int vt = SPLIT ? 2 : 1;
   const int smem = 1024 + kPanel + vt * NT * 128, columns = NT * vt;
-  if ((int64_t)q.kt * q.mt > 65535) return invalid("grouped_linear: too many features");
   kernel<<<dim3((unsigned)q.parts, (unsigned)(q.kt * q.mt)), kThreads, smem, st>>>(p, columns);
   return launch_status("grouped_linear_bwd");
 }
@@ -2539,13 +2541,13 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
       if (rc) return rc;
     }
     const int64_t each = (int64_t)s.M * (s.K + 1);
-    if (s.G > 65535) return invalid("grouped_linear: more than 65535 groups");
+    const unsigned gy = s.G < 65535 ? s.G : 65535;
     // about parts / G places a group: few are not worth sharing out
     if (q.parts < 8 * (int64_t)s.G)
-      join_kernel<T, 1><<<dim3((unsigned)ceil_div(each, 256), (unsigned)s.G), 256, 0, st>>>(
+      join_kernel<T, 1><<<dim3((unsigned)ceil_div(each, 256), gy), 256, 0, st>>>(
           s, q.parts, q.copies, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
     else
-      join_kernel<T, 8><<<dim3((unsigned)ceil_div(each, 32), (unsigned)s.G), 256, 0, st>>>(
+      join_kernel<T, 8><<<dim3((unsigned)ceil_div(each, 32), gy), 256, 0, st>>>(
           s, q.parts, q.copies, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
   }
   return launch_status("grouped_linear_bwd");
@@ -2567,6 +2569,7 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
 
 // Rows are counted in 32 bits, some tiles past the last.
 constexpr int64_t kRowsMost = INT32_MAX - 4096;
+constexpr int32_t kFeaturesMost = 16384;  // 128 x 256 tiles of weights: a grid's second side
 
 int bad_params(const gs_grouped_params* p) {
   if (!p || p->rows < 0 || p->n < 0 || p->groups < 1 || p->in_features < 1 ||
@@ -2576,6 +2579,8 @@ int bad_params(const gs_grouped_params* p) {
     return invalid("grouped_linear: 2^31 - 4096 rows or more");
   if (!p->use_row_ids && p->n != p->rows)
     return invalid("grouped_linear: x has another number of rows");
+  if (p->in_features > kFeaturesMost || p->out_features > kFeaturesMost)
+    return invalid("grouped_linear: more than 16384 features");
   if (p->dtype < GS_F32 || p->dtype > GS_F16) return invalid("grouped_linear: unknown dtype");
   if (p->activation < GS_ACT_NONE || p->activation > GS_ACT_SIGMOID)
     return invalid("grouped_linear: unknown activation");
@@ -2636,4 +2641,20 @@ extern "C" int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
   const Shape s{p->rows, p->n, p->groups, p->in_features, p->out_features};
   GROUPED_DISPATCH(p, run_bwd, p, s, x, row_ids, offsets, weights, y, v_y, v_x, v_weights, v_biases,
                    static_cast<float*>(workspace), as_stream(stream));
+}
+
+extern "C" int gs_grouped_linear_check(gs_stream_t stream) {
+  unsigned int gave_up = 0, none = 0;
+  cudaStream_t s = as_stream(stream);
+  if (cudaMemcpyFromSymbolAsync(&gave_up, g_wait_gave_up, sizeof(gave_up), 0,
+                                cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return launch_status("grouped_linear_check");
+  if (!gave_up) return GS_OK;
+  if (cudaMemcpyToSymbolAsync(g_wait_gave_up, &none, sizeof(none), 0, cudaMemcpyHostToDevice, s) !=
+          cudaSuccess ||
+      cudaStreamSynchronize(s) != cudaSuccess)
+    return launch_status("grouped_linear_check");
+  set_error("grouped_linear: a wait for a tensor-core tile gave up: results are void");
+  return GS_ERR_DEVICE;
 }

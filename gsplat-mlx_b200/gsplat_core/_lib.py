@@ -158,6 +158,7 @@ SIGNATURES = {
     "gs_grouped_linear_fwd": (ct.c_int, [_P(GroupedParams)] + [_vp] * 7),
     "gs_grouped_linear_bwd_workspace_size": (_sz, [_P(GroupedParams)]),
     "gs_grouped_linear_bwd": (ct.c_int, [_P(GroupedParams)] + [_vp] * 10 + [_sz, _vp]),
+    "gs_grouped_linear_check": (ct.c_int, [_vp]),
     "gs_rasterize_fwd": (ct.c_int, [_P(RasterParams)] + [_vp] * 12),
     "gs_rasterize_bwd": (ct.c_int, [_P(RasterParams)] + [_vp] * 19),
 }

@@ -21,7 +21,8 @@ import ctypes as ct
 import torch
 
 from . import _lib
-from ._lib import GroupedParams, check, on_device_of
+from ._lib import GroupedParams, on_device_of
+from ._lib import check as check_status
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2}
@@ -44,7 +45,7 @@ def group_offsets(ids, groups):
     ids = ids.contiguous()
     off = torch.empty((int(groups) + 1,), dtype=torch.int32, device=ids.device)
     lib = _lib.load()
-    check(on_device_of(ids, lambda stream: lib.gs_group_offsets(
+    check_status(on_device_of(ids, lambda stream: lib.gs_group_offsets(
         ids.numel(), _ptr(ids), int(groups), _ptr(off), stream)), "group_offsets")
     return off
 
@@ -63,8 +64,8 @@ def _validated(inputs, activation):
     if w.dim() != 3 or w.shape[2] != x.shape[1] or w.dtype != x.dtype:
         raise RuntimeError("grouped_linear: weights must have shape [G, M, K] and x's type.")
     G, M, K = w.shape
-    if min(G, M, K) < 1:
-        raise RuntimeError("grouped_linear: G, M and K must be at least 1.")
+    if min(G, M, K) < 1 or max(M, K) > 16384:
+        raise RuntimeError("grouped_linear: G, M and K must be at least 1, M and K at most 16384.")
     if off.shape != (G + 1,) or off.dtype != torch.int32:
         raise RuntimeError("grouped_linear: offsets must have shape [G + 1] and type int32.")
     if b is not None and (b.shape != (G, M) or b.dtype != x.dtype):
@@ -104,7 +105,7 @@ def grouped_linear_forward(inputs, activation="none"):
     _on_cuda(x)
     y = torch.empty((p.rows, p.out_features), dtype=x.dtype, device=x.device)
     lib = _lib.load()
-    check(on_device_of(x, lambda stream: lib.gs_grouped_linear_fwd(
+    check_status(on_device_of(x, lambda stream: lib.gs_grouped_linear_fwd(
         ct.byref(p), _ptr(x), _ptr(ids), _ptr(off), _ptr(w), _ptr(b), _ptr(y), stream)),
         "grouped_linear_forward")
     return y
@@ -148,5 +149,13 @@ def grouped_linear_backward(inputs, y, v_y, activation="none",
             _ptr(out.get("v_x")), _ptr(out.get("v_weights")), _ptr(out.get("v_biases")),
             _ptr(ws), need, stream)
 
-    check(on_device_of(x, call), "grouped_linear_backward")
+    check_status(on_device_of(x, call), "grouped_linear_backward")
     return out
+
+
+def check():
+    """Waits for the current stream and raises if a bounded on-device wait of
+    a grouped_linear kernel gave up (its results would be invalid)."""
+    lib = _lib.load()
+    check_status(lib.gs_grouped_linear_check(torch.cuda.current_stream().cuda_stream),
+                 "grouped_linear")

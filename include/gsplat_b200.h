@@ -678,8 +678,8 @@ typedef struct {
   int64_t rows;         /* R, below 2^31 - 4096                             */
   int64_t n;            /* rows of x: R without row_ids; below 2^31 - 4096  */
   int32_t groups;       /* G                                                */
-  int32_t in_features;  /* K                                                */
-  int32_t out_features; /* M                                                */
+  int32_t in_features;  /* K, up to 16384                                   */
+  int32_t out_features; /* M, up to 16384                                   */
   int32_t dtype;        /* gs_dtype of x, weights, biases, y and gradients  */
   int32_t activation;   /* gs_activation                                    */
   int32_t use_row_ids;  /* 1: row_ids is given; 0: id(r) = r                */
@@ -696,6 +696,7 @@ int gs_grouped_linear_fwd(const gs_grouped_params* p, const void* x,
                           const void* weights, const void* biases, void* y,
                           gs_stream_t stream);
 
+/* Bytes of scratch of the backward, on a 16-byte boundary. */
 size_t gs_grouped_linear_bwd_workspace_size(const gs_grouped_params* p);
 
 /* Its reverse mode from y (the forward's; may be NULL for GS_ACT_NONE) and
@@ -711,6 +712,12 @@ int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
                           void* v_x, void* v_weights, void* v_biases,
                           void* workspace, size_t workspace_bytes,
                           gs_stream_t stream);
+
+/* Waits for the stream and tells whether a wait inside a grouped_linear
+ * kernel of this device gave up since the last check (GS_ERR_DEVICE: what it
+ * wrote is void).  The waits are for the kernel's own copies and tensor-core
+ * tiles and are bounded, at a second or more. */
+int gs_grouped_linear_check(gs_stream_t stream);
 
 #ifdef __cplusplus
 }

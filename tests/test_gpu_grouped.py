@@ -18,6 +18,13 @@ SHAPES = [
     ([2500, 1800, 3000], 5000, 64, 32), ([64], 0, 65, 33), ([4097], 0, 8, 100), ([300], 0, 520, 40),
 ]
 
+# up to 8 outputs, of rows that fill one to 32 lanes, and the first past that
+FEW = [
+    ([1000], 0, 32, 1), ([300, 0, 77], 500, 64, 3), ([257, 4], 0, 128, 4), ([90, 91], 60, 100, 2),
+    ([513], 700, 48, 8), ([40] * 40, 100, 16, 5), ([333], 0, 250, 3), ([129, 1], 99, 7, 7),
+    ([700], 0, 256, 8), ([2000, 3000], 1500, 4, 4), ([65], 0, 129, 3), ([65], 80, 257, 3),
+    ([31, 1, 1, 64], 20, 8, 6), ([5], 3, 1, 8)]
+
 
 def _case(sizes, N, K, M, dtype, seed=0, bias=True):
     g = torch.Generator().manual_seed(seed)
@@ -71,7 +78,7 @@ def _check_backward(c, y, v_y, got, act):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("sizes,N,K,M", SHAPES)
+@pytest.mark.parametrize("sizes,N,K,M", SHAPES + FEW)
 @pytest.mark.parametrize("act", ["none", "relu", "sigmoid"])
 def test_grouped_matches_64_bits(gs, cuda, dtype, sizes, N, K, M, act):
     from gsplat_core.grouped import grouped_linear_backward, grouped_linear_forward
@@ -302,3 +309,70 @@ def test_large_offsets_pass_32_bits(gs, cuda):
     assert not g["v_x"][:-300].any()
     g["v_x"] = g["v_x"][-300:].contiguous()
     _check_backward(tail, y[-300:].contiguous(), v[-300:].contiguous(), g, "none")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["none", "relu", "sigmoid"])
+@pytest.mark.parametrize("K,M", [(16, 16), (24, 72)])
+def test_long_group(gs, cuda, dtype, act, K, M):
+    """Many tiles of one group for every CTA: sums that leave the accumulators
+    in between are neither lost nor added twice.  All positive, so that the
+    magnitude is the value.  One accumulator takes at most 32 tiles of 8
+    additions (each of up to 16 products), then come at most 48 pieces and 296
+    places: 1000 additions one after the other are an upper bound."""
+    from gsplat_core.grouped import grouped_linear_backward
+    R = 800_000
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rand = lambda *s: torch.rand(s, generator=g, device="cuda").to(TYPES[dtype])  # noqa: E731
+    c = {"x": rand(R, K), "weights": rand(2, M, K), "biases": rand(2, M),
+         "offsets": torch.tensor([0, 700, R], dtype=torch.int32, device="cuda")}
+    y, v_y = rand(R, M), rand(R, M)
+    got = grouped_linear_backward(c, y, v_y, activation=act, wanted=("v_weights", "v_biases"))
+    want = linear(*_parts(c), act=act, v_y=v_y, y=y)
+    for k in got:
+        val, mag = want[k]
+        extra = 0.0
+        if act == "sigmoid" and dtype != "fp32":
+            extra = 2.0 ** -15 * mag + (2.0 ** -25 * R if dtype == "fp16" else 0.0)
+        if dtype == "fp16":
+            _half_sums(got[k], val, mag, extra, k)
+        else:
+            assert_sums(got[k], val, mag, 1000, TYPES[dtype], extra, k)
+
+
+def _half_sums(got, val, mag, extra, what):
+    """fp16 overflows at 65504: infinite exactly where the sum is past it (by
+    more than the tolerance), else within the tolerance."""
+    far = val > 65520 * (1 + 1e-3)
+    assert bool(torch.isinf(got.cpu()[far]).all()), what
+    near = val < 65520 * (1 - 1e-3)
+    ex = extra[near] if isinstance(extra, torch.Tensor) else extra
+    assert_sums(got.cpu()[near], val[near], mag[near], 1000, torch.float16, ex, what)
+
+
+def test_many_groups(gs, cuda):
+    """More groups than a grid is high, most of them of one row or none."""
+    from gsplat_core.grouped import grouped_linear_backward, grouped_linear_forward
+    rng = np.random.default_rng(5)
+    sizes = rng.integers(0, 3, size=70_000)
+    for K, M in ((4, 2), (8, 16)):
+        c, v_y = _case(sizes.tolist(), 0, K, M, torch.float32)
+        y = grouped_linear_forward(c, activation="relu")
+        row = torch.from_numpy(np.repeat(np.arange(70_000), sizes)).cuda()
+        z = torch.einsum("rk,rmk->rm", c["x"].double(), c["weights"][row].double()) + c["biases"][row]
+        assert torch.allclose(y.double(), z.clamp(min=0), rtol=1e-6, atol=1e-5)
+        g = grouped_linear_backward(c, y, v_y, activation="relu")
+        v = torch.where(y > 0, v_y, torch.zeros_like(v_y)).double()
+        vw = torch.zeros(70_000, M, K, dtype=torch.float64, device="cuda").index_add_(
+            0, row, v[:, :, None] * c["x"].double()[:, None])
+        assert torch.allclose(g["v_weights"].double(), vw, rtol=1e-6, atol=1e-5)
+        vb = torch.zeros(70_000, M, dtype=torch.float64, device="cuda").index_add_(0, row, v)
+        assert torch.allclose(g["v_biases"].double(), vb, rtol=1e-6, atol=1e-5)
+        vx = torch.einsum("rm,rmk->rk", v, c["weights"][row].double())
+        assert torch.allclose(g["v_x"].double(), vx, rtol=1e-6, atol=1e-5)
+
+
+def test_no_wait_gave_up(gs, cuda):
+    """Last in this file: no bounded wait of the calls above ran out."""
+    from gsplat_core import grouped
+    grouped.check()

@@ -71,6 +71,7 @@ def _inputs(**kw):
     (dict(weights=torch.zeros(2, 5, 3)), "weights must have"),
     (dict(weights=torch.zeros(2, 5, 4).half()), "weights must have"),
     (dict(weights=torch.zeros(2, 0, 4)), "at least 1"),
+    (dict(weights=torch.zeros(1, 1, 4).expand(2, 16385, 4)), "at most 16384"),
     (dict(offsets=torch.zeros(2, dtype=torch.int32)), "offsets must have"),
     (dict(offsets=torch.zeros(3, dtype=torch.int64)), "offsets must have"),
     (dict(biases=torch.zeros(2, 4)), "biases must have"),
@@ -127,6 +128,7 @@ def test_c_entries_refuse_before_launch(gs):
     fwd = lambda q: lib.gs_grouped_linear_fwd(ct.byref(q), *[None] * 7)  # noqa: E731
     assert fwd(prm(rows=0, n=0)) == L.GS_OK
     for q in (prm(), prm(n=5), prm(rows=-1), prm(G=0), prm(K=0), prm(M=0), prm(dtype=5), prm(act=3),
+              prm(K=16385), prm(M=16385), prm(rows=2 ** 31 - 4000, n=2 ** 31 - 4000),
               prm(rows=2 ** 31, n=2 ** 31)):
         assert fwd(q) == L.GS_ERR_INVALID
         assert lib.gs_last_error()
