@@ -1055,7 +1055,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 // eight lanes of an access take the diagonal blocks (column block l, row
 // block l ^ p), which keeps both the reads and the writes free of conflicts in
 // the swizzled panels.  Two groups of four front warps take every second
-// panel of 32 rows, each with operand memory of its own.
+// panel of 32 rows, with operand memory of its own for one or two of them.
 //
 // The tensor core cuts a sum to fp32 at each addition; left to itself that
 // was 2e-5 of the result after 8000 rows.  So every kFlush panels the MMAs
@@ -1076,7 +1076,8 @@ struct Weight32Args {
   float* part;         // as in WeightArgs, with kBiasCopies32 rows of v_b
   int kt;              // tiles of K (128)
   int kx, mx;          // boxes of a K tile and of an M tile
-  int slots;           // panels of boxes; even with copies
+  int slots;           // panels of boxes; even with copies, and at least `sets`
+  int sets;            // of operands: 2 or 4
   int x_mode, v_mode;  // 0: TMA, 1: gathered, 2: the front's copies of 4 bytes
   int biases;
 };
@@ -1095,20 +1096,21 @@ __global__ void __launch_bounds__(kCta, 1)
   const int kn = min(128, K - k0), mn = min(NT, M - m0);
   const int boxes = p.kx + p.mx;                          // x's, then v_y's
   const int slot_bytes = (boxes + (HAS_Y ? p.mx : 0)) * kBox;  // then y's
-  // operands: two sets of values and low parts of x, of v_z.  An MMA reads
+  // operands: sets of values and low parts of x, of v_z.  An MMA reads
   // 128 rows of x's whatever kn is: what lies behind goes to unused lanes.
   const int set_bytes = 2 * boxes * kBox;
   char* const s_sets = smem_raw;
-  char* const s_slots = s_sets + 2 * set_bytes;
+  char* const s_slots = s_sets + p.sets * set_bytes;
   uint64_t* const s_bars = reinterpret_cast<uint64_t*>(s_slots + p.slots * slot_bytes);
-  uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + 24);
+  uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + 28);
   const uint32_t bar0 = tc::smem_addr(s_bars);
   auto full = [&](int i) { return bar0 + 8 * i; };          // TMA's boxes are there
   auto free_ = [&](int i) { return bar0 + 8 * (8 + i); };   // and have been read
   auto ready = [&](int i) { return bar0 + 8 * (16 + i); };  // operands
-  auto spent = [&](int i) { return bar0 + 8 * (18 + i); };
-  auto made = [&](int i) { return bar0 + 8 * (20 + i); };   // accumulators
-  auto taken = [&](int i) { return bar0 + 8 * (22 + i); };
+  auto spent = [&](int i) { return bar0 + 8 * (20 + i); };
+  auto made = [&](int i) { return bar0 + 8 * (24 + i); };   // accumulators
+  auto taken = [&](int i) { return bar0 + 8 * (26 + i); };
+  const int log_sets = p.sets == 4 ? 2 : 1;
   const int tma_boxes = (p.x_mode == 0 ? p.kx : 0) + (p.v_mode == 0 ? p.mx * (HAS_Y ? 2 : 1) : 0);
   const bool sent = tma_boxes > 0 || p.x_mode == 1;  // by other than the front warps
   if (warp == 0) tc::alloc(&s_tmem, 4 * NT);
@@ -1117,9 +1119,11 @@ __global__ void __launch_bounds__(kCta, 1)
       tc::bar_init(full(i), max((tma_boxes > 0 ? 1 : 0) + (p.x_mode == 1 ? kLoaders : 0), 1));
       tc::bar_init(free_(i), 4);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       tc::bar_init(ready(i), 4);
       tc::bar_init(spent(i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       tc::bar_init(made(i), 1);
       tc::bar_init(taken(i), 8);
     }
@@ -1229,8 +1233,8 @@ __global__ void __launch_bounds__(kCta, 1)
     int q = 0, held = 0, sums = 0;
     for (Run cur = after(none); cur.n > 0; cur = after(cur))
     for (int left = cur.n; left > 0; left -= kRows32, ++q) {
-      const int set = q & 1, buf = sums & 1;
-      wait(ready(set), q >> 1);
+      const int set = q & (p.sets - 1), buf = sums & 1;
+      wait(ready(set), q >> log_sets);
       if (held == 0 && sums > 1) wait(taken(buf), (sums >> 1) - 1);
       tc::fence_after_sync();
       const uint32_t x_at = tc::smem_addr(s_sets + set * set_bytes);
@@ -1256,7 +1260,7 @@ __global__ void __launch_bounds__(kCta, 1)
         held = 0;
       }
     }
-    if (q > 0) wait(spent((q - 1) & 1), (q - 1) >> 1);
+    if (q > 0) wait(spent((q - 1) & (p.sets - 1)), (q - 1) >> log_sets);
   } else if (warp < 8) {
     // ------------------------------------------------------------ front warps
     const int fg = warp >> 2, tid = threadIdx.x & 127;
@@ -1348,12 +1352,14 @@ __global__ void __launch_bounds__(kCta, 1)
             tc::bar_sync(1 + fg, 128);
           }
         }
-        // (first: it says that every panel before has been through its slot, so
-        // that the slot's barrier is at this panel)
-        if (q > 1) wait(spent(fg), (q >> 1) - 1);
+        // (first: it says that all panels up to the one `sets` <= `slots` before
+        // have been through their slots, so that the slot's barrier is at this
+        // panel)
+        const int at_set = q & (p.sets - 1);
+        if (q >= p.sets) wait(spent(at_set), (q >> log_sets) - 1);
         if (sent) wait(full(slot), ring.turn);
         const char* const from = s_slots + slot * slot_bytes;
-        char* const set = s_sets + fg * set_bytes;
+        char* const set = s_sets + at_set * set_bytes;
 #pragma unroll
         for (int it = 0; it < ITS; ++it) {
           const int b = 2 * it + (tid >> 6);
@@ -1400,7 +1406,7 @@ __global__ void __launch_bounds__(kCta, 1)
         tc::fence_smem();
         __syncwarp();
         if (lane == 0) {
-          tc::arrive(ready(fg));
+          tc::arrive(ready(at_set));
           if (sent) tc::arrive(free_(slot));
         }
       }
@@ -2395,9 +2401,13 @@ int launch_weights32(const Shape& s, const void* x, const void* y, const void* v
   p.x_mode = wide_x && s.n > 0 ? (ids ? 1 : 0) : 2;
   p.v_mode = s.M % 4 == 0 && on16(vy) && (!y || on16(y)) ? 0 : 2;
   const int set = 2 * (p.kx + p.mx) * kBox, slot = (p.kx + p.mx * (ACT ? 2 : 1)) * kBox;
-  const int fixed = 2 * set + 24 * 8 + 8;
+  const int bars = 28 * 8 + 8;
   // an x operand's MMA reads 128 rows from its start on: they lie in the sets
   // and slots behind it
+  // Two sets a front group where there is room: the next panel's operands are
+  // made while this one's are multiplied (64-64: 256 -> @@ us).
+  p.sets = (kAll - bars - 4 * set) / slot >= 4 ? 4 : 2;
+  const int fixed = p.sets * set + bars;
   p.slots = (kAll - fixed) / slot;
   p.slots = p.slots > 8 ? 8 : p.slots;
   if (p.x_mode == 2 || p.v_mode == 2) p.slots = p.slots / 2 * 2;
