@@ -1485,6 +1485,8 @@ struct BothArgs {
   int pk, pm;        // panels (64 columns) of K and M: 1 or 2
   int slots, ys;     // tiles of v_y and x, and panels of y, in shared memory
   int biases;
+  int vx_width;      // columns of v_x: K, or fewer where K was padded
+  int wide_out;
 };
 
 // Rows of K and M of up to 128 features, on 16-byte boundaries: v_y, y and x
@@ -1801,9 +1803,9 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         if (into >= p.s.n) into = -1;
         if (!SHARED || live)
           take_results<T, ACT, MODE, TERMS>(live, tmem + buf * TERMS * nk + ((uint32_t)row0 << 16),
-                                            nk, bw >> 2, rows, K, nullptr, into,
-                                            s_stage + bw * 2048, p.vx,
-                                            SHARED ? 0 : row, K, 0, 1);
+                                            nk, bw >> 2, rows, p.vx_width, nullptr, into,
+                                            s_stage + bw * 2048, p.vx, SHARED ? 0 : row,
+                                            p.vx_width, 0, p.wide_out);
         if (live) {
           tc::fence_before_sync();
           __syncwarp();
@@ -1856,18 +1858,21 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
 }
 
 // v_W and v_b of a group: the places of the CTAs that had rows of it, in
-// order; a place has M x K sums and `copies` rows of M sums.  A block takes 256 / SHARES values; its warps take a share of the
+// order; a place has mp x kp sums, of which M x K are wanted, and `copies`
+// rows of mp sums.  A block takes 256 / SHARES values; its warps take a share of the
 // places each, and the shares are added in order.
 template <typename T, int SHARES>
-__global__ void __launch_bounds__(256) join_kernel(Shape s, int parts, int copies,
+__global__ void __launch_bounds__(256) join_kernel(Shape s, int kp, int mp, int parts, int copies,
                                                    const int32_t* __restrict__ off,
                                                    const float* __restrict__ part,
                                                    T* __restrict__ vw, T* __restrict__ vb) {
   constexpr int VALUES = 256 / SHARES;
   __shared__ float s_sum[SHARES][VALUES];
   const int share = threadIdx.x / VALUES, at = threadIdx.x % VALUES;
-  const int64_t mk = (int64_t)s.M * s.K, each = mk + s.M, place = mk + (int64_t)copies * s.M;
+  const int64_t mk = (int64_t)s.M * s.K, each = mk + s.M;
+  const int64_t sums = (int64_t)mp * kp, place = sums + (int64_t)copies * mp;
   const int64_t i = (int64_t)blockIdx.x * VALUES + at;
+  const int64_t in_place = i >= mk ? sums + (i - mk) : kp == s.K ? i : i / s.K * kp + i % s.K;
   const int64_t tiles = (s.R + kTile - 1) / kTile;
   auto part_of = [&](int64_t r) { return (int)(((r / kTile + 1) * parts - 1) / tiles); };
   for (int g = blockIdx.y; g < s.G; g += gridDim.y) {
@@ -1877,13 +1882,13 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int parts, int copie
     if (r0 < r1 && i < each) {
       const int b0 = part_of(r0), n = part_of(r1 - 1) - b0 + 1;
       const int from = n * share / SHARES, to = n * (share + 1) / SHARES;
-      const float* p = part + (int64_t)(b0 + g + from) * place + i;
+      const float* p = part + (int64_t)(b0 + g + from) * place + in_place;
       if (i < mk) {
 #pragma unroll 8
         for (int b = from; b < to; ++b, p += place) sum += __ldg(p);
       } else {
         for (int b = from; b < to; ++b, p += place)
-          for (int c = 0; c < copies; ++c) sum += __ldg(p + (int64_t)c * s.M);
+          for (int c = 0; c < copies; ++c) sum += __ldg(p + (int64_t)c * mp);
       }
     }
     if (SHARES > 1) {
@@ -2168,6 +2173,23 @@ __global__ void __launch_bounds__(256, 2) narrow_bwd_kernel(NarrowArgs p) {
   }
 }
 
+// 16-bit rows of `width` values, `rows` of each `groups`, to rows of `wide`
+// (a multiple of 8), `tall` of each group: what is added is zero.
+template <typename T>
+__global__ void __launch_bounds__(256) pad_kernel(int64_t groups, int64_t rows, int64_t tall,
+                                                  int width, int wide, const T* __restrict__ a,
+                                                  T* __restrict__ b) {
+  const int chunks = wide / 8;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < groups * tall * chunks;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / chunks, g = groups > 1 ? row / tall : 0;
+    const int c = (int)(i - row * chunks) * 8;
+    const bool in = row - g * tall < rows;
+    const int64_t from = in ? (row - g * (tall - rows)) * width + c : 0;
+    reinterpret_cast<uint4*>(b)[i] = get_chunk<T, false>(a + from, in ? width - c : 0);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) round_kernel(int64_t n, const float* __restrict__ a,
                                                     T* __restrict__ b) {
@@ -2361,7 +2383,10 @@ struct Plan {
   int nt, kt, mt, parts;
   int copies;  // of v_b's sums in a place
   bool narrow;
+  bool padded;  // 16-bit rows are copied to whole chunks first
+  int kp, mp;   // K and M as the kernels see them
   size_t part_floats, sum_floats;
+  size_t pad_x, pad_w, pad_v;  // 16-bit values of the copies
 };
 
 Plan plan_of(const gs_grouped_params* p) {  // one CTA an SM, or two
@@ -2371,16 +2396,26 @@ Plan plan_of(const gs_grouped_params* p) {  // one CTA an SM, or two
   q.mt = (int)ceil_div(p->out_features, q.nt);
   const int64_t tiles = ceil_div(p->rows, kTile);
   q.narrow = is_narrow(p->in_features, p->out_features, p->dtype, true);
-  const bool two = q.narrow || (p->dtype != GS_F32 &&
-                                !dims_fit_both(p->in_features, p->out_features));
+  // Rows of 16-bit values that are no whole chunks: a copy of them costs a
+  // fraction of what taking them apart by single values does (200 k rows 77-45:
+  // 223 -> 96 us).
+  q.kp = p->in_features, q.mp = p->out_features;
+  const int k8 = (int)ceil_div(q.kp, 8) * 8, m8 = (int)ceil_div(q.mp, 8) * 8;
+  q.padded = p->dtype != GS_F32 && p->n > 0 && !q.narrow && !dims_fit_both(q.kp, q.mp) &&
+             dims_fit_both(k8, m8);
+  if (q.padded) q.kp = k8, q.mp = m8;
+  const bool two = q.narrow || (p->dtype != GS_F32 && !dims_fit_both(q.kp, q.mp));
   int64_t n = (int64_t)sm_count() * (two ? 2 : 1) / ((int64_t)q.kt * q.mt);
   n = n < 1 ? 1 : n > tiles ? tiles : n;
   q.parts = (int)n;
   q.copies = p->dtype == GS_F32 && !q.narrow ? kBiasCopies32 : 1;
-  q.part_floats =
-      ((size_t)q.parts + p->groups) * p->out_features * ((size_t)p->in_features + q.copies);
+  q.part_floats = ((size_t)q.parts + p->groups) * q.mp * ((size_t)q.kp + q.copies);
   q.sum_floats = p->use_row_ids && p->dtype != GS_F32 ? (size_t)p->n * p->in_features : 0;
   q.part_floats = (q.part_floats + 63) / 64 * 64;  // the sums start on 256 bytes
+  q.sum_floats = (q.sum_floats + 63) / 64 * 64;
+  q.pad_x = q.padded ? (size_t)p->n * q.kp : 0;
+  q.pad_w = q.padded ? (size_t)p->groups * q.mp * q.kp : 0;
+  q.pad_v = q.padded ? (size_t)p->rows * q.mp : 0;
   return q;
 }
 
@@ -2405,7 +2440,7 @@ int launch_weights32(const Shape& s, const void* x, const void* y, const void* v
   // an x operand's MMA reads 128 rows from its start on: they lie in the sets
   // and slots behind it
   // Two sets a front group where there is room: the next panel's operands are
-  // made while this one's are multiplied (64-64: 256 -> @@ us).
+  // made while this one's are multiplied (1.2 M rows 64-64: 256 -> 200 us).
   p.sets = (kAll - bars - 4 * set) / slot >= 4 ? 4 : 2;
   const int fixed = p.sets * set + bars;
   p.slots = (kAll - fixed) / slot;
@@ -2479,7 +2514,8 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
   if (ACT == GS_ACT_NONE) y = nullptr;
   const bool shared = prm->use_row_ids != 0;
   float* const sum = sizeof(T) == 4 ? static_cast<float*>(vx) : ws + q.part_floats;
-  const bool both = !q.narrow && (vw || vb) && fits_both<T>(s, x, w, y, vy, vx);
+  const bool pad = q.padded && (vw || vb) && s.R > 0 && s.n > 0;
+  const bool both = pad || (!q.narrow && (vw || vb) && fits_both<T>(s, x, w, y, vy, vx));
   if (q.narrow) {
     if (vx && shared && cudaMemsetAsync(sum, 0, sizeof(float) * s.n * s.K, st) != cudaSuccess)
       return launch_status("grouped_linear_bwd");
@@ -2502,9 +2538,27 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
         return launch_status("grouped_linear_bwd");
       BothArgs p{};
       p.s = s;
-      p.ids = ids, p.off = off, p.w = w, p.part = ws;
+      p.ids = ids, p.off = off, p.part = ws;
       p.vx = !vx ? nullptr : shared ? sum : vx;
+      p.vx_width = s.K;
+      p.wide_out = s.K * (shared ? 4 : 2) % 16 == 0 && on16(p.vx);
       p.biases = vb != nullptr;
+      if (pad) {
+        T* const xp = reinterpret_cast<T*>(ws + q.part_floats + q.sum_floats);
+        T *const wp = xp + q.pad_x, *const vp = wp + q.pad_w, *const yp = vp + q.pad_v;
+        auto copy = [&](int64_t groups, int64_t rows, int64_t tall, int width, int wide,
+                        const void* from, T* to) {
+          pad_kernel<T><<<grid_for(groups * tall * (wide / 8), 256), 256, 0, st>>>(
+              groups, rows, tall, width, wide, static_cast<const T*>(from), to);
+        };
+        copy(1, s.n, s.n, s.K, q.kp, x, xp);
+        copy(s.G, s.M, q.mp, s.K, q.kp, w, wp);
+        copy(1, s.R, s.R, s.M, q.mp, vy, vp);
+        if (ACT) copy(1, s.R, s.R, s.M, q.mp, y, yp);
+        x = xp, w = wp, vy = vp, y = ACT ? yp : nullptr;
+        p.s.K = q.kp, p.s.M = q.mp;
+      }
+      p.w = w;
       const int rc = shared ? launch_both<T, ACT, true>(p, x, vy, y, q, st)
                             : launch_both<T, ACT, false>(p, x, vy, y, q, st);
       if (rc) return rc;
@@ -2552,13 +2606,14 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
     }
     const int64_t each = (int64_t)s.M * (s.K + 1);
     const unsigned gy = s.G < 65535 ? s.G : 65535;
-    // about parts / G places a group: few are not worth sharing out
-    if (q.parts < 8 * (int64_t)s.G)
+    // a thread a value fills the GPU, or eight warps share a value's places
+    // (19 groups 77-45: 20 against 10 us; 32 groups 128-128: 12 against 27)
+    if (ceil_div(each, 256) * gy >= 2 * sm_count())
       join_kernel<T, 1><<<dim3((unsigned)ceil_div(each, 256), gy), 256, 0, st>>>(
-          s, q.parts, q.copies, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
+          s, q.kp, q.mp, q.parts, q.copies, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
     else
       join_kernel<T, 8><<<dim3((unsigned)ceil_div(each, 32), gy), 256, 0, st>>>(
-          s, q.parts, q.copies, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
+          s, q.kp, q.mp, q.parts, q.copies, off, ws, static_cast<T*>(vw), static_cast<T*>(vb));
   }
   return launch_status("grouped_linear_bwd");
 }
@@ -2628,7 +2683,8 @@ extern "C" int gs_grouped_linear_fwd(const gs_grouped_params* p, const void* x,
 extern "C" size_t gs_grouped_linear_bwd_workspace_size(const gs_grouped_params* p) {
   if (bad_params(p) != GS_OK) return 0;
   const Plan q = plan_of(p);
-  return sizeof(float) * (q.part_floats + q.sum_floats);
+  return sizeof(float) * (q.part_floats + q.sum_floats) +
+         2 * (q.pad_x + q.pad_w + q.pad_v * (p->activation == GS_ACT_NONE ? 1 : 2));
 }
 
 extern "C" int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,

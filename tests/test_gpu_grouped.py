@@ -154,6 +154,14 @@ def test_no_rows(gs, cuda, dtype):
     c["x"] = c["x"][:0]
     assert torch.equal(grouped_linear_forward(c), c["biases"].repeat_interleave(
         torch.tensor([5, 6], device="cuda"), dim=0))
+    # and their gradients: none for x, zeros for the weights, v_y's sums for the biases
+    for K, M in ((8, 4), (16, 16), (77, 45), (200, 9)):
+        c, v_y = _case([5, 6], 4, K, M, TYPES[dtype])
+        c["x"] = c["x"][:0]
+        g = grouped_linear_backward(c, None, v_y)
+        assert g["v_x"].shape == (0, K) and not g["v_weights"].any()
+        want = torch.stack([v_y[:5].double().sum(0), v_y[5:].double().sum(0)]).cpu()
+        assert_sums(g["v_biases"], want, v_y.double().abs().sum(0).cpu().expand(2, M), 11, TYPES[dtype])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
