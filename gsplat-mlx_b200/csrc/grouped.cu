@@ -77,7 +77,9 @@ __device__ __forceinline__ float through(float v, float y) {
 // Operands in 16 bits go to the tensor core as they are.  An fp32 value goes
 // as two tf32 parts, x = hi + lo to 2^-22 |x|; the products hi hi are summed
 // in one accumulator and the three others in a second, which are added in
-// fp32 when the sum is read: about the accuracy of fp32 multiply-adds.  Where the first is not finite it is the
+// fp32 when the sum is read: about the accuracy of fp32 multiply-adds.
+// (A NaN all of whose payload lies in the 13 low bits counts as an infinity.)
+// Where the first accumulator is not finite it is the
 // result: the second has inf - inf and inf * 0 there, and is not finite only
 // where the first is not.  v_z of the
 // sigmoid in 16 bits goes as two parts in the same manner, so that it is not
@@ -420,6 +422,13 @@ __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second
 // the backward through an activation rewrites the panel as v_z.  The group's
 // weights are staged once per group, and stay.
 //
+// Bound by HBM where the MMAs keep up: 2 M rows 128-128 bf16 forward 180 us,
+// 5.7 TB/s of a copy's 6.5; v_x of 1.2 M rows 64-64 fp32, gathered, 180 us, 6.2
+// TB/s of DRAM traffic (the sums' lines are read and written).  fp32 at 128
+// features is bound by its four MMAs a step (600 k rows forward 204 us, twice
+// the floor).  A form that ran a tile's loads, MMAs and results one after the
+// other, two CTAs an SM, took 284 us of the first.
+//
 // How rows arrive: by TMA; gathered, by two warps' copies; by copies of the
 // front warps.  (TMA's four-row gathers took 19 cycles a 128-byte row, 49 us
 // where the copies take 40: 316 k rows 64-64 fp32.)
@@ -428,7 +437,7 @@ constexpr int kLoaders = 64;                          // threads of the gatherin
 constexpr int kCta = 2 * kThreads + 64 + kLoaders;    // front, back, MMA, TMA, gathers
 
 template <typename T, int ACT, int MODE, int LOAD, bool WIDE, bool SPLIT>
-__global__ void __launch_bounds__(kCta, 1)
+__global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
     rows_mma_kernel(RowsArgs p, int columns, const __grid_constant__ CUtensorMap map_a,
                     const __grid_constant__ CUtensorMap map_y) {
   using L = RowsLayout<T, ACT, MODE, SPLIT>;
@@ -1061,6 +1070,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 // was 2e-5 of the result after 8000 rows.  So every kFlush panels the MMAs
 // change accumulators, and the back warps add the finished one to sums that
 // they hold in registers.
+//
+// 1.2 M gathered rows 64-64: 200 us, 4.6 TB/s.  The MMAs (16 a panel, 48 cycles
+// each), the transposition and the copies share the shared memory's 128 bytes
+// a cycle: about 1400 of the 1500 cycles that a panel takes.
 constexpr int kFlush = 4;
 constexpr int kRows32 = 32;
 constexpr int kBox = kRows32 * 128;
@@ -1495,6 +1508,8 @@ struct BothArgs {
 // rows as lanes and the weights (v_x), and with rows as depth and x (v_W: both
 // operands are "MN-major" then, as the weights are in the first product), so
 // nothing is transposed.  The roles of the warps are those of the rows kernel.
+// HBM-bound: 2 M rows 128-128 bf16, relu, 319 us, 6.4 TB/s; v_x and v_W by kernels
+// of their own took 1107 us.
 //
 // v_W's accumulator is added to the CTA's place in `part` at the end of a
 // group, and every kPiece tiles: the tensor core cuts sums to fp32 instead of
@@ -1916,6 +1931,9 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int kp, int mp, int 
 // take a row, 16 bytes each; a lane keeps its columns of the group's weights
 // in registers, and of v_W's sums in the backward, which does all of its parts
 // in the one pass.  A warp has 16 / MP rows per lane in flight.
+//
+// 4 M gathered rows 32-3 fp32: 125 us (as tensor-core tiles 278), 4.6 TB/s of row
+// reads; the instructions issue at 69%.  Its backward, 1.2 M rows: 146 us.
 struct NarrowArgs {
   Shape s;
   const void* x;
@@ -1992,7 +2010,8 @@ __device__ __forceinline__ void hand_over(float (&v)[16], int lane, int o, int& 
 }
 
 template <typename T, int MP, bool WIDE>
-__global__ void __launch_bounds__(256, MP == 4 && sizeof(T) == 4 ? 4 : 2) narrow_fwd_kernel(NarrowArgs p) {
+__global__ void __launch_bounds__(256, MP == 4 && sizeof(T) == 4 ? 4 : 2)
+    narrow_fwd_kernel(NarrowArgs p) {
   NARROW_SETUP
   const T* const bias = static_cast<const T*>(p.bias);
   T* const y = static_cast<T*>(p.y);
@@ -2308,7 +2327,8 @@ int launch_rows(RowsArgs p, cudaStream_t st) {
     if (L::kY)
       if (int rc = make_map(&map_y, p.y, dtype_of<T>, p.s.R, p.depth)) return rc;
   }
-  kernel<<<dim3((unsigned)nx, (unsigned)ny), kCta, L::smem(p), st>>>(
+  kernel<<<dim3((unsigned)nx, (unsigned)ny), LOAD == kGather ? kCta : kCta - kLoaders,
+           L::smem(p), st>>>(
       p, L::columns(p.nt), map_a, map_y);
   return launch_status("grouped_linear");
 }
@@ -2473,7 +2493,8 @@ int launch_weights(const WeightArgs& p, const Plan& q, cudaStream_t st) {
 template <typename T>
 bool fits_both(const Shape& s, const void* x, const void* w, const void* y, const void* vy,
                const void* vx) {
-  return sizeof(T) == 2 && dims_fit_both(s.K, s.M) && s.R > 0 && s.n > 0 && on16(x) && on16(w) && on16(vy) && (!y || on16(y)) && (!vx || on16(vx));
+  return sizeof(T) == 2 && dims_fit_both(s.K, s.M) && s.R > 0 && s.n > 0 && on16(x) && on16(w) &&
+         on16(vy) && (!y || on16(y)) && (!vx || on16(vx));
 }
 
 template <typename T, int ACT, bool SHARED>
