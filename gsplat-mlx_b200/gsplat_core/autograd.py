@@ -25,6 +25,7 @@ non-differentiable.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _gsplat_core as G
 from .dropout import dropout_backward, dropout_forward
@@ -212,6 +213,7 @@ class _GroupedLinear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, v_y):
         x, weights, offsets, biases, row_ids, y = ctx.saved_tensors
         names = {"v_x": 0, "v_weights": 1, "v_biases": 3}
@@ -238,6 +240,7 @@ class _Dropout(torch.autograd.Function):
         return dropout_forward(x, p, seed, step, rows)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, v_y):
         p, seed, step, rows = ctx.cfg
         step = ctx.saved_tensors[0] if step is None else step

@@ -56,6 +56,9 @@ def dropout_forward(x, p, seed, step=0, rows=False, out=None):
         raise RuntimeError("dropout: x must be a CUDA tensor (there is no CPU fallback).")
     x = x.contiguous()
     y = torch.empty_like(x) if out is None else out
+    size = x.numel() * x.element_size()
+    if out is not None and 0 < abs(y.data_ptr() - x.data_ptr()) < size:
+        raise RuntimeError("dropout: out overlaps x without being x.")
     prm = DropoutParams(n, width, int(seed) & _U64, int(step) & _U64, p, _DTYPES[x.dtype],
                         int(bool(rows)))
     lib = _lib.load()

@@ -45,8 +45,7 @@ class ImageFitStep:
         self.lib = _lib.load()
         e = lambda *shape: torch.empty(shape, dtype=torch.float32, device=self.dev)  # noqa: E731
         self.quats_n, self.scales, self.colors, self.opacities = e(n, 4), e(n, 3), e(n, 3), e(n)
-        if self.dropout > 0.0:
-            self.opacities_kept = e(n)
+        self.opacities_kept = e(n if self.dropout > 0.0 else 0)  # of the last iteration
         self.m1 = torch.zeros((n, 14), dtype=torch.float32, device=self.dev)
         self.m2 = torch.zeros((n, 14), dtype=torch.float32, device=self.dev)
         self.hp = AdamParams(n, float(lr), float(beta1), float(beta2), float(eps))
@@ -65,6 +64,8 @@ class ImageFitStep:
         opacities, draw = self.opacities, None
         if self.dropout > 0.0:
             draw = (self.dropout, self.dropout_seed, self.iteration, True)
+            if self.opacities_kept.numel() != self.n:
+                self.opacities_kept = torch.empty_like(opacities)
             opacities = dropout_forward(opacities, *draw, out=self.opacities_kept)
         st.run(self.means, self.quats_n, self.scales, opacities, self.coeffs_unused,
                self.viewmats, self.Ks, None, None, colors=self.colors, target=self.target)

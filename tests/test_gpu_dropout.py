@@ -97,6 +97,9 @@ def test_in_place_and_far_places(gs, cuda):
     x = _x((4097,), torch.float32)
     y = dropout_forward(x, 0.4, 9)
     assert dropout_forward(x, 0.4, 9, out=x) is x and torch.equal(x, y)
+    buf = torch.zeros((4100,), device="cuda")
+    with pytest.raises(RuntimeError, match="overlaps"):
+        dropout_forward(buf[:4097], 0.4, 9, out=buf[3:])
     n = (1 << 31) + 4096 + 7
     big = torch.ones((n,), dtype=torch.bfloat16, device="cuda")
     dropout_forward(big, 0.5, 21, step=2, out=big)

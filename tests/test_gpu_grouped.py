@@ -24,6 +24,8 @@ FEW = [
     ([513], 700, 48, 8), ([40] * 40, 100, 16, 5), ([333], 0, 250, 3), ([129, 1], 99, 7, 7),
     ([700], 0, 256, 8), ([2000, 3000], 1500, 4, 4), ([65], 0, 129, 3), ([65], 80, 257, 3),
     ([31, 1, 1, 64], 20, 8, 6), ([5], 3, 1, 8)]
+# more features than shared memory holds weights of
+MANY = [([150, 90], 0, 3700, 24), ([150, 90], 60, 24, 3700), ([140], 0, 1000, 40)]
 
 
 def _case(sizes, N, K, M, dtype, seed=0, bias=True):
@@ -78,7 +80,7 @@ def _check_backward(c, y, v_y, got, act):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("sizes,N,K,M", SHAPES + FEW)
+@pytest.mark.parametrize("sizes,N,K,M", SHAPES + FEW + MANY)
 @pytest.mark.parametrize("act", ["none", "relu", "sigmoid"])
 def test_grouped_matches_64_bits(gs, cuda, dtype, sizes, N, K, M, act):
     from gsplat_core.grouped import grouped_linear_backward, grouped_linear_forward
@@ -228,6 +230,52 @@ def test_wanted_gradients(gs, cuda):
         got = grouped_linear_backward(c, y, v_y, activation="sigmoid", wanted=wanted)
         assert set(got) == set(wanted)
         _check_backward(c, y, v_y, got, "sigmoid")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K,M,N", [(64, 32, 0), (77, 45, 300), (32, 3, 300), (200, 40, 0)])
+def test_wanted_gradients_of_each_kernel(gs, cuda, dtype, K, M, N):
+    """Any subset gives the bits of the whole (v_x of shared rows: within
+    their tolerance, their order is not fixed)."""
+    from gsplat_core.grouped import grouped_linear_backward, grouped_linear_forward
+    c, v_y = _case([500, 0, 300], N, K, M, TYPES[dtype])
+    y = grouped_linear_forward(c, activation="relu")
+    whole = grouped_linear_backward(c, y, v_y, activation="relu")
+    _check_backward(c, y, v_y, whole, "relu")
+    for wanted in (("v_x",), ("v_weights",), ("v_biases",), ("v_x", "v_biases")):
+        got = grouped_linear_backward(c, y, v_y, activation="relu", wanted=wanted)
+        assert set(got) == set(wanted)
+        _check_backward(c, y, v_y, got, "relu")
+        for k in wanted:
+            if k != "v_x":
+                assert torch.equal(got[k], whole[k]), k
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strided_inputs(gs, cuda, dtype):
+    """Inputs that are not contiguous are taken as they read."""
+    from gsplat_core.grouped import grouped_linear_backward, grouped_linear_forward
+    c, v_y = _case([200, 70], 150, 32, 24, TYPES[dtype])
+    s = {"x": c["x"].t().contiguous().t(), "weights": c["weights"].transpose(1, 2).contiguous().transpose(1, 2),
+         "biases": c["biases"].repeat_interleave(2, dim=1)[:, ::2],
+         "offsets": c["offsets"].repeat_interleave(3)[::3], "row_ids": c["row_ids"].repeat_interleave(2)[::2]}
+    assert not any(t.is_contiguous() for t in s.values())
+    y = grouped_linear_forward(s, activation="sigmoid")
+    assert torch.equal(y, grouped_linear_forward(c, activation="sigmoid"))
+    g = grouped_linear_backward(s, y.t().contiguous().t(), v_y.t().contiguous().t(), activation="sigmoid")
+    _check_backward(c, y, v_y, g, "sigmoid")
+
+
+def test_no_second_derivative(gs, cuda):
+    """A second derivative is refused instead of being zero."""
+    from gsplat_core import autograd as A
+    c, _ = _case([20], 0, 8, 4, torch.float32)
+    x = c["x"].clone().requires_grad_(True)
+    for y in (A.grouped_linear(x, c["weights"], c["offsets"], activation="sigmoid"),
+              A.dropout(x, 0.5, 1)):
+        g, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
 
 
 def test_graphs_and_streams(gs, cuda):
