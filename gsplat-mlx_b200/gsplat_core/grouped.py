@@ -58,31 +58,34 @@ def _validated(inputs, activation):
             raise RuntimeError(f"grouped_linear missing input: {k}")
     x, w, off = inputs["x"], inputs["weights"], inputs["offsets"]
     b, ids = inputs.get("biases"), inputs.get("row_ids")
-    if x.dim() != 2 or x.dtype not in _DTYPES:
+    dtype = x.dtype
+    if x.dim() != 2 or dtype not in _DTYPES:
         raise RuntimeError("grouped_linear: x must have shape [rows, K] and type float32, "
                            "bfloat16 or float16.")
-    if w.dim() != 3 or w.shape[2] != x.shape[1] or w.dtype != x.dtype:
+    n, K = x.shape
+    if w.dim() != 3 or w.shape[2] != K or w.dtype != dtype:
         raise RuntimeError("grouped_linear: weights must have shape [G, M, K] and x's type.")
-    G, M, K = w.shape
+    G, M, _ = w.shape
     if min(G, M, K) < 1 or max(M, K) > 16384:
         raise RuntimeError("grouped_linear: G, M and K must be at least 1, M and K at most 16384.")
     if off.shape != (G + 1,) or off.dtype != torch.int32:
         raise RuntimeError("grouped_linear: offsets must have shape [G + 1] and type int32.")
-    if b is not None and (b.shape != (G, M) or b.dtype != x.dtype):
+    if b is not None and (b.shape != (G, M) or b.dtype != dtype):
         raise RuntimeError("grouped_linear: biases must have shape [G, M] and x's type.")
     if ids is not None and (ids.dim() != 1 or ids.dtype != torch.int32):
         raise RuntimeError("grouped_linear: row_ids must have shape [rows] and type int32.")
     if activation not in _ACTIVATIONS:
         raise RuntimeError("grouped_linear: activation must be none, relu or sigmoid.")
-    ts = [x, w, off, b, ids]
-    if any(t is not None and t.device != x.device for t in ts):
+    at = x.get_device()  # -1: the host
+    if (w.get_device() != at or off.get_device() != at or (b is not None and b.get_device() != at)
+            or (ids is not None and ids.get_device() != at)):
         raise RuntimeError("grouped_linear: inputs on different devices.")
-    R = x.shape[0] if ids is None else ids.shape[0]
-    if max(R, x.shape[0]) >= 2 ** 31 - 4096:
+    R = n if ids is None else ids.shape[0]
+    if max(R, n) >= 2 ** 31 - 4096:
         raise RuntimeError("grouped_linear: 2^31 - 4096 rows or more.")
-    p = GroupedParams(R, x.shape[0], G, K, M, _DTYPES[x.dtype], _ACTIVATIONS[activation],
-                      int(ids is not None))
-    return p, [None if t is None else t.contiguous() for t in ts]
+    p = GroupedParams(R, n, G, K, M, _DTYPES[dtype], _ACTIVATIONS[activation], int(ids is not None))
+    return p, (x.contiguous(), w.contiguous(), off.contiguous(),
+               None if b is None else b.contiguous(), None if ids is None else ids.contiguous())
 
 
 def _on_cuda(t):
@@ -103,7 +106,7 @@ def grouped_linear_forward(inputs, activation="none"):
     zeros; a row id outside [0, N) reads zeros."""
     p, (x, w, off, b, ids) = _validated(inputs, activation)
     _on_cuda(x)
-    y = torch.empty((p.rows, p.out_features), dtype=x.dtype, device=x.device)
+    y = x.new_empty((p.rows, p.out_features))
     lib = _lib.load()
     check_status(on_device_of(x, lambda stream: lib.gs_grouped_linear_fwd(
         ct.byref(p), _ptr(x), _ptr(ids), _ptr(off), _ptr(w), _ptr(b), _ptr(y), stream)),
@@ -143,7 +146,7 @@ def grouped_linear_backward(inputs, y, v_y, activation="none",
 
     def call(stream):
         need = lib.gs_grouped_linear_bwd_workspace_size(ct.byref(p))
-        ws = torch.empty((need,), dtype=torch.uint8, device=x.device)
+        ws = off.new_empty((need + 3) // 4)
         return lib.gs_grouped_linear_bwd(
             ct.byref(p), _ptr(x), _ptr(ids), _ptr(off), _ptr(w), _ptr(y), _ptr(v_y),
             _ptr(out.get("v_x")), _ptr(out.get("v_weights")), _ptr(out.get("v_biases")),
