@@ -1933,8 +1933,9 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int kp, int mp, int 
 // in registers, and of v_W's sums in the backward, which does all of its parts
 // in the one pass.  A warp has 16 / MP rows per lane in flight.
 //
-// 4 M gathered rows 32-3 fp32: 125 us (as tensor-core tiles 278), 4.6 TB/s of row
-// reads; the instructions issue at 69%.  Its backward, 1.2 M rows: 125 us.
+// 4 M gathered rows 32-3 fp32: 125 us (as tensor-core tiles 278), 4.1 TB/s of
+// scattered 128-byte row reads, which is what bounds it: 7% fewer instructions
+// changed nothing.  Its backward, 1.2 M rows: 125 us.
 struct NarrowArgs {
   Shape s;
   const void* x;
@@ -1999,15 +2000,12 @@ __device__ __forceinline__ float through_as(int act, float v, float y) {
 
 // A lane keeps H of its 2 H values, with the partner's share of them.
 template <int H>
-__device__ __forceinline__ void hand_over(float (&v)[16], int lane, int o, int& n, int& first) {
-  const bool up = lane & o;
+__device__ __forceinline__ void hand_over(float (&v)[16], bool up, int o) {
 #pragma unroll
   for (int i = 0; i < H; ++i) {
     const float mine = up ? v[i + H] : v[i];
     v[i] = mine + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + H], o);
   }
-  n = H;
-  first += up ? H : 0;
 }
 
 template <typename T, int MP, bool WIDE>
@@ -2016,6 +2014,11 @@ __global__ void __launch_bounds__(256, MP == 4 && sizeof(T) == 4 ? 4 : 2)
   NARROW_SETUP
   const T* const bias = static_cast<const T*>(p.bias);
   T* const y = static_cast<T*>(p.y);
+  // A row's lanes end up with 16 / lpr of its U x MP values each: lane c with
+  // those from c 16 / lpr on, n of them (of 32 lanes every second has one).
+  const int n = p.lpr > 16 ? 1 - (lane & 1) : 16 / p.lpr;
+  const int first = p.lpr > 16 ? c >> 1 : c * (16 / p.lpr);
+  const int m0 = first % MP, u0 = first / MP;
   for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
     const int stop = cur.row + cur.n;
     if (cur.g < 0 || cur.g >= p.s.G) {
@@ -2024,6 +2027,12 @@ __global__ void __launch_bounds__(256, MP == 4 && sizeof(T) == 4 ? 4 : 2)
       continue;
     }
     read_weights(cur.g);
+    float b[MP];  // of the values that this lane ends up with
+#pragma unroll
+    for (int i = 0; i < MP; ++i) {
+      const int m = n < MP ? m0 + i : i;
+      b[i] = bias && m < M ? to_f(__ldg(bias + (int64_t)cur.g * M + m)) : 0.0f;
+    }
     int r = cur.row + warp * U * set;
     read_ids(r, stop);
     for (; r < stop; r += 8 * U * set) {
@@ -2045,25 +2054,19 @@ __global__ void __launch_bounds__(256, MP == 4 && sizeof(T) == 4 ? 4 : 2)
           v[u * MP + m] = a;
         }
       // The row's lanes add up their parts; each step a lane hands half of its
-      // values to the partner and adds the partner's other half, until lane
-      // c has the 16 / lpr values from c 16 / lpr on (one, twice, for 32).
-      int n = 16, first = 0;
-      if (p.lpr > 1) hand_over<8>(v, lane, p.lpr >> 1, n, first);
-      if (p.lpr > 2) hand_over<4>(v, lane, p.lpr >> 2, n, first);
-      if (p.lpr > 4) hand_over<2>(v, lane, p.lpr >> 3, n, first);
-      if (p.lpr > 8) hand_over<1>(v, lane, p.lpr >> 4, n, first);
-      if (p.lpr > 16) {
-        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
-        if (lane & 1) n = 0;
-      }
+      // values to the partner and adds the partner's other half.
+      if (p.lpr > 1) hand_over<8>(v, lane & (p.lpr >> 1), p.lpr >> 1);
+      if (p.lpr > 2) hand_over<4>(v, lane & (p.lpr >> 2), p.lpr >> 2);
+      if (p.lpr > 4) hand_over<2>(v, lane & (p.lpr >> 3), p.lpr >> 3);
+      if (p.lpr > 8) hand_over<1>(v, lane & (p.lpr >> 4), p.lpr >> 4);
+      if (p.lpr > 16) v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         if (i >= n) break;
-        const int m = (first + i) % MP, row = r + (first + i) / MP * set + rg;
-        if (m < M && row < stop) {
-          const float b = bias ? to_f(__ldg(bias + (int64_t)cur.g * M + m)) : 0.0f;
-          y[(int64_t)row * M + m] = from_f<T>(activate_as(p.act, v[i] + b));
-        }
+        // (n values of one row, or whole rows)
+        const int m = n < MP ? m0 + i : i % MP, row = r + (u0 + i / MP) * set + rg;
+        if (m < M && row < stop)
+          y[(int64_t)row * M + m] = from_f<T>(activate_as(p.act, v[i] + b[i % MP]));
       }
     }
   }
