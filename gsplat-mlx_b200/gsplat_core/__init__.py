@@ -7,7 +7,9 @@ module ``_gsplat_core``; this package does the same with a ctypes binding of
 
 Extras beyond the reference surface live in submodules: ``autograd``
 (torch.autograd wiring of the operators' VJPs), ``pipeline`` (preallocated
-fused training step), ``synthetic`` (seeded benchmark scenes).
+fused training step), ``packed`` (rows of visible entries), ``grouped`` and
+``dropout`` (colours learned per camera, and their regulariser),
+``synthetic`` (seeded benchmark scenes).
 """
 from ._gsplat_core import *  # noqa: F401,F403
 from ._gsplat_core import (floor_log2_plus_one, intersect_tile_count,  # noqa: F401
