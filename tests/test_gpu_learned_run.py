@@ -118,3 +118,35 @@ def test_fit_step_with_dropout(gs, cuda):
         assert (m[~seen] == 0).all() and (m[seen] != 0).any()
     a, b = mk(), mk(dropout=0.0, dropout_seed=5)
     assert float(a.run()) == pytest.approx(float(b.run()), rel=1e-6)
+
+
+def test_captured_training_step(gs, cuda):
+    """Forward and backward through autograd in one captured graph, with a
+    new mask at each replay: the gradients of an eager step of that mask."""
+    from gsplat_core import autograd as A
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(900, 16, generator=g).cuda().requires_grad_(True)
+    w = (torch.randn(3, 24, 16, generator=g) / 4).cuda().requires_grad_(True)
+    b = torch.randn(3, 24, generator=g).cuda().requires_grad_(True)
+    off = torch.tensor([0, 300, 320, 900], dtype=torch.int32, device="cuda")
+    v = torch.randn(900, 24, generator=g).cuda()
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+
+    def run(at):
+        h = A.dropout(A.grouped_linear(x, w, off, b, None, "relu"), 0.3, 7, at)
+        return torch.autograd.grad(h, (x, w, b), v)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            run(step)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = run(step)
+    for it in (0, 3, 11):
+        step.fill_(it)
+        graph.replay()
+        for got, want in zip(grads, run(it)):
+            assert torch.equal(got, want), it
