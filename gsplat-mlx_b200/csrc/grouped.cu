@@ -1488,6 +1488,20 @@ __global__ void __launch_bounds__(kCta, 1)
   if (warp == 0) tc::dealloc(tmem, 4 * NT);
 }
 
+// A lane's 16 sums of an accumulator (`there` of them are wanted) to its column of
+// the CTA's place, `pitch` floats apart: the first piece of a group is
+// written, the others are added without waiting for what is there.  No other
+// thread has these sums, so the order of the additions is the pieces'.
+__device__ __forceinline__ void add_piece(float* at, int pitch, int there, const float (&v)[16],
+                                          bool first) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (i >= there) break;
+    if (first) at[(int64_t)i * pitch] = v[i];
+    else atomicAdd(at + (int64_t)i * pitch, v[i]);
+  }
+}
+
 // ------------------------------------------------- the whole backward, 16 bits
 struct BothArgs {
   Shape s;
@@ -1514,8 +1528,10 @@ struct BothArgs {
 //
 // v_W's accumulator is added to the CTA's place in `part` at the end of a
 // group, and every kPiece tiles: the tensor core cuts sums to fp32 instead of
-// rounding them, 2^-24 of the sum at each of a tile's 8 additions.
-constexpr int kPiece = 32;
+// rounding them, 2^-24 of the sum on average at each of a tile's 8 additions
+// (32 tiles: 2 M rows 128-128 were 2e-6 low).
+constexpr int kPiece = 4;
+constexpr int kBothBars = 29;
 
 template <typename T, int ACT, bool SHARED>
 __global__ void __launch_bounds__(2 * kThreads + 64, 1)
@@ -1523,7 +1539,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
                     const __grid_constant__ CUtensorMap map_y,
                     const __grid_constant__ CUtensorMap map_x) {
   constexpr int TERMS = ACT == GS_ACT_SIGMOID ? 2 : 1;  // parts of v_z
-  constexpr int NBUF = TERMS == 2 ? 1 : 2;              // accumulators of v_x
+  constexpr int NBUF = TERMS == 2 ? 1 : 2;              // accumulators of v_x, and of v_W
   constexpr bool HAS_Y = ACT != GS_ACT_NONE;
   // all of it dynamic: the panels have to start on 1024 bytes, with nothing lost
   extern __shared__ __align__(1024) char smem_raw[];
@@ -1538,7 +1554,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   char* const s_stage = s_w + p.pk * kPanel;
   float (*const s_db)[64] = reinterpret_cast<float (*)[64]>(s_stage + 8 * 2048);
   uint64_t* const s_bars = reinterpret_cast<uint64_t*>(s_db + 8);
-  uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + 27);
+  uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + kBothBars);
   const uint32_t bar0 = tc::smem_addr(s_bars);
   auto full = [&](int i) { return bar0 + 8 * i; };
   auto free_ = [&](int i) { return bar0 + 8 * (4 + i); };
@@ -1547,7 +1563,9 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   auto y_free = [&](int i) { return bar0 + 8 * (16 + i); };
   auto made = [&](int i) { return bar0 + 8 * (20 + i); };
   auto taken = [&](int i) { return bar0 + 8 * (22 + i); };
-  const uint32_t weighed = bar0 + 8 * 24, sum_made = bar0 + 8 * 25, sum_taken = bar0 + 8 * 26;
+  auto sum_made = [&](int i) { return bar0 + 8 * (24 + i); };
+  auto sum_taken = [&](int i) { return bar0 + 8 * (26 + i); };
+  const uint32_t weighed = bar0 + 8 * 28;
 
   if (warp == 0) tc::alloc(&s_tmem, columns);
   if (threadIdx.x == 32) {
@@ -1561,10 +1579,10 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     for (int i = 0; i < 2; ++i) {
       tc::bar_init(made(i), 1);
       tc::bar_init(taken(i), 8);
+      tc::bar_init(sum_made(i), 1);
+      tc::bar_init(sum_taken(i), 8);
     }
     tc::bar_init(weighed, 8);
-    tc::bar_init(sum_made, 1);
-    tc::bar_init(sum_taken, 8);
     tc::bar_init_done();
   }
   tc::fence_before_sync();
@@ -1669,21 +1687,23 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         }
         tc::commit(leader, made(buf));
       }
-      if (piece == 0 && sums > 0) wait(sum_taken, sums - 1);
+      const int sum_buf = NBUF == 2 ? sums & 1 : 0;
+      if (piece == 0 && sums >= NBUF) wait(sum_taken(sum_buf), sums / NBUF - 1);
       tc::fence_after_sync();
+      const uint32_t sum = sum_acc + sum_buf * nm;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {        // 16 rows
         const uint64_t dx = tc::smem_desc_mn(x_at + i * 2048, k_blocks);
-        tc::mma<false>(leader, sum_acc, dx, tc::smem_desc_mn(v_at + i * 2048, kPanel), by_sums,
+        tc::mma<false>(leader, sum, dx, tc::smem_desc_mn(v_at + i * 2048, kPanel), by_sums,
                        piece > 0 || i > 0);
         if (TERMS == 2)
-          tc::mma<false>(leader, sum_acc + nm, dx, tc::smem_desc_mn(low_at + i * 2048, kPanel),
+          tc::mma<false>(leader, sum + nm, dx, tc::smem_desc_mn(low_at + i * 2048, kPanel),
                          by_sums, piece > 0 || i > 0);
       }
       tc::commit(leader, free_(slot));
       for (int j = 0; TERMS == 2 && j < p.pm; ++j) tc::commit(leader, y_free(ys + j));
       if (++piece == kPiece || left <= kTile) {
-        tc::commit(leader, sum_made);
+        tc::commit(leader, sum_made(sum_buf));
         ++sums;
         piece = 0;
       }
@@ -1832,35 +1852,27 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         ++t;
         const bool last = left <= kTile;
         if (++piece == kPiece || last) {
-          wait(sum_made, sums);
+          const int sum_buf = NBUF == 2 ? sums & 1 : 0;
+          wait(sum_made(sum_buf), sums / NBUF);
           tc::fence_after_sync();
+          const uint32_t sum = sum_acc + sum_buf * nm + ((uint32_t)row0 << 16);
           float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1));
           const int kk = row0 + lane;
           for (int c0 = (bw >> 2) * 16; c0 < M; c0 += 32) {
             float v[16];
-            tc::load16(sum_acc + ((uint32_t)row0 << 16) + c0, v);
+            tc::load16(sum + c0, v);
             if (TERMS == 2) {
               float u[16];
-              tc::load16(sum_acc + nm + ((uint32_t)row0 << 16) + c0, u);
+              tc::load16(sum + nm + c0, u);
 #pragma unroll
               for (int i = 0; i < 16; ++i)
                 if (fabsf(v[i]) < INFINITY) v[i] += u[i];
             }
-            float* const at = to + (int64_t)c0 * K + kk;
-            if (!first && kk < K) {  // all read before the first is written
-              float u[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) u[i] = c0 + i < M ? at[(int64_t)i * K] : 0.0f;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] += u[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (kk < K && c0 + i < M) at[(int64_t)i * K] = v[i];
+            if (kk < K) add_piece(to + (int64_t)c0 * K + kk, K, M - c0, v, first);
           }
           tc::fence_before_sync();
           __syncwarp();
-          if (lane == 0) tc::arrive(sum_taken);
+          if (lane == 0) tc::arrive(sum_taken(sum_buf));
           ++sums;
           piece = 0;
           first = last;
@@ -2516,19 +2528,19 @@ int launch_both(BothArgs p, const void* x, const void* vy, const void* y, const 
   constexpr int kAll = 227 * 1024;  // this kernel has no static shared memory
   if (int rc = allow_smem<kernel, kAll>()) return rc;
   p.pk = p.s.K > 64 ? 2 : 1, p.pm = p.s.M > 64 ? 2 : 1;
-  const int terms = ACT == GS_ACT_SIGMOID ? 2 : 1;
+  const int terms = ACT == GS_ACT_SIGMOID ? 2 : 1;  // parts of v_z
   // As many tiles as there is room for beside one tile of y, then as many
   // panels of y (whole tiles where the low parts of v_z lie in them).
   p.slots = 2, p.ys = ACT ? p.pm : 0;
   auto smem = [&]() {
-    return 8 * 2048 + 2048 + 27 * 8 + 8 + kPanel * (p.pk + p.slots * (p.pm + p.pk) + p.ys);
+    return 8 * 2048 + 2048 + kBothBars * 8 + 8 + kPanel * (p.pk + p.slots * (p.pm + p.pk) + p.ys);
   };
   while (p.slots < 4 && smem() + (p.pm + p.pk) * kPanel <= kAll) ++p.slots;
   const int more = terms == 2 ? p.pm : 1;
   while (ACT && p.ys + more <= 4 && smem() + more * kPanel <= kAll) p.ys += more;
   const int nk = (p.s.K + 31) / 32 * 32, nm = (p.s.M + 31) / 32 * 32;
   int columns = 32;
-  while (columns < 2 * nk + terms * nm) columns *= 2;
+  while (columns < 2 * nk + 2 * nm) columns *= 2;  // two accumulators, or two parts of one
   CUtensorMap map_v{}, map_y{}, map_x{};
   if (int rc = make_map(&map_v, vy, dtype_of<T>, p.s.R, p.s.M)) return rc;
   if (ACT)
