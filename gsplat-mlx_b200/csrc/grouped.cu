@@ -83,7 +83,10 @@ __device__ __forceinline__ float through(float v, float y) {
 // result: the second has inf - inf and inf * 0 there, and is not finite only
 // where the first is not.  v_z of the
 // sigmoid in 16 bits goes as two parts in the same manner, so that it is not
-// rounded to 16 bits on its way.
+// rounded to 16 bits on its way.  fp16 ends at 2^-24, next to the gradients of a
+// mean over an image, so its second part is held times 2^11 (it is at most 2^4:
+// half a step of the first) and what it gives is scaled back where the sums are
+// joined: v_z is carried to 2^-22 of itself and to 2^-36.  bf16 has fp32's range.
 __device__ unsigned int g_wait_gave_up;
 constexpr uint32_t kWaitLimit = 1u << 16;  // polls of the hardware's own bounded wait
 
@@ -120,6 +123,18 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
 }
 
+// What the second part of a value in 16 bits is held times.
+template <typename T> constexpr float kLowScale = 1.0f;
+template <> constexpr float kLowScale<__half> = 2048.0f;
+
+// Sums of the first parts joined with those of the second.
+template <typename T>
+__device__ __forceinline__ void join_parts(float (&v)[16], const float (&u)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (fabsf(v[i]) < INFINITY) v[i] = fmaf(u[i], 1.0f / kLowScale<T>, v[i]);
+}
+
 // Writes f[0..E) as one operand chunk: one part, or two at a panel's distance.
 template <typename T, bool SPLIT>
 __device__ __forceinline__ void put_chunk(char* at, ptrdiff_t lo_offset, const float* f) {
@@ -127,7 +142,7 @@ __device__ __forceinline__ void put_chunk(char* at, ptrdiff_t lo_offset, const f
 #pragma unroll
   for (int e = 0; e < Chunk<T>::E; ++e) {
     hi.v[e] = from_f<T>(f[e]);
-    if (SPLIT && sizeof(T) == 2) lo.v[e] = from_f<T>(f[e] - to_f(hi.v[e]));
+    if (SPLIT && sizeof(T) == 2) lo.v[e] = from_f<T>((f[e] - to_f(hi.v[e])) * kLowScale<T>);
   }
   *reinterpret_cast<uint4*>(at) = hi.q;
   if constexpr (sizeof(T) == 4) put_low(at + lo_offset, hi);
@@ -328,9 +343,7 @@ __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second
         if (TERMS == 2) {
           float u[16];
           tc::load16(acc + second + c0 + h * 16, u);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+          join_parts<T>(v, u);
         }
       }
       if (!live) {
@@ -1024,9 +1037,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (SPLIT) {
           float u[16];
           tc::load16(from + NT, u);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+          join_parts<T>(v, u);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -1864,9 +1875,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
             if (TERMS == 2) {
               float u[16];
               tc::load16(sum + nm + c0, u);
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (fabsf(v[i]) < INFINITY) v[i] += u[i];
+              join_parts<T>(v, u);
             }
             if (kk < K) add_piece(to + (int64_t)c0 * K + kk, K, M - c0, v, first);
           }

@@ -704,7 +704,9 @@ size_t gs_grouped_linear_bwd_workspace_size(const gs_grouped_params* p);
  * v_y [R,M].  With v_z = v_y act'(y): v_x [n,K] = the sum over the rows that
  * read it of v_z[r] weights[g] (zeros where none does), v_weights [G,M,K] =
  * the sum over g's rows of v_z[r]^T x[id(r)], v_biases [G,M] = the sum of
- * v_z[r]; each may be NULL (not wanted).  v_weights and v_biases are summed
+ * v_z[r]; each may be NULL (not wanted).  Behind a sigmoid v_z is carried to
+ * 2^-22 of itself and to 2^-36 in fp16, and to 2^-16 in bf16.  v_weights and
+ * v_biases are summed
  * in a fixed order; v_x is too, except that with row_ids the rows of one id
  * are added atomically in fp32. */
 int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,

@@ -80,3 +80,41 @@ def test_long_group_in_one_pass(gs, cuda, dtype, act):
     bound = _bound(32, 160, TYPES[dtype]) + extra
     _assert_sums(got["v_weights"], w, bound, what="v_weights")
     _assert_sums(got["v_biases"], b, _bound(0, 1200, TYPES[dtype]) + extra, what="v_biases")
+
+
+@pytest.mark.parametrize("gathered", [False, True])
+@pytest.mark.parametrize("K,M,R", [(64, 16, 200_000), (77, 45, 50_000), (200, 136, 50_000), (32, 3, 50_000)])
+@pytest.mark.parametrize("size", ["1e-6", "2^-24", "1"])
+def test_small_gradients_of_fp16_behind_a_sigmoid(gs, cuda, gathered, K, M, R, size):
+    """v_z = v_y y (1 - y) is below fp16's normal range, or all of its range,
+    before it is multiplied: it is carried to 2^-22 of itself and to 2^-36,
+    and its sums are right where fp16 holds them."""
+    from gsplat_core.grouped import grouped_linear_backward
+    half = torch.float16
+    top = {"1e-6": 1e-6, "2^-24": 2.0 ** -24, "1": 1.0}[size]
+    c, y, v = _positive(R, 2, K, M, half, 8)
+    v = torch.full_like(v, top) if top < 1 else v / 64
+    edges = [0, 900, R]
+    c["offsets"] = torch.tensor(edges, dtype=torch.int32, device="cuda")
+    w = c["weights"] = c["weights"] * (1 if top == 1 else 256)  # so that v_x is in fp16's range
+    rows = c["x"]
+    if gathered:
+        ids = torch.randperm(R, generator=torch.Generator().manual_seed(1)).cuda()
+        c["row_ids"] = ids.to(torch.int32)
+        rows = rows[ids]
+    vz = v.double() * y.double() * (1 - y.double())
+    want_w, want_b = _weight_sums(rows, y, v, "sigmoid", edges)
+    want_x = torch.cat([vz[:900] @ w[0].double(), vz[900:] @ w[1].double()])
+    # of itself: two parts, three roundings; below: half a step of the second part
+    part = 2.0 ** -22 + 3 * 2.0 ** -24
+    low = lambda other: 2.0 ** -36 * other.double().abs().sum(0)  # noqa: E731
+    for wanted in (("v_x", "v_weights", "v_biases"), ("v_x",)):
+        got = grouped_linear_backward(c, y, v, activation="sigmoid", wanted=wanted)
+        x = got["v_x"][ids] if gathered else got["v_x"]
+        for s, g in ((slice(0, 900), 0), (slice(900, R), 1)):
+            _assert_sums(x[s], want_x[s], _bound(9, 4, half) + part, low(w[g]), what="v_x")
+            if "v_weights" in got:
+                _assert_sums(got["v_weights"][g], want_w[g], _bound(64, 400, half) + part,
+                             low(rows[s]), what="v_weights")
+                _assert_sums(got["v_biases"][g], want_b[g], _bound(0, 400, half) + part,
+                             what="v_biases")
