@@ -854,6 +854,24 @@ struct WeightArgs {
   int biases;
 };
 
+// The first piece of a sum is written, the others are added without waiting
+// for what is there.  No other thread has the sum, so the order of the
+// additions is the pieces'.
+__device__ __forceinline__ void add_to(float* at, float v, bool first) {
+  if (first) *at = v;
+  else atomicAdd(at, v);
+}
+// A lane's 16 sums of an accumulator (`there` of them are wanted) to its column of
+// the CTA's place, `pitch` floats apart.
+__device__ __forceinline__ void add_piece(float* at, int pitch, int there, const float (&v)[16],
+                                          bool first) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (i >= there) break;
+    add_to(at + (int64_t)i * pitch, v[i], first);
+  }
+}
+
 // v_W[g] (as K lanes x M columns) = sum over g's rows of x[r]^T v_z[r], of
 // 16-bit rows that the kernel for the whole backward does not take: off the 16-byte
 // boundary, or more than 128 features.
@@ -863,7 +881,11 @@ struct WeightArgs {
 // columns as chunks.  A CTA sums the rows of its consecutive tiles; what it
 // has at the end of a group goes to its own place in `part` (CTA b and group
 // g: place b + g; both only ever grow), and the places of a group are added
-// in order by another kernel, so the sums have a fixed order.
+// in order by another kernel, so the sums have a fixed order.  So does what it
+// has after every kPiecePanels panels, since the tensor core cuts sums to fp32:
+// 600 k rows 200-130 of one sign were 5e-5 low without that.
+constexpr int kPiecePanels = 8;
+
 template <typename T, int ACT, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 2)
     weights_mma_kernel(WeightArgs p, int columns) {
@@ -967,6 +989,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   if (cur.n > 0) load_run(cur, 0);
   int pending = 0;              // panels in the accumulators
+  bool first = true;            // none of the group have left them yet
 
   for (int k = 0; cur.n > 0; ++k) {
     if (pending > 0) wait_mma();  // the panels' memory is free again
@@ -1025,7 +1048,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       after = next_run(nxt);
       if (tid < DP) next_id = id_of(after, tid);
     }
-    if (nxt.n == 0 || nxt.g != cur.g) {  // the group ends here: its sums to their place
+    const bool last = nxt.n == 0 || nxt.g != cur.g;  // of the group
+    if (last || pending == kPiecePanels) {  // the sums to their place
       wait_mma();
       float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)p.s.M * (p.s.K + 1));
       const int kk = (warp & 3) * 32 + lane;
@@ -1039,12 +1063,9 @@ __global__ void __launch_bounds__(kThreads, 2)
           tc::load16(from + NT, u);
           join_parts<T>(v, u);
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int m = (warp >> 2) * HALF + c + i;
-          if (kk < kn && m < mn)
-            to[(int64_t)(m0 + m) * p.s.K + k0 + kk] = v[i];
-        }
+        const int m = (warp >> 2) * HALF + c;
+        if (kk < kn)
+          add_piece(to + (int64_t)(m0 + m) * p.s.K + k0 + kk, p.s.K, mn - m, v, first);
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -1052,10 +1073,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
         if (has_v && p.biases && k0 == 0 && (tid & 7) == 0 && vc + e < mn)
-          to[(int64_t)p.s.M * p.s.K + m0 + vc + e] = b;
+          add_to(to + (int64_t)p.s.M * p.s.K + m0 + vc + e, b, first);
         bsum[e] = 0.0f;
       }
       pending = 0;
+      first = last;
       tc::fence_before_sync();
       __syncthreads();
     }
@@ -1497,20 +1519,6 @@ __global__ void __launch_bounds__(kCta, 1)
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 0) tc::dealloc(tmem, 4 * NT);
-}
-
-// A lane's 16 sums of an accumulator (`there` of them are wanted) to its column of
-// the CTA's place, `pitch` floats apart: the first piece of a group is
-// written, the others are added without waiting for what is there.  No other
-// thread has these sums, so the order of the additions is the pieces'.
-__device__ __forceinline__ void add_piece(float* at, int pitch, int there, const float (&v)[16],
-                                          bool first) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if (i >= there) break;
-    if (first) at[(int64_t)i * pitch] = v[i];
-    else atomicAdd(at + (int64_t)i * pitch, v[i]);
-  }
 }
 
 // ------------------------------------------------- the whole backward, 16 bits

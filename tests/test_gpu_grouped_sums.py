@@ -82,6 +82,25 @@ def test_long_group_in_one_pass(gs, cuda, dtype, act):
     _assert_sums(got["v_biases"], b, _bound(0, 1200, TYPES[dtype]) + extra, what="v_biases")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("act", ["none", "sigmoid"])
+@pytest.mark.parametrize("R,K,M", [(600_000, 200, 130), (40_000, 1024, 1024)])
+def test_long_group_of_wide_rows(gs, cuda, dtype, act, R, K, M):
+    """16-bit rows past 128 features: the second shape has four CTAs to a tile
+    of the weights, 10,000 rows each.  An accumulator takes 8 panels of 4 steps,
+    then come up to 20 pieces and 74 places.  v_biases: a thread's rows of a
+    piece, and the same."""
+    from gsplat_core.grouped import grouped_linear_backward
+    edges = [0, 700, R]
+    c, y, v = _positive(R, 2, K, M, TYPES[dtype], 4, top=1 / 16)
+    c["offsets"] = torch.tensor(edges, dtype=torch.int32, device="cuda")
+    got = grouped_linear_backward(c, y, v, activation=act, wanted=("v_weights", "v_biases"))
+    w, b = _weight_sums(c["x"], y, v, act, edges)
+    extra = (3 * 2.0 ** -24 + 2.0 ** (-22 if dtype == "fp16" else -16)) if act == "sigmoid" else 0.0
+    _assert_sums(got["v_weights"], w, _bound(32, 94, TYPES[dtype]) + extra, what="v_weights")
+    _assert_sums(got["v_biases"], b, _bound(0, 300, TYPES[dtype]) + extra, what="v_biases")
+
+
 @pytest.mark.parametrize("gathered", [False, True])
 @pytest.mark.parametrize("K,M,R", [(64, 16, 200_000), (77, 45, 50_000), (200, 136, 50_000), (32, 3, 50_000)])
 @pytest.mark.parametrize("size", ["1e-6", "2^-24", "1"])
@@ -114,7 +133,7 @@ def test_small_gradients_of_fp16_behind_a_sigmoid(gs, cuda, gathered, K, M, R, s
         for s, g in ((slice(0, 900), 0), (slice(900, R), 1)):
             _assert_sums(x[s], want_x[s], _bound(9, 4, half) + part, low(w[g]), what="v_x")
             if "v_weights" in got:
-                _assert_sums(got["v_weights"][g], want_w[g], _bound(64, 400, half) + part,
+                _assert_sums(got["v_weights"][g], want_w[g], _bound(32, 400, half) + part,
                              low(rows[s]), what="v_weights")
                 _assert_sums(got["v_biases"][g], want_b[g], _bound(0, 400, half) + part,
                              what="v_biases")
