@@ -318,22 +318,46 @@ __device__ __forceinline__ void arrived(int n) {
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
+// Which piece of a depth an accumulator holds.
+enum { kWhole, kFirst, kMiddle, kLast };
+
 // A warp's 32 lanes of an accumulator (columns of its half), 64 bytes of
 // results at a time: through `stage`, the warp's own 2 KB of shared memory, and
 // in pieces of rows to `out_rows`.  into: the row that lane's row is added to
-// (kScatter).  A tile that is not live gives zeros.
+// (kScatter).  A tile that is not live gives zeros.  Of a depth in pieces (fp32)
+// the sums so far wait in the place of the result.
 template <typename T, int ACT, int MODE, int TERMS>
 __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second, int half,
                                              int rows, int cols, const float* my_bias, int into,
                                              char* stage, void* out_rows, int row, int pitch,
-                                             int n0, int wide_out) {
+                                             int n0, int wide_out, int part = kWhole) {
   constexpr bool BACK = MODE != kForward;
   constexpr int OB = MODE == kScatter ? 4 : sizeof(T);  // bytes of a result
   constexpr int OE = 16 / OB, SC = 64 / OB;             // results in 16 and in 64 bytes
+  constexpr bool PIECES = sizeof(T) == 4 && MODE != kScatter;
   const int lane = threadIdx.x & 31;
   auto stage_at = [&](int r, int c) { return stage + r * 64 + ((c ^ ((r >> 1) & 3)) << 4); };
   for (int c0 = half * SC; c0 < cols; c0 += 2 * SC) {
     const int width = min(SC, cols - c0);  // columns here
+    if constexpr (PIECES) {
+      if (part == kMiddle || part == kLast) {  // the sums so far, written with the piece before
+        const float* const from = static_cast<const float*>(out_rows) + (int64_t)row * pitch + n0 + c0;
+        if (wide_out) {
+          const int c = lane & 3;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((lane >> 2) + 8 * i < rows && c * 4 < width)
+              *reinterpret_cast<float4*>(stage_at((lane >> 2) + 8 * i, c)) =
+                  *reinterpret_cast<const float4*>(from + (int64_t)((lane >> 2) + 8 * i) * pitch + c * 4);
+        } else {
+          for (int i = lane; i < rows * width; i += 32) {
+            const int r = i / width, e = i - r * width;
+            reinterpret_cast<float*>(stage_at(r, e / 4))[e % 4] = from[(int64_t)r * pitch + e];
+          }
+        }
+        __syncwarp();
+      }
+    }
 #pragma unroll
     for (int h = 0; h < SC / 16; ++h) {
       if (h * 16 >= width) break;
@@ -346,10 +370,19 @@ __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second
           join_parts<T>(v, u);
         }
       }
+      if constexpr (PIECES) {
+        if (part == kMiddle || part == kLast) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float4 s = *reinterpret_cast<const float4*>(stage_at(lane, h * 4 + k));
+            v[k * 4] += s.x, v[k * 4 + 1] += s.y, v[k * 4 + 2] += s.z, v[k * 4 + 3] += s.w;
+          }
+        }
+      }
       if (!live) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-      } else if (!BACK) {
+      } else if (!BACK && (!PIECES || part == kWhole || part == kLast)) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (ACT == GS_ACT_SIGMOID && h * 16 + k * 4 >= width) break;  // 20 instructions each
@@ -446,6 +479,12 @@ __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second
 // front warps.  (TMA's four-row gathers took 19 cycles a 128-byte row, 49 us
 // where the copies take 40: 316 k rows 64-64 fp32.)
 enum { kTma, kGather, kCopy };
+
+// Panels of fp32 rows that go through one accumulator: 256 features, 32 steps,
+// of which each cuts the sum to fp32 (16384 features of one sign were 1.2e-4 low in
+// one).  16-bit rows keep one: the 1024 steps of 16384 features lose 1e-4 of a sum
+// of one sign, a fifth of fp16's own rounding.
+constexpr int kPieceDepth = 8;
 constexpr int kLoaders = 64;                          // threads of the gathering warps
 constexpr int kCta = 2 * kThreads + 64 + kLoaders;    // front, back, MMA, TMA, gathers
 
@@ -458,6 +497,7 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
   constexpr int DP = 128 / sizeof(T);   // depth of a panel
   constexpr int STEP = 32 / sizeof(T);  // depth of an MMA
   constexpr bool BACK = MODE != kForward;
+  constexpr bool kPieces = sizeof(T) == 4;
   extern __shared__ char smem_raw[];
   __shared__ uint64_t s_bars[3 * kSlotsMost + 5];
   __shared__ uint32_t s_tmem;
@@ -593,12 +633,13 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
     Ring ring(p.slots);
     int stagings = 0, q = 0, t = 0;
     for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
-    for (int row = 0; row < cur.n; row += kTile, ++t) {
+    for (int row = 0; row < cur.n; row += kTile, t += kPieces ? 0 : 1) {
+      int held = 0;  // panels in the accumulator
       for (int j = 0; j < p.panels; ++j, ++q, ring.next()) {
         const int slot = ring.slot;
         if (row + j == 0 || !p.resident) wait(weighed, stagings++);
         wait(kWork ? ready(slot) : full(slot), ring.turn);
-        if (j == 0 && t > 1) wait(taken(t & 1), (t >> 1) - 1);
+        if ((kPieces ? held : j) == 0 && t > 1) wait(taken(t & 1), (t >> 1) - 1);
         tc::fence_after_sync();
         const int steps = steps_of(j);
         const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms;
@@ -612,7 +653,7 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
         for (int i = 0; i < 4; ++i) {
           if (i >= steps) break;
           const uint64_t step = 2 * i;  // 32 bytes
-          const bool more = j > 0 || i > 0;
+          const bool more = (kPieces ? held : j) > 0 || i > 0;
           if (L::kTerms == 2) {
             tc::mma<Mma<T>::TF32>(leader, acc + p.nt, dl + step, dw + step, idesc, more);
             if (L::kWTerms == 2) {
@@ -623,7 +664,13 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
           tc::mma<Mma<T>::TF32>(leader, acc, da + step, dw + step, idesc, more);
         }
         tc::commit(leader, free_(slot));
-        if (j + 1 == p.panels) tc::commit(leader, made(t & 1));
+        if constexpr (!kPieces) {
+          if (j + 1 == p.panels) tc::commit(leader, made(t & 1));
+        } else if (++held == kPieceDepth || j + 1 == p.panels) {
+          tc::commit(leader, made(t & 1));
+          ++t;
+          held = 0;
+        }
       }
     }
     // every MMA is done before the memory goes
@@ -810,28 +857,36 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
       const int rows = min(32, cur.row + cur.n - row - row0);
       int32_t into = -1;  // where lane's row is added up
       if (MODE == kScatter && live && lane < rows) into = __ldg(p.ids + row + row0 + lane);
-      const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms + ((uint32_t)row0 << 16);
-      if (live) {
-        if (!BACK && cur.g != biased) {
-          __syncwarp();
-          for (int i = lane; i < p.nt; i += 32)
-            my_bias[i] = bias && i < cols ? to_f(bias[(int64_t)cur.g * p.s.M + n0 + i]) : 0.0f;
-          __syncwarp();
-          biased = cur.g;
-        }
-        wait(made(t & 1), t >> 1);
-        tc::fence_after_sync();
-      }
-      if (into >= p.s.n) into = -1;
-      take_results<T, ACT, MODE, L::kTerms>(live, acc, p.nt, bw >> 2, rows, cols, my_bias, into,
-                                            s_stage + bw * 2048, p.out,
-                                            MODE == kScatter ? 0 : row + row0, p.width,
-                                            n0, p.wide_out);
-      if (live) {
-        tc::fence_before_sync();
+      if (live && !BACK && cur.g != biased) {
         __syncwarp();
-        if (lane == 0) tc::arrive(taken(t & 1));
-        ++t;
+        for (int i = lane; i < p.nt; i += 32)
+          my_bias[i] = bias && i < cols ? to_f(bias[(int64_t)cur.g * p.s.M + n0 + i]) : 0.0f;
+        __syncwarp();
+        biased = cur.g;
+      }
+      auto take = [&](int part) {
+        const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms + ((uint32_t)row0 << 16);
+        if (live) {
+          wait(made(t & 1), t >> 1);
+          tc::fence_after_sync();
+        }
+        if (into >= p.s.n) into = -1;
+        take_results<T, ACT, MODE, L::kTerms>(live, acc, p.nt, bw >> 2, rows, cols, my_bias, into,
+                                              s_stage + bw * 2048, p.out,
+                                              MODE == kScatter ? 0 : row + row0, p.width,
+                                              n0, p.wide_out, part);
+        if (live) {
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::arrive(taken(t & 1));
+          ++t;
+        }
+      };
+      if (kPieces && live && p.panels > kPieceDepth) {
+        for (int left = p.panels; left > 0; left -= kPieceDepth)
+          take(left == p.panels ? kFirst : left > kPieceDepth ? kMiddle : kLast);
+      } else {
+        take(kWhole);
       }
     }
   }

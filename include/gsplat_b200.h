@@ -689,7 +689,10 @@ typedef struct {
  * offsets[g + 1]: x [n,K], weights [G,M,K], biases [G,M] or NULL, offsets
  * [G+1] int32 ascending, row_ids [R] int32 (with use_row_ids), y [R,M].
  * Sums are in fp32 and rounded once; fp32 factors are carried to 2^-22 of
- * themselves (and to 2^-126).  Rows outside every group are written
+ * themselves (and to 2^-126).  The tensor core cuts sums instead of rounding
+ * them, so that one of equal signs comes out low, by 3e-6 of itself at most; in
+ * the 16-bit y and v_x, which are summed in one go, by 1e-7 for each 16 features
+ * where that is more.  Rows outside every group are written
  * as zeros; an id outside [0, n) reads a row of zeros.  Offsets that do not
  * ascend give unspecified values and no access out of bounds. */
 int gs_grouped_linear_fwd(const gs_grouped_params* p, const void* x,

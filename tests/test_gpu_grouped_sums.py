@@ -102,6 +102,48 @@ def test_long_group_of_wide_rows(gs, cuda, dtype, act, R, K, M):
 
 
 @pytest.mark.parametrize("gathered", [False, True])
+@pytest.mark.parametrize("K,M,act", [(16384, 40, "none"), (6001, 70, "sigmoid"), (2048, 128, "relu"),
+                                     (777, 33, "none")])
+def test_deep_rows_fp32(gs, cuda, gathered, K, M, act):
+    """Forward and v_x through many features: an accumulator takes 8 panels of
+    4 additions, and up to 64 pieces are added up in fp32."""
+    from gsplat_core.grouped import grouped_linear_backward, grouped_linear_forward
+    R, edges = 300, [0, 130, 131, 131, 300]
+    spans = list(zip(edges, edges[1:]))
+    c, _, _ = _positive(R, 4, K, M, torch.float32, 6)
+    if act == "sigmoid":  # z of order one, so that y says something of it
+        c["weights"] /= K / 4
+    c["offsets"] = torch.tensor(edges, dtype=torch.int32, device="cuda")
+    ids = torch.randperm(R, generator=torch.Generator().manual_seed(1)).cuda()
+    rows = c["x"].double()
+    if gathered:
+        c["row_ids"] = ids.to(torch.int32)
+        rows = rows[ids]
+    z = torch.cat([rows[a:b] @ c["weights"][g].double().T + c["biases"][g].double()
+                   for g, (a, b) in enumerate(spans)])
+    y = grouped_linear_forward(c, activation=act)
+    bound = _bound(32, 64, torch.float32)
+    if act == "sigmoid":  # dy = y (1 - y) dz, and eight units of its own
+        want = torch.sigmoid(z)
+        off = bound * z * want * (1 - want) + 8 * 2.0 ** -24 * want
+        assert bool(((y.double() - want).abs() <= off).all())
+    else:
+        _assert_sums(y, z, bound, what="y")
+    # v_x: the same with M and K in each other's place
+    c, _, v = _positive(R, 4, M, K, torch.float32, 7)
+    c["offsets"] = torch.tensor(edges, dtype=torch.int32, device="cuda")
+    if gathered:
+        c["row_ids"] = ids.to(torch.int32)
+    y = torch.full_like(v, 0.25)
+    vz = {"none": 1.0, "relu": 1.0, "sigmoid": 0.1875}[act] * v.double()
+    want = torch.cat([vz[a:b] @ c["weights"][g].double() for g, (a, b) in enumerate(spans)])
+    got = grouped_linear_backward(c, y, v, activation=act, wanted=("v_x",))["v_x"]
+    if gathered:
+        got = got[ids]
+    _assert_sums(got, want, bound + (3 * 2.0 ** -24 if act == "sigmoid" else 0.0), what="v_x")
+
+
+@pytest.mark.parametrize("gathered", [False, True])
 @pytest.mark.parametrize("K,M,R", [(64, 16, 200_000), (77, 45, 50_000), (200, 136, 50_000), (32, 3, 50_000)])
 @pytest.mark.parametrize("size", ["1e-6", "2^-24", "1"])
 def test_small_gradients_of_fp16_behind_a_sigmoid(gs, cuda, gathered, K, M, R, size):
