@@ -101,6 +101,24 @@ def test_long_group_of_wide_rows(gs, cuda, dtype, act, R, K, M):
     _assert_sums(got["v_biases"], b, _bound(0, 300, TYPES[dtype]) + extra, what="v_biases")
 
 
+@pytest.mark.parametrize("act", ["none", "sigmoid"])
+@pytest.mark.parametrize("K,M", [(64, 64), (64, 100), (32, 3)])
+def test_long_group_fp32(gs, cuda, act, K, M):
+    """An accumulator takes 4 panels of 4 steps, registers then 43 of them, then
+    come 148 places (few outputs have no accumulator: a lane's 10 runs of 4
+    rows up to 32 lanes, 8 warps and 296 places).  Kept in one accumulator a
+    CTA's 675 steps would lose 2.3e-5, six times what is allowed here."""
+    from gsplat_core.grouped import grouped_linear_backward
+    R, edges = 800_000, [0, 700, 800_000]
+    c, y, v = _positive(R, 2, K, M, torch.float32, 5)
+    c["offsets"] = torch.tensor(edges, dtype=torch.int32, device="cuda")
+    got = grouped_linear_backward(c, y, v, activation=act, wanted=("v_weights", "v_biases"))
+    w, b = _weight_sums(c["x"], y, v, act, edges)
+    extra = 3 * 2.0 ** -24 if act == "sigmoid" else 0.0
+    _assert_sums(got["v_weights"], w, _bound(16, 400, torch.float32) + extra, what="v_weights")
+    _assert_sums(got["v_biases"], b, _bound(0, 400, torch.float32) + extra, what="v_biases")
+
+
 @pytest.mark.parametrize("gathered", [False, True])
 @pytest.mark.parametrize("K,M,act", [(16384, 40, "none"), (6001, 70, "sigmoid"), (2048, 128, "relu"),
                                      (777, 33, "none")])
