@@ -42,16 +42,16 @@ struct Shape {
 __device__ __forceinline__ int group_of(const int32_t* __restrict__ off, int G, int r) {
   const int lane = threadIdx.x & 31;
   const int first = __ldg(off), last = __ldg(off + G);
-  int lo = 0, hi = G;  // off[lo] <= r < off[hi]
+  uint32_t lo = 0, hi = G;  // off[lo] <= r < off[hi]
   while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const uint32_t step = (hi - lo + 31) / 32, at = lo + lane * step;  // up to 2^31 + 30
     const uint32_t below = __ballot_sync(0xffffffffu, at < hi && __ldg(off + at) <= r);
     // the places where the row is above one and below the next
     const int i = below == 0xffffffffu ? 31 : max(__ffs(~below) - 2, 0);
     lo += i * step;
     hi = min(hi, lo + step);
   }
-  return r < first ? -1 : r >= last ? G : lo;
+  return r < first ? -1 : r >= last ? G : (int)lo;
 }
 
 template <int ACT>
@@ -1975,14 +1975,14 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int kp, int mp, int 
   const int64_t in_place = i >= mk ? sums + (i - mk) : kp == s.K ? i : i / s.K * kp + i % s.K;
   const int64_t tiles = (s.R + kTile - 1) / kTile;
   auto part_of = [&](int64_t r) { return (int)(((r / kTile + 1) * parts - 1) / tiles); };
-  for (int g = blockIdx.y; g < s.G; g += gridDim.y) {
+  for (int64_t g = blockIdx.y; g < s.G; g += gridDim.y) {
     const int64_t r0 = max((int64_t)__ldg(off + g), (int64_t)0);
     const int64_t r1 = min((int64_t)__ldg(off + g + 1), s.R);
     float sum = 0.0f;
     if (r0 < r1 && i < each) {
       const int b0 = part_of(r0), n = part_of(r1 - 1) - b0 + 1;
       const int from = n * share / SHARES, to = n * (share + 1) / SHARES;
-      const float* p = part + (int64_t)(b0 + g + from) * place + in_place;
+      const float* p = part + (b0 + g + from) * place + in_place;
       if (i < mk) {
 #pragma unroll 8
         for (int b = from; b < to; ++b, p += place) sum += __ldg(p);
@@ -2002,7 +2002,7 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int kp, int mp, int 
       if (i < mk) {
         if (vw) vw[g * mk + i] = from_f<T>(sum);
       } else if (vb) {
-        vb[(int64_t)g * s.M + (i - mk)] = from_f<T>(sum);
+        vb[g * s.M + (i - mk)] = from_f<T>(sum);
       }
     }
   }
@@ -2315,7 +2315,8 @@ __global__ void __launch_bounds__(256) round_kernel(int64_t n, const float* __re
 
 __global__ void __launch_bounds__(256) offsets_kernel(int64_t n, const int32_t* __restrict__ ids,
                                                       int G, int32_t* __restrict__ off) {
-  for (int g = blockIdx.x * blockDim.x + threadIdx.x; g <= G; g += gridDim.x * blockDim.x) {
+  for (int64_t g = blockIdx.x * blockDim.x + threadIdx.x; g <= G;
+       g += gridDim.x * blockDim.x) {  // past 2^31 where G is next to it
     int64_t lo = 0, hi = n;  // ids below g end in [lo, hi]
     while (lo < hi) {
       const int64_t mid = (lo + hi) >> 1;
@@ -2757,6 +2758,7 @@ int bad_params(const gs_grouped_params* p) {
   if (!p || p->rows < 0 || p->n < 0 || p->groups < 1 || p->in_features < 1 ||
       p->out_features < 1)
     return invalid("grouped_linear: bad params");
+  if (p->groups == INT32_MAX) return invalid("grouped_linear: 2^31 - 1 groups or more");
   if (p->rows > kRowsMost || p->n > kRowsMost)
     return invalid("grouped_linear: 2^31 - 4096 rows or more");
   if (!p->use_row_ids && p->n != p->rows)

@@ -25,6 +25,7 @@ from ._lib import GroupedParams, on_device_of
 from ._lib import check as check_status
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_GROUPS_MOST = 2 ** 31 - 2
 _ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2}
 
 
@@ -40,6 +41,8 @@ def group_offsets(ids, groups):
         raise RuntimeError("group_offsets: ids must be a 1-D int32 tensor.")
     if int(groups) < 0:
         raise RuntimeError("group_offsets: negative number of groups.")
+    if int(groups) > _GROUPS_MOST:
+        raise RuntimeError("group_offsets: 2^31 - 1 groups or more.")
     if not ids.is_cuda:
         raise RuntimeError("group_offsets: ids must be a CUDA tensor (there is no CPU fallback).")
     ids = ids.contiguous()
@@ -68,6 +71,8 @@ def _validated(inputs, activation):
     G, M, _ = w.shape
     if min(G, M, K) < 1 or max(M, K) > 16384:
         raise RuntimeError("grouped_linear: G, M and K must be at least 1, M and K at most 16384.")
+    if G > _GROUPS_MOST:
+        raise RuntimeError("grouped_linear: 2^31 - 1 groups or more.")
     if off.shape != (G + 1,) or off.dtype != torch.int32:
         raise RuntimeError("grouped_linear: offsets must have shape [G + 1] and type int32.")
     if b is not None and (b.shape != (G, M) or b.dtype != dtype):

@@ -677,7 +677,7 @@ enum gs_activation { GS_ACT_NONE = 0, GS_ACT_RELU = 1, GS_ACT_SIGMOID = 2 };
 typedef struct {
   int64_t rows;         /* R, below 2^31 - 4096                             */
   int64_t n;            /* rows of x: R without row_ids; below 2^31 - 4096  */
-  int32_t groups;       /* G                                                */
+  int32_t groups;       /* G, below 2^31 - 1                                */
   int32_t in_features;  /* K, up to 16384                                   */
   int32_t out_features; /* M, up to 16384                                   */
   int32_t dtype;        /* gs_dtype of x, weights, biases, y and gradients  */
