@@ -14,6 +14,8 @@
 #include <cuda_fp16.h>
 
 #include <climits>
+#include <cstring>
+#include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
@@ -87,8 +89,43 @@ __device__ __forceinline__ float through(float v, float y) {
 // mean over an image, so its second part is held times 2^11 (it is at most 2^4:
 // half a step of the first) and what it gives is scaled back where the sums are
 // joined: v_z is carried to 2^-22 of itself and to 2^-36.  bf16 has fp32's range.
-__device__ unsigned int g_wait_gave_up;
-constexpr uint32_t kWaitLimit = 1u << 16;  // polls of the hardware's own bounded wait
+//
+// Waits are for the CTA's own copies, MMAs and warps, and are bounded.  A warp
+// whose wait gives up says so in *status and to the CTA's other warps, which
+// then give up their next wait that does not end at once.  From then on it sends
+// no copies, issues no MMAs and arrives nowhere, so that no barrier moves on by
+// what was not done: it leaves its loops, or walks on to the named barriers at
+// which other warps meet it.  Whoever sent bulk copies or MMAs waits for those
+// (with a limit of its own) before the CTA gives its memory back.  The results
+// are void.
+constexpr uint32_t kWaitLimit = 1u << 16;   // polls of 20 us: a second or more
+constexpr uint32_t kDrainLimit = 1u << 12;  // for what takes microseconds
+
+struct WaitArgs {
+  uint32_t limit;
+  uint32_t* status;
+};
+
+// False for the whole warp where the wait gave up.
+__device__ __forceinline__ bool waited(uint32_t bar, uint32_t parity, const WaitArgs& p,
+                                       uint32_t* stop) {
+  if (tc::bar_wait(bar, parity & 1, p.limit, stop)) return true;
+  *static_cast<volatile uint32_t*>(stop) = 1;
+  *static_cast<volatile uint32_t*>(p.status) = 1;
+  return false;
+}
+// A wait of a role that leaves its loops where one gives up.
+#define WAIT_OR(done, bar, parity) \
+  if (!waited(bar, parity, p.waits, &s_stop)) goto done
+
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
+  tc::bar_wait(bar, parity & 1, kDrainLimit, nullptr);
+}
+// The last of `sent` copies into a ring of slots, those that may be under way.
+template <typename Full>
+__device__ __forceinline__ void drain_ring(int sent, int slots, Full full) {
+  for (int i = max(sent - slots, 0); i < sent; ++i) drain(full(i % slots), i / slots);
+}
 
 template <typename T> struct Mma;
 template <> struct Mma<float> {
@@ -240,6 +277,7 @@ struct RowsArgs {
   int resident;            // all weight panels of the tile stay in shared memory
   int slots;               // panels of rows that are in flight or in use
   int wide_w, wide_out;    // 16-byte accesses are aligned
+  WaitArgs waits;
 };
 
 enum { kForward, kBackward, kScatter };
@@ -499,8 +537,8 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
   constexpr bool BACK = MODE != kForward;
   constexpr bool kPieces = sizeof(T) == 4;
   extern __shared__ char smem_raw[];
-  __shared__ uint64_t s_bars[3 * kSlotsMost + 5];
-  __shared__ uint32_t s_tmem;
+  __shared__ uint64_t s_bars[3 * kSlotsMost + 6];
+  __shared__ uint32_t s_tmem, s_stop;
   __shared__ __align__(16) float s_bias[8][kTile];
   char* const s_low = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
   char* const s_stage = s_low + L::kLow;
@@ -514,6 +552,7 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
   auto made = [&](int i) { return bar0 + 8 * (3 * kSlotsMost + i); };    // an accumulator is
   auto taken = [&](int i) { return bar0 + 8 * (3 * kSlotsMost + 2 + i); };
   const uint32_t weighed = bar0 + 8 * (3 * kSlotsMost + 4);              // the weights are there
+  const uint32_t drained = bar0 + 8 * (3 * kSlotsMost + 5);              // all MMAs are done
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be uniform
   const int n0 = blockIdx.y * p.nt;
@@ -528,6 +567,8 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
       tc::bar_init(ready(i), 8);
     }
     tc::bar_init(weighed, 8);
+    tc::bar_init(drained, 1);
+    s_stop = 0;
     for (int i = 0; i < 2; ++i) {
       tc::bar_init(made(i), 1);
       tc::bar_init(taken(i), 8);
@@ -538,12 +579,9 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
-  uint32_t limit = kWaitLimit;
+  bool alive = true;  // no wait of this warp gave up
   auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (!tc::bar_wait(bar, parity & 1, limit)) {
-      limit = 0;  // results are void: no later wait holds the kernel up
-      g_wait_gave_up = 1;
-    }
+    alive = alive && waited(bar, parity, p.waits, &s_stop);
   };
 
   const int64_t tiles = (p.s.R + kTile - 1) / kTile;
@@ -566,11 +604,12 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
     // ------------------------------------------------------------- TMA
     if (LOAD == kTma) {
       Ring ring(p.slots);
+      int sent = 0;
       for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
         for (int i = 0; i < cur.n; i += kTile)
           for (int j = 0; j < p.panels; ++j, ring.next()) {
             const int slot = ring.slot;
-            if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+            if (ring.turn > 0) WAIT_OR(sent_all, free_(slot), ring.turn - 1);
             if (tc::elected()) {
               const uint32_t to = tc::smem_addr(s_rows + slot * kPanel);
               tc::expect(full(slot), kPanel * (L::kY ? 2 : 1));
@@ -579,7 +618,10 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
                 tc::load_box(to + p.slots * kPanel, &map_y, j * DP, cur.row + i, full(slot));
             }
             __syncwarp();
+            ++sent;
           }
+    sent_all:
+      drain_ring(sent, p.slots, full);
     }
   } else if (warp >= 18) {
     // ------------------------------------------------------------- gathers
@@ -589,7 +631,7 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
       constexpr int N = kTile / 8;  // rows of a thread: r8 + 8 i
       Ring ring(p.slots);
       Run ahead = after_live(none);
-      int ahead_row = 0, id[N];
+      int ahead_row = 0, sent = 0, id[N];
       auto read_ids = [&]() {  // no use yet of what is read
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -611,7 +653,7 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
         read_ids();  // of the next tile
         for (int j = 0; j < p.panels; ++j, ring.next()) {
           const int slot = ring.slot, d = j * DP + c16 * E;
-          if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+          if (ring.turn > 0) WAIT_OR(gathered, free_(slot), ring.turn - 1);
           if (c16 < 2 * steps_of(j)) {
             char* const to = s_rows + slot * kPanel + chunk_at(r8, c16);  // r & 7 is r8
             const T* const ad = d < p.depth ? a + d : a;
@@ -622,9 +664,12 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
             }
           }
           tc::arrive_copied(full(slot));
+          ++sent;
         }
       }
+    gathered:
       arrived(0);
+      drain_ring(sent, p.slots, full);
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
@@ -637,9 +682,9 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
       int held = 0;  // panels in the accumulator
       for (int j = 0; j < p.panels; ++j, ++q, ring.next()) {
         const int slot = ring.slot;
-        if (row + j == 0 || !p.resident) wait(weighed, stagings++);
-        wait(kWork ? ready(slot) : full(slot), ring.turn);
-        if ((kPieces ? held : j) == 0 && t > 1) wait(taken(t & 1), (t >> 1) - 1);
+        if (row + j == 0 || !p.resident) WAIT_OR(mma_done, weighed, stagings++);
+        WAIT_OR(mma_done, kWork ? ready(slot) : full(slot), ring.turn);
+        if ((kPieces ? held : j) == 0 && t > 1) WAIT_OR(mma_done, taken(t & 1), (t >> 1) - 1);
         tc::fence_after_sync();
         const int steps = steps_of(j);
         const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms;
@@ -674,7 +719,9 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
       }
     }
     // every MMA is done before the memory goes
-    if (q > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
+  mma_done:
+    tc::commit(leader, drained);
+    drain(drained, 0);
   } else if (warp < 8) {
     // ------------------------------------------------------------ front warps
     const int tid = threadIdx.x;
@@ -789,7 +836,7 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
     for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur)) {
       if (p.resident) {
         // every MMA of the group before is done
-        if (q > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
+        if (q > 0) WAIT_OR(fronted, free_(ring.slot_before(1)), ring.turn_before(1));
         stage_weights(cur.g, 0, p.panels);
         tc::fence_smem();
         __syncwarp();
@@ -799,7 +846,7 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
       for (int j = 0; j < p.panels; ++j, ++q, ring.next()) {
         const int slot = ring.slot;
         if (!p.resident) {
-          if (q > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
+          if (q > 0) WAIT_OR(fronted, free_(ring.slot_before(1)), ring.turn_before(1));
           stage_weights(cur.g, j, j + 1);
           tc::fence_smem();
           __syncwarp();
@@ -807,12 +854,12 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
         }
         if (kWork) {
           // the panel `lag` before is done with: its slot, and its low parts
-          if (q >= lag) wait(free_(ring.slot_before(lag)), ring.turn_before(lag));
+          if (q >= lag) WAIT_OR(fronted, free_(ring.slot_before(lag)), ring.turn_before(lag));
           if (LOAD == kCopy) {
             send();
             arrived(p.slots - lag);
           } else {
-            wait(full(slot), ring.turn);
+            WAIT_OR(fronted, full(slot), ring.turn);
           }
           if ((L::kTerms == 2 || L::kY) && c16 < 2 * steps_of(j)) {
             char* const here = s_rows + slot * kPanel;
@@ -840,10 +887,11 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
         } else {
           // keeps pace: a barrier says whether its last phase is over, not
           // which one that is
-          wait(free_(slot), ring.turn);
+          WAIT_OR(fronted, free_(slot), ring.turn);
         }
       }
     }
+  fronted:
     if (LOAD == kCopy) arrived(0);
   } else {
     // ------------------------------------------------------------- back warps
@@ -868,6 +916,7 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
         const uint32_t acc = tmem + (t & 1) * p.nt * L::kTerms + ((uint32_t)row0 << 16);
         if (live) {
           wait(made(t & 1), t >> 1);
+          if (!alive) return;
           tc::fence_after_sync();
         }
         if (into >= p.s.n) into = -1;
@@ -907,6 +956,7 @@ struct WeightArgs {
   int kt, mt;        // tiles of K (128) and M (NT)
   int wide_x, wide_y;
   int biases;
+  WaitArgs waits;
 };
 
 // The first piece of a sum is written, the others are added without waiting
@@ -950,8 +1000,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   constexpr int VTERMS = SPLIT ? 2 : 1;
   constexpr int VPANEL = NT * 128;
   extern __shared__ char smem_raw[];
-  __shared__ uint64_t s_bar;
-  __shared__ uint32_t s_tmem;
+  __shared__ uint64_t s_bars[2];
+  __shared__ uint32_t s_tmem, s_stop;
   __shared__ int32_t s_ids[4][DP];
   char* const s_x = smem_raw + (1024 - (tc::smem_addr(smem_raw) & 1023)) % 1024;
   char* const s_v = s_x + kPanel;
@@ -965,20 +1015,20 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 0) tc::alloc(&s_tmem, columns);
   if (tid == 0) {
-    tc::bar_init(tc::smem_addr(&s_bar), 1);
+    tc::bar_init(tc::smem_addr(s_bars), 1);
+    tc::bar_init(tc::smem_addr(s_bars + 1), 1);
+    s_stop = 0;
     tc::bar_init_done();
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = s_tmem, bar = tc::smem_addr(&s_bar);
+  const uint32_t tmem = s_tmem, bar = tc::smem_addr(s_bars), drained = bar + 8;
   const uint32_t idesc = tc::instr_desc(Mma<T>::format, (mn + 15) / 16 * 16);
-  uint32_t phase = 0, limit = kWaitLimit;
+  uint32_t phase = 0;
+  bool alive = true;  // no wait of this warp gave up
   auto wait_mma = [&]() {
-    if (!tc::bar_wait(bar, phase, limit)) {
-      limit = 0;
-      g_wait_gave_up = 1;
-    }
+    alive = alive && waited(bar, phase, p.waits, &s_stop);
     phase ^= 1;
     tc::fence_after_sync();
   };
@@ -1082,7 +1132,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     __syncthreads();
     if (warp == 0) {
       tc::fence_after_sync();
-      const uint32_t leader = tc::elected();
+      const uint32_t elect = tc::elected(), leader = alive ? elect : 0;
       const uint64_t dx = tc::smem_desc(tc::smem_addr(s_x)), dv = tc::smem_desc(tc::smem_addr(s_v));
       const int steps = (cur.n + STEP - 1) / STEP;
 #pragma unroll
@@ -1139,7 +1189,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     cur = nxt;
     nxt = after;
   }
-  if (warp == 0) tc::dealloc(tmem, columns);
+  if (warp == 0) {
+    tc::commit(tc::elected(), drained);
+    drain(drained, 0);
+    tc::dealloc(tmem, columns);
+  }
 }
 
 // v_W and v_b of fp32 rows.
@@ -1165,6 +1219,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 constexpr int kFlush = 4;
 constexpr int kRows32 = 32;
 constexpr int kBox = kRows32 * 128;
+constexpr int kBars32 = 29;
 constexpr int kBiasCopies32 = 4;  // partial sums of v_b: front groups x halves
 
 struct Weight32Args {
@@ -1181,6 +1236,7 @@ struct Weight32Args {
   int sets;            // of operands: 2 or 4
   int x_mode, v_mode;  // 0: TMA, 1: gathered, 2: the front's copies of 4 bytes
   int biases;
+  WaitArgs waits;
 };
 
 template <int ACT, int NT>
@@ -1203,7 +1259,8 @@ __global__ void __launch_bounds__(kCta, 1)
   char* const s_sets = smem_raw;
   char* const s_slots = s_sets + p.sets * set_bytes;
   uint64_t* const s_bars = reinterpret_cast<uint64_t*>(s_slots + p.slots * slot_bytes);
-  uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + 28);
+  uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + kBars32);
+  uint32_t& s_stop = (&s_tmem)[1];
   const uint32_t bar0 = tc::smem_addr(s_bars);
   auto full = [&](int i) { return bar0 + 8 * i; };          // TMA's boxes are there
   auto free_ = [&](int i) { return bar0 + 8 * (8 + i); };   // and have been read
@@ -1211,6 +1268,7 @@ __global__ void __launch_bounds__(kCta, 1)
   auto spent = [&](int i) { return bar0 + 8 * (20 + i); };
   auto made = [&](int i) { return bar0 + 8 * (24 + i); };   // accumulators
   auto taken = [&](int i) { return bar0 + 8 * (26 + i); };
+  const uint32_t drained = bar0 + 8 * 28;
   const int log_sets = p.sets == 4 ? 2 : 1;
   const int tma_boxes = (p.x_mode == 0 ? p.kx : 0) + (p.v_mode == 0 ? p.mx * (HAS_Y ? 2 : 1) : 0);
   const bool sent = tma_boxes > 0 || p.x_mode == 1;  // by other than the front warps
@@ -1228,18 +1286,17 @@ __global__ void __launch_bounds__(kCta, 1)
       tc::bar_init(made(i), 1);
       tc::bar_init(taken(i), 8);
     }
+    tc::bar_init(drained, 1);
+    s_stop = 0;
     tc::bar_init_done();
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem;
-  uint32_t limit = kWaitLimit;
+  bool alive = true;  // no wait of this warp gave up
   auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (!tc::bar_wait(bar, parity & 1, limit)) {
-      limit = 0;
-      g_wait_gave_up = 1;
-    }
+    alive = alive && waited(bar, parity, p.waits, &s_stop);
   };
 
   const int64_t tiles = (p.s.R + kTile - 1) / kTile;
@@ -1260,10 +1317,11 @@ __global__ void __launch_bounds__(kCta, 1)
     // ------------------------------------------------------------- TMA
     if (tma_boxes > 0) {
       Ring ring(p.slots);
+      int panels = 0;
       for (Run cur = after(none); cur.n > 0; cur = after(cur))
         for (int row = cur.row; row < cur.row + cur.n; row += kRows32, ring.next()) {
           const int slot = ring.slot;
-          if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+          if (ring.turn > 0) WAIT_OR(sent_all, free_(slot), ring.turn - 1);
           if (tc::elected()) {
             const uint32_t to = tc::smem_addr(s_slots + slot * slot_bytes);
             tc::expect(full(slot), tma_boxes * kBox);
@@ -1278,7 +1336,10 @@ __global__ void __launch_bounds__(kCta, 1)
               }
           }
           __syncwarp();
+          ++panels;
         }
+    sent_all:
+      drain_ring(panels, p.slots, full);
     }
   } else if (warp >= 18) {
     // ------------------------------------------------------------- gathers
@@ -1286,7 +1347,7 @@ __global__ void __launch_bounds__(kCta, 1)
       const int lt = threadIdx.x - (kCta - kLoaders), c16 = lt & 7, r8 = lt >> 3;
       Ring ring(p.slots);
       Run ahead = after(none);
-      int ahead_row = 0, id[2][4];  // rows r8 + 8 i of the next two panels
+      int panels = 0, ahead_row = 0, id[2][4];  // rows r8 + 8 i of the next two panels
       auto read_ids = [&](int (&to)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1312,7 +1373,7 @@ __global__ void __launch_bounds__(kCta, 1)
             id[0][i] = id[1][i];
           }
           read_ids(id[1]);
-          if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+          if (ring.turn > 0) WAIT_OR(gathered, free_(slot), ring.turn - 1);
           char* const to = s_slots + slot * slot_bytes + chunk_at(r8, c16);
           for (int j = 0; j < p.kx; ++j) {
             const int k = j * 32 + c16 * 4;
@@ -1324,8 +1385,11 @@ __global__ void __launch_bounds__(kCta, 1)
             }
           }
           tc::arrive_copied(full(slot));
+          ++panels;
         }
+    gathered:
       arrived(0);
+      drain_ring(panels, p.slots, full);
     }
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
@@ -1335,8 +1399,8 @@ __global__ void __launch_bounds__(kCta, 1)
     for (Run cur = after(none); cur.n > 0; cur = after(cur))
     for (int left = cur.n; left > 0; left -= kRows32, ++q) {
       const int set = q & (p.sets - 1), buf = sums & 1;
-      wait(ready(set), q >> log_sets);
-      if (held == 0 && sums > 1) wait(taken(buf), (sums >> 1) - 1);
+      WAIT_OR(mma_done, ready(set), q >> log_sets);
+      if (held == 0 && sums > 1) WAIT_OR(mma_done, taken(buf), (sums >> 1) - 1);
       tc::fence_after_sync();
       const uint32_t x_at = tc::smem_addr(s_sets + set * set_bytes);
       const uint64_t xh = tc::smem_desc(x_at), xl = tc::smem_desc(x_at + p.kx * kBox);
@@ -1361,7 +1425,9 @@ __global__ void __launch_bounds__(kCta, 1)
         held = 0;
       }
     }
-    if (q > 0) wait(spent((q - 1) & (p.sets - 1)), (q - 1) >> log_sets);
+  mma_done:
+    tc::commit(leader, drained);  // every MMA is done before the memory goes
+    drain(drained, 0);
   } else if (warp < 8) {
     // ------------------------------------------------------------ front warps
     const int fg = warp >> 2, tid = threadIdx.x & 127;
@@ -1436,9 +1502,10 @@ __global__ void __launch_bounds__(kCta, 1)
 #pragma unroll
       for (int j = 0; j < 4; ++j) db[it][j] = 0.0f;
     Ring ring(p.slots);
-    int q = 0;
-    for (Run cur = after(none); cur.n > 0; cur = after(cur)) {
-      for (int left = cur.n; left > 0; left -= kRows32, ++q, ring.next()) {
+    int q = 0, left = 0;
+    Run cur;
+    for (cur = after(none); cur.n > 0; cur = after(cur)) {
+      for (left = cur.n; left > 0; left -= kRows32, ++q, ring.next()) {
         if ((q & 1) != fg) continue;
         const int slot = ring.slot;
         if (copies) {
@@ -1457,8 +1524,8 @@ __global__ void __launch_bounds__(kCta, 1)
         // have been through their slots, so that the slot's barrier is at this
         // panel)
         const int at_set = q & (p.sets - 1);
-        if (q >= p.sets) wait(spent(at_set), (q >> log_sets) - 1);
-        if (sent) wait(full(slot), ring.turn);
+        if (q >= p.sets) WAIT_OR(walk, spent(at_set), (q >> log_sets) - 1);
+        if (sent) WAIT_OR(walk, full(slot), ring.turn);
         const char* const from = s_slots + slot * slot_bytes;
         char* const set = s_sets + at_set * set_bytes;
 #pragma unroll
@@ -1532,6 +1599,14 @@ __global__ void __launch_bounds__(kCta, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) db[it][j] = 0.0f;
     }
+  walk:
+    // behind a wait that gave up: the group's other warps still meet this one
+    while (copies && cur.n > 0) {
+      left -= kRows32, ++q;
+      if (left <= 0) cur = after(cur), left = cur.n;
+      if (cur.n > 0 && (q & 1) == fg)
+        for (int i = own > 1 ? 1 : 0; i < 2; ++i) tc::bar_sync(1 + fg, 128);
+    }
     if (copies) arrived(0);
   } else {
     // ------------------------------------------------------------- back warps
@@ -1544,7 +1619,7 @@ __global__ void __launch_bounds__(kCta, 1)
     for (Run cur = after(none); cur.n > 0; cur = after(cur))
       for (int left = cur.n; left > 0; left -= kFlush * kRows32) {
         const int buf = sums & 1;
-        wait(made(buf), sums >> 1);
+        WAIT_OR(taken_all, made(buf), sums >> 1);
         tc::fence_after_sync();
 #pragma unroll
         for (int c = 0; c < HALF; c += 16) {
@@ -1570,6 +1645,7 @@ __global__ void __launch_bounds__(kCta, 1)
           }
         }
       }
+  taken_all:;
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -1589,6 +1665,7 @@ struct BothArgs {
   int biases;
   int vx_width;      // columns of v_x: K, or fewer where K was padded
   int wide_out;
+  WaitArgs waits;
 };
 
 // Rows of K and M of up to 128 features, on 16-byte boundaries: v_y, y and x
@@ -1605,7 +1682,7 @@ struct BothArgs {
 // rounding them, 2^-24 of the sum on average at each of a tile's 8 additions
 // (32 tiles: 2 M rows 128-128 were 2e-6 low).
 constexpr int kPiece = 4;
-constexpr int kBothBars = 29;
+constexpr int kBothBars = 30;
 
 template <typename T, int ACT, bool SHARED>
 __global__ void __launch_bounds__(2 * kThreads + 64, 1)
@@ -1629,6 +1706,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   float (*const s_db)[64] = reinterpret_cast<float (*)[64]>(s_stage + 8 * 2048);
   uint64_t* const s_bars = reinterpret_cast<uint64_t*>(s_db + 8);
   uint32_t& s_tmem = *reinterpret_cast<uint32_t*>(s_bars + kBothBars);
+  uint32_t& s_stop = (&s_tmem)[1];
   const uint32_t bar0 = tc::smem_addr(s_bars);
   auto full = [&](int i) { return bar0 + 8 * i; };
   auto free_ = [&](int i) { return bar0 + 8 * (4 + i); };
@@ -1639,7 +1717,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   auto taken = [&](int i) { return bar0 + 8 * (22 + i); };
   auto sum_made = [&](int i) { return bar0 + 8 * (24 + i); };
   auto sum_taken = [&](int i) { return bar0 + 8 * (26 + i); };
-  const uint32_t weighed = bar0 + 8 * 28;
+  const uint32_t weighed = bar0 + 8 * 28, drained = bar0 + 8 * 29;
 
   if (warp == 0) tc::alloc(&s_tmem, columns);
   if (threadIdx.x == 32) {
@@ -1657,18 +1735,17 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       tc::bar_init(sum_taken(i), 8);
     }
     tc::bar_init(weighed, 8);
+    tc::bar_init(drained, 1);
+    s_stop = 0;
     tc::bar_init_done();
   }
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem, sum_acc = tmem + NBUF * TERMS * nk;
-  uint32_t limit = kWaitLimit;
+  bool alive = true;  // no wait of this warp gave up
   auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (!tc::bar_wait(bar, parity & 1, limit)) {
-      limit = 0;
-      g_wait_gave_up = 1;
-    }
+    alive = alive && waited(bar, parity, p.waits, &s_stop);
   };
 
   const int64_t tiles = (p.s.R + kTile - 1) / kTile;
@@ -1686,7 +1763,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   if (warp == 17) {
     // ------------------------------------------------------------- TMA
     Ring ring(p.slots), y_ring(p.ys);
-    int id[4];
+    int sent = 0, y_sent = 0, id[4];
     auto read_ids = [&](const Run& t, int row) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -1704,7 +1781,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         for (int i = 0; i < 4; ++i) rows[i] = id[i];
         read_ids(cur, row + kTile);
       }
-      if (ring.turn > 0) wait(free_(slot), ring.turn - 1);
+      if (ring.turn > 0) WAIT_OR(sent_all, free_(slot), ring.turn - 1);
       if (tc::elected()) {
         const uint32_t to = tc::smem_addr(s_tiles + slot * tile_bytes);
         tc::expect(full(slot), tile_bytes);
@@ -1719,16 +1796,21 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         tc::load_rows4(tc::smem_addr(s_tiles + slot * tile_bytes) + (p.pm + j) * kPanel + lane * 512,
                        &map_x, j * 64, rows, full(slot));
       __syncwarp();
+      ++sent;
       for (int j = 0; HAS_Y && j < p.pm; ++j, y_ring.next()) {
         const int ys = y_ring.slot;
-        if (y_ring.turn > 0) wait(y_free(ys), y_ring.turn - 1);
+        if (y_ring.turn > 0) WAIT_OR(sent_all, y_free(ys), y_ring.turn - 1);
         if (tc::elected()) {
           tc::expect(y_full(ys), kPanel);
           tc::load_box(tc::smem_addr(s_y + ys * kPanel), &map_y, j * 64, row, y_full(ys));
         }
         __syncwarp();
+        ++y_sent;
       }
     }
+  sent_all:
+    drain_ring(sent, p.slots, full);
+    if (HAS_Y) drain_ring(y_sent, p.ys, y_full);
   } else if (warp == 16) {
     // ------------------------------------------------------------- MMAs
     const uint32_t by_rows = tc::instr_desc(Mma<T>::format, (K + 15) / 16 * 16) | tc::kMnMajorB;
@@ -1745,11 +1827,11 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       char* const vz = s_tiles + slot * tile_bytes;
       const uint32_t v_at = tc::smem_addr(vz), x_at = v_at + p.pm * kPanel;
       const uint32_t low_at = tc::smem_addr(s_y + ys * kPanel);  // whole tiles: ys % pm == 0
-      wait(ready(slot), ring.turn);
+      WAIT_OR(mma_done, ready(slot), ring.turn);
       if (p.vx) {
-        if (left == cur.n) wait(weighed, stagings++);
+        if (left == cur.n) WAIT_OR(mma_done, weighed, stagings++);
         const int buf = NBUF == 2 ? t & 1 : 0;
-        if (t >= NBUF) wait(taken(buf), t / NBUF - 1);
+        if (t >= NBUF) WAIT_OR(mma_done, taken(buf), t / NBUF - 1);
         tc::fence_after_sync();
         const uint32_t acc = tmem + buf * TERMS * nk;
         for (int i = 0; i < steps; ++i) {  // 16 of M: 32 bytes of a row, 16 rows of weights
@@ -1762,7 +1844,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         tc::commit(leader, made(buf));
       }
       const int sum_buf = NBUF == 2 ? sums & 1 : 0;
-      if (piece == 0 && sums >= NBUF) wait(sum_taken(sum_buf), sums / NBUF - 1);
+      if (piece == 0 && sums >= NBUF) WAIT_OR(mma_done, sum_taken(sum_buf), sums / NBUF - 1);
       tc::fence_after_sync();
       const uint32_t sum = sum_acc + sum_buf * nm;
 #pragma unroll
@@ -1783,7 +1865,9 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       }
       ys = ys + p.pm >= p.ys ? 0 : ys + p.pm;
     }
-    if (t > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
+  mma_done:
+    tc::commit(leader, drained);  // every MMA is done before the memory goes
+    drain(drained, 0);
   } else if (warp < 8) {
     // ------------------------------------------------------------ front warps
     const int tid = threadIdx.x;
@@ -1817,7 +1901,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         stage_weights(cur.g);
         tc::fence_smem();
         __syncwarp();
-        if (lane == 0) tc::arrive(weighed);
+        if (lane == 0 && alive) tc::arrive(weighed);
       }
       wait(full(slot), ring.turn);
       char* const vz = s_tiles + slot * tile_bytes;
@@ -1850,7 +1934,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
           if (TERMS == 1) {
             tc::fence_smem();  // read before TMA writes there again
             __syncwarp();
-            if (lane == 0) tc::arrive(y_free(ys));
+            if (lane == 0 && alive) tc::arrive(y_free(ys));
           }
           y_ring.next();
         }
@@ -1864,7 +1948,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       }
       tc::fence_smem();
       __syncwarp();
-      if (lane == 0) tc::arrive(ready(slot));
+      if (lane == 0 && alive) tc::arrive(ready(slot));
       if (left <= kTile) {  // the group's v_b, summed in a fixed order
         if (p.biases) {
           float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1)) +
@@ -1907,7 +1991,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         int into = -1;
         if (SHARED && live && lane < rows) into = __ldg(p.ids + row + lane);
         if (live) {
-          wait(made(buf), t / NBUF);
+          WAIT_OR(taken_all, made(buf), t / NBUF);
           tc::fence_after_sync();
         }
         if (into >= p.s.n) into = -1;
@@ -1927,7 +2011,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         const bool last = left <= kTile;
         if (++piece == kPiece || last) {
           const int sum_buf = NBUF == 2 ? sums & 1 : 0;
-          wait(sum_made(sum_buf), sums / NBUF);
+          WAIT_OR(taken_all, sum_made(sum_buf), sums / NBUF);
           tc::fence_after_sync();
           const uint32_t sum = sum_acc + sum_buf * nm + ((uint32_t)row0 << 16);
           float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1));
@@ -1951,6 +2035,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         }
       }
     }
+  taken_all:;
   }
   tc::fence_before_sync();
   __syncthreads();
@@ -2473,8 +2558,8 @@ int launch_narrow(NarrowArgs p, bool backward, int parts, cudaStream_t st) {
 }
 
 template <typename T, int ACT>
-int run_fwd(const Shape& s, const void* x, const int32_t* ids, const int32_t* off, const void* w,
-            const void* b, void* y, cudaStream_t st) {
+int run_fwd(const Shape& s, const WaitArgs& waits, const void* x, const int32_t* ids,
+            const int32_t* off, const void* w, const void* b, void* y, cudaStream_t st) {
   if (is_narrow(s.K, s.M, dtype_of<T>, false)) {
     NarrowArgs p{};
     p.s = s;
@@ -2487,6 +2572,7 @@ int run_fwd(const Shape& s, const void* x, const int32_t* ids, const int32_t* of
   p.s = s;
   p.a = x, p.ids = ids, p.off = off, p.w = w, p.bias = b, p.out = y;
   p.depth = s.K, p.width = s.M;
+  p.waits = waits;
   p.wide_w = s.K * sizeof(T) % 16 == 0 && on16(w);
   p.wide_out = s.M * sizeof(T) % 16 == 0 && on16(y);
   return launch_rows<T, ACT, kForward, false>(p, st);
@@ -2539,7 +2625,7 @@ Plan plan_of(const gs_grouped_params* p) {  // one CTA an SM, or two
 template <int ACT, int NT>
 int launch_weights32(const Shape& s, const void* x, const void* y, const void* vy,
                      const int32_t* ids, const int32_t* off, float* part, const void* vb,
-                     const Plan& q, cudaStream_t st) {
+                     const WaitArgs& waits, const Plan& q, cudaStream_t st) {
   constexpr auto kernel = weights32_kernel<ACT, NT>;
   constexpr int kAll = 227 * 1024;  // this kernel has no static shared memory
   if (int rc = allow_smem<kernel, kAll>()) return rc;
@@ -2547,13 +2633,13 @@ int launch_weights32(const Shape& s, const void* x, const void* y, const void* v
   p.s = s;
   p.x = static_cast<const float*>(x), p.y = static_cast<const float*>(y);
   p.vy = static_cast<const float*>(vy), p.ids = ids, p.off = off, p.part = part;
-  p.kt = q.kt, p.biases = vb != nullptr;
+  p.kt = q.kt, p.biases = vb != nullptr, p.waits = waits;
   p.kx = ((s.K < 128 ? s.K : 128) + 31) / 32, p.mx = ((s.M < NT ? s.M : NT) + 31) / 32;
   const bool wide_x = s.K % 4 == 0 && on16(x);
   p.x_mode = wide_x && s.n > 0 ? (ids ? 1 : 0) : 2;
   p.v_mode = s.M % 4 == 0 && on16(vy) && (!y || on16(y)) ? 0 : 2;
   const int set = 2 * (p.kx + p.mx) * kBox, slot = (p.kx + p.mx * (ACT ? 2 : 1)) * kBox;
-  const int bars = 28 * 8 + 8;
+  const int bars = kBars32 * 8 + 8;
   // an x operand's MMA reads 128 rows from its start on: they lie in the sets
   // and slots behind it
   // Two sets a front group where there is room: the next panel's operands are
@@ -2624,9 +2710,9 @@ int launch_both(BothArgs p, const void* x, const void* vy, const void* y, const 
 }
 
 template <typename T, int ACT>
-int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const int32_t* ids,
-            const int32_t* off, const void* w, const void* y, const void* vy, void* vx, void* vw,
-            void* vb, float* ws, cudaStream_t st) {
+int run_bwd(const gs_grouped_params* prm, const Shape& s, const WaitArgs& waits, const void* x,
+            const int32_t* ids, const int32_t* off, const void* w, const void* y, const void* vy,
+            void* vx, void* vw, void* vb, float* ws, cudaStream_t st) {
   constexpr bool kSplit = sizeof(T) == 2 && ACT == GS_ACT_SIGMOID;
   const Plan q = plan_of(prm);
   if (ACT == GS_ACT_NONE) y = nullptr;
@@ -2658,7 +2744,7 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
       p.s = s;
       p.ids = ids, p.off = off, p.part = ws;
       p.vx = !vx ? nullptr : shared ? sum : vx;
-      p.vx_width = s.K;
+      p.vx_width = s.K, p.waits = waits;
       p.wide_out = s.K * (shared ? 4 : 2) % 16 == 0 && on16(p.vx);
       p.biases = vb != nullptr;
       if (pad) {
@@ -2692,7 +2778,7 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
       RowsArgs p{};
       p.s = s;
       p.a = vy, p.y = y, p.ids = ids, p.off = off, p.w = w, p.out = shared ? sum : vx;
-      p.depth = s.M, p.width = s.K;
+      p.depth = s.M, p.width = s.K, p.waits = waits;
       const size_t each = shared ? 4 : sizeof(T);
       p.wide_out = s.K * each % 16 == 0 && on16(p.out);
       const int rc = shared ? launch_rows<T, ACT, kScatter, kSplit>(p, st)
@@ -2707,15 +2793,16 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
     if (q.narrow) {
     } else if constexpr (sizeof(T) == 4) {
       if (s.R > 0) {
-        const int rc = q.nt == 64 ? launch_weights32<ACT, 64>(s, x, y, vy, ids, off, ws, vb, q, st)
-                                  : launch_weights32<ACT, 128>(s, x, y, vy, ids, off, ws, vb, q, st);
+        const int rc =
+            q.nt == 64 ? launch_weights32<ACT, 64>(s, x, y, vy, ids, off, ws, vb, waits, q, st)
+                      : launch_weights32<ACT, 128>(s, x, y, vy, ids, off, ws, vb, waits, q, st);
         if (rc) return rc;
       }
     } else if (s.R > 0 && !both) {
       WeightArgs p{};
       p.s = s;
       p.x = x, p.y = y, p.vy = vy, p.ids = ids, p.off = off, p.part = ws;
-      p.kt = q.kt, p.mt = q.mt, p.biases = vb != nullptr;
+      p.kt = q.kt, p.mt = q.mt, p.biases = vb != nullptr, p.waits = waits;
       p.wide_x = s.K * sizeof(T) % 16 == 0 && on16(x);
       p.wide_y = s.M * sizeof(T) % 16 == 0 && on16(vy) && (!y || on16(y));
       const int rc = q.nt == 64 ? launch_weights<T, ACT, 64, kSplit>(p, q, st)
@@ -2749,6 +2836,47 @@ int run_bwd(const gs_grouped_params* prm, const Shape& s, const void* x, const i
     case 7: return f<__half, GS_ACT_RELU>(__VA_ARGS__);                                \
     default: return f<__half, GS_ACT_SIGMOID>(__VA_ARGS__);                            \
   }
+
+// The word of the current device that says that a wait of a call without a word of
+// its own gave up: in pinned host memory, so that the host reads it without
+// waiting for the device.
+int device_word(uint32_t** word) {
+  static std::mutex mutex;
+  static uint32_t* words = nullptr;  // a cache line for each device
+  constexpr int kDevices = 64, kApart = 32;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return launch_status("grouped_linear");
+  if (dev < 0 || dev >= kDevices) return invalid("grouped_linear: device index past 63");
+  std::lock_guard<std::mutex> lock(mutex);
+  if (!words) {
+    // the current stream may be recording a graph, of which this is no part
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    void* p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, kDevices * kApart * sizeof(uint32_t),
+                                        cudaHostAllocPortable | cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return launch_status("grouped_linear");
+    std::memset(p, 0, kDevices * kApart * sizeof(uint32_t));
+    words = static_cast<uint32_t*>(p);
+  }
+  *word = words + dev * kApart;
+  return GS_OK;
+}
+
+int gave_up() {
+  set_error("grouped_linear: a wait inside a kernel gave up: its call's results are void");
+  return GS_ERR_DEVICE;
+}
+
+// Where a call's waits report to, and how long they are.
+int waits_of(const gs_grouped_params* p, WaitArgs* w) {
+  w->limit = p->wait_limit ? p->wait_limit - 1 : kWaitLimit;
+  w->status = p->status;
+  if (p->status) return GS_OK;
+  if (int rc = device_word(&w->status)) return rc;
+  return __atomic_load_n(w->status, __ATOMIC_ACQUIRE) ? gave_up() : GS_OK;
+}
 
 // Rows are counted in 32 bits, some tiles past the last.
 constexpr int64_t kRowsMost = INT32_MAX - 4096;
@@ -2796,7 +2924,9 @@ extern "C" int gs_grouped_linear_fwd(const gs_grouped_params* p, const void* x,
     return invalid("grouped_linear: missing buffer");
   if (!p->use_row_ids) row_ids = nullptr;
   const Shape s{p->rows, p->n, p->groups, p->in_features, p->out_features};
-  GROUPED_DISPATCH(p, run_fwd, s, x, row_ids, offsets, weights, biases, y, as_stream(stream));
+  WaitArgs waits;
+  if (int rc = waits_of(p, &waits)) return rc;
+  GROUPED_DISPATCH(p, run_fwd, s, waits, x, row_ids, offsets, weights, biases, y, as_stream(stream));
 }
 
 extern "C" size_t gs_grouped_linear_bwd_workspace_size(const gs_grouped_params* p) {
@@ -2824,22 +2954,17 @@ extern "C" int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
   }
   if (!p->use_row_ids) row_ids = nullptr;
   const Shape s{p->rows, p->n, p->groups, p->in_features, p->out_features};
-  GROUPED_DISPATCH(p, run_bwd, p, s, x, row_ids, offsets, weights, y, v_y, v_x, v_weights, v_biases,
-                   static_cast<float*>(workspace), as_stream(stream));
+  WaitArgs waits;
+  if (int rc = waits_of(p, &waits)) return rc;
+  GROUPED_DISPATCH(p, run_bwd, p, s, waits, x, row_ids, offsets, weights, y, v_y, v_x, v_weights,
+                   v_biases, static_cast<float*>(workspace), as_stream(stream));
 }
 
 extern "C" int gs_grouped_linear_check(gs_stream_t stream) {
-  unsigned int gave_up = 0, none = 0;
-  cudaStream_t s = as_stream(stream);
-  if (cudaMemcpyFromSymbolAsync(&gave_up, g_wait_gave_up, sizeof(gave_up), 0,
-                                cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
+  if (cudaStreamSynchronize(as_stream(stream)) != cudaSuccess)
     return launch_status("grouped_linear_check");
-  if (!gave_up) return GS_OK;
-  if (cudaMemcpyToSymbolAsync(g_wait_gave_up, &none, sizeof(none), 0, cudaMemcpyHostToDevice, s) !=
-          cudaSuccess ||
-      cudaStreamSynchronize(s) != cudaSuccess)
-    return launch_status("grouped_linear_check");
-  set_error("grouped_linear: a wait for a tensor-core tile gave up: results are void");
-  return GS_ERR_DEVICE;
+  uint32_t* word = nullptr;
+  if (int rc = device_word(&word)) return rc;
+  if (!__atomic_exchange_n(word, 0u, __ATOMIC_ACQ_REL)) return GS_OK;
+  return gave_up();
 }

@@ -161,9 +161,13 @@ def grouped_linear_backward(inputs, y, v_y, activation="none",
     return out
 
 
-def check():
-    """Waits for the current stream and raises if a bounded on-device wait of
-    a grouped_linear kernel gave up (its results would be invalid)."""
+def check(device=None):
+    """Waits for the current stream of ``device`` (None: the current one) and
+    raises if a bounded on-device wait of a grouped_linear call on that device
+    gave up since the last check: what that call gave is void.  Until then the
+    calls behind it on the device raise, too (the backward of a step, or the
+    next step, without waiting for anything); after it they run again."""
     lib = _lib.load()
-    check_status(lib.gs_grouped_linear_check(torch.cuda.current_stream().cuda_stream),
-                 "grouped_linear")
+    with torch.cuda.device(device):
+        check_status(lib.gs_grouped_linear_check(torch.cuda.current_stream().cuda_stream),
+                     "grouped_linear")

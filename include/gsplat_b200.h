@@ -683,6 +683,11 @@ typedef struct {
   int32_t dtype;        /* gs_dtype of x, weights, biases, y and gradients  */
   int32_t activation;   /* gs_activation                                    */
   int32_t use_row_ids;  /* 1: row_ids is given; 0: id(r) = r                */
+  uint32_t wait_limit;  /* 0, or n: a wait inside a kernel gives up after n - 1
+                           polls of 20 us (see gs_grouped_linear_check)     */
+  uint32_t* status;     /* a word that kernels can write (device or pinned
+                           host memory), which the call sets to 1 where a wait
+                           gives up; NULL: the library's, one a device      */
 } gs_grouped_params;
 
 /* y[r] = act(weights[g] x[id(r)] + biases[g]) for offsets[g] <= r <
@@ -719,10 +724,15 @@ int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
                           void* workspace, size_t workspace_bytes,
                           gs_stream_t stream);
 
-/* Waits for the stream and tells whether a wait inside a grouped_linear
- * kernel of this device gave up since the last check (GS_ERR_DEVICE: what it
- * wrote is void).  The waits are for the kernel's own copies and tensor-core
- * tiles and are bounded, at a second or more. */
+/* The grouped_linear kernels wait for their own copies and tensor-core tiles,
+ * for a second or more at most.  One that gives up (a defect, not a workload
+ * condition) leaves its call's results void, sets the call's status word, and
+ * returns.  The word of calls without one of their own is the device's: from
+ * then on such calls are refused on that device (GS_ERR_DEVICE, before they
+ * launch anything) until this has reported it.  Waits for the stream, then
+ * reads and clears the current device's word in one step: GS_OK, or
+ * GS_ERR_DEVICE where a call of any stream of the device gave up since the
+ * last check.  A call whose report must be nobody else's brings a word. */
 int gs_grouped_linear_check(gs_stream_t stream);
 
 #ifdef __cplusplus
