@@ -2594,6 +2594,8 @@ struct Plan {
 
 Plan plan_of(const gs_grouped_params* p) {  // one CTA an SM, or two
   Plan q;
+  const int wanted = p->wanted ? p->wanted : GS_WANT_V_X | GS_WANT_V_WEIGHTS | GS_WANT_V_BIASES;
+  const bool sums = wanted & (GS_WANT_V_WEIGHTS | GS_WANT_V_BIASES);
   q.nt = p->out_features > 64 ? 128 : 64;
   q.kt = (int)ceil_div(p->in_features, 128);
   q.mt = (int)ceil_div(p->out_features, q.nt);
@@ -2612,13 +2614,15 @@ Plan plan_of(const gs_grouped_params* p) {  // one CTA an SM, or two
   n = n < 1 ? 1 : n > tiles ? tiles : n;
   q.parts = (int)n;
   q.copies = p->dtype == GS_F32 && !q.narrow ? kBiasCopies32 : 1;
-  q.part_floats = ((size_t)q.parts + p->groups) * q.mp * ((size_t)q.kp + q.copies);
-  q.sum_floats = p->use_row_ids && p->dtype != GS_F32 ? (size_t)p->n * p->in_features : 0;
+  q.part_floats = sums ? ((size_t)q.parts + p->groups) * q.mp * ((size_t)q.kp + q.copies) : 0;
+  q.sum_floats = wanted & GS_WANT_V_X && p->use_row_ids && p->dtype != GS_F32
+                     ? (size_t)p->n * p->in_features : 0;
   q.part_floats = (q.part_floats + 63) / 64 * 64;  // the sums start on 256 bytes
   q.sum_floats = (q.sum_floats + 63) / 64 * 64;
-  q.pad_x = q.padded ? (size_t)p->n * q.kp : 0;
-  q.pad_w = q.padded ? (size_t)p->groups * q.mp * q.kp : 0;
-  q.pad_v = q.padded ? (size_t)p->rows * q.mp : 0;
+  const bool copies = q.padded && sums;
+  q.pad_x = copies ? (size_t)p->n * q.kp : 0;
+  q.pad_w = copies ? (size_t)p->groups * q.mp * q.kp : 0;
+  q.pad_v = copies ? (size_t)p->rows * q.mp : 0;
   return q;
 }
 
@@ -2896,6 +2900,8 @@ int bad_params(const gs_grouped_params* p) {
   if (p->dtype < GS_F32 || p->dtype > GS_F16) return invalid("grouped_linear: unknown dtype");
   if (p->activation < GS_ACT_NONE || p->activation > GS_ACT_SIGMOID)
     return invalid("grouped_linear: unknown activation");
+  if (p->wanted & ~(GS_WANT_V_X | GS_WANT_V_WEIGHTS | GS_WANT_V_BIASES))
+    return invalid("grouped_linear: unknown gradient wanted");
   return GS_OK;
 }
 
@@ -2943,12 +2949,16 @@ extern "C" int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
                                      size_t workspace_bytes, gs_stream_t stream) {
   if (int rc = bad_params(p)) return rc;
   if (!v_x && !v_weights && !v_biases) return GS_OK;
+  const int given = (v_x ? GS_WANT_V_X : 0) | (v_weights ? GS_WANT_V_WEIGHTS : 0) |
+                    (v_biases ? GS_WANT_V_BIASES : 0);
+  if (p->wanted && given & ~p->wanted)
+    return invalid("grouped_linear: a gradient that wanted does not name");
   if (!offsets || !weights || (p->n > 0 && !x) ||
       (p->rows > 0 && (!v_y || (p->activation != GS_ACT_NONE && !y) ||
                        (p->use_row_ids && !row_ids))))
     return invalid("grouped_linear: missing buffer");
   const size_t need = gs_grouped_linear_bwd_workspace_size(p);
-  if (!workspace || workspace_bytes < need || !on16(workspace)) {
+  if (need > 0 && (!workspace || workspace_bytes < need || !on16(workspace))) {
     set_error("grouped_linear: a workspace of %zu bytes on a 16-byte boundary is needed", need);
     return GS_ERR_WORKSPACE;
   }

@@ -25,6 +25,7 @@ from ._lib import GroupedParams, on_device_of
 from ._lib import check as check_status
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_WANTED = {"v_x": 1, "v_weights": 2, "v_biases": 4}
 _GROUPS_MOST = 2 ** 31 - 2
 _ACTIVATIONS = {"none": 0, "relu": 1, "sigmoid": 2}
 
@@ -147,6 +148,9 @@ def grouped_linear_backward(inputs, y, v_y, activation="none",
         out["v_weights"] = torch.empty_like(w)
     if "v_biases" in wanted and b is not None:
         out["v_biases"] = torch.empty_like(b)
+    if not out:
+        return out
+    p.wanted = sum(_WANTED[k] for k in out)  # scratch for these alone
     lib = _lib.load()
 
     def call(stream):

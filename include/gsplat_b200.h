@@ -672,6 +672,7 @@ int gs_dropout(const gs_dropout_params* p, const void* x, const int64_t* step_de
 int gs_group_offsets(int64_t n, const int32_t* sorted_ids, int32_t groups,
                      int32_t* offsets, gs_stream_t stream);
 
+enum gs_grouped_wanted { GS_WANT_V_X = 1, GS_WANT_V_WEIGHTS = 2, GS_WANT_V_BIASES = 4 };
 enum gs_activation { GS_ACT_NONE = 0, GS_ACT_RELU = 1, GS_ACT_SIGMOID = 2 };
 
 typedef struct {
@@ -685,6 +686,8 @@ typedef struct {
   int32_t use_row_ids;  /* 1: row_ids is given; 0: id(r) = r                */
   uint32_t wait_limit;  /* 0, or n: a wait inside a kernel gives up after n - 1
                            polls of 20 us (see gs_grouped_linear_check)     */
+  int32_t wanted;       /* the backward: gs_grouped_wanted bits of the gradients
+                           that may be asked for (less scratch), or 0: any  */
   uint32_t* status;     /* a word that kernels can write (device or pinned
                            host memory), which the call sets to 1 where a wait
                            gives up; NULL: the library's, one a device      */
@@ -705,7 +708,9 @@ int gs_grouped_linear_fwd(const gs_grouped_params* p, const void* x,
                           const void* weights, const void* biases, void* y,
                           gs_stream_t stream);
 
-/* Bytes of scratch of the backward, on a 16-byte boundary. */
+/* Bytes of scratch of the backward, on a 16-byte boundary: for partial sums
+ * of v_weights and v_biases, for fp32 sums of a 16-bit v_x with row_ids, and for
+ * copies of odd 16-bit widths; none for what params.wanted leaves out. */
 size_t gs_grouped_linear_bwd_workspace_size(const gs_grouped_params* p);
 
 /* Its reverse mode from y (the forward's; may be NULL for GS_ACT_NONE) and

@@ -51,7 +51,7 @@ class Call:
         self.sizes = (R, n, 3, K, M, list(TYPES).index(dtype), ACTS[act], int(bool(N)))
 
     def params(self, limit, status):
-        return self.L.GroupedParams(*self.sizes, limit, None if status is None else status.data_ptr())
+        return self.L.GroupedParams(*self.sizes, limit, 0, None if status is None else status.data_ptr())
 
     def forward(self, limit=0, status=None):
         y, p = torch.empty_like(self.y), self.params(limit, status)
