@@ -458,7 +458,8 @@ __global__ void __launch_bounds__(kScanThreads) visible_depth_keys_kernel(
 // With the scanned block counts of visible_count_kernel: the visible
 // elements' projection outputs as packed rows, in element (image, Gaussian)
 // order -- image and Gaussian ids, radii, means2d, depths, conics and, when
-// given, compensations.  Rows past `capacity` are dropped.
+// given, compensations.  Rows past `capacity` are dropped.  image_offsets, if
+// given: the rows in front of each image, and of the end.
 struct PackArgs {
   int64_t n, capacity;
   int N;
@@ -466,6 +467,7 @@ struct PackArgs {
   const float *means2d, *depths, *conics, *comps;
   int32_t *image_ids, *gaussian_ids, *p_radii;
   float *p_means2d, *p_depths, *p_conics, *p_comps;
+  int32_t* image_offsets;
 };
 
 __global__ void __launch_bounds__(kScanThreads) pack_rows_kernel(const PackArgs a,
@@ -482,6 +484,17 @@ __global__ void __launch_bounds__(kScanThreads) pack_rows_kernel(const PackArgs 
   }
   int64_t total;
   int64_t run = block_exclusive_scan<kScanThreads>(acc, s_warp, &total) + sums[blockIdx.x];
+  const int64_t first = base + (int64_t)threadIdx.x * kScanItems;
+  if (a.image_offsets && first < a.n) {  // where an image starts among this thread's elements
+    const int64_t end = min(first + kScanItems, a.n);
+    int64_t image = (first + a.N - 1) / a.N, rows = run, at = first;
+#pragma unroll
+    for (int k = 0; k < kScanItems; ++k, ++at) {
+      if (at < end && at == image * a.N) a.image_offsets[image++] = (int32_t)rows;
+      rows += f[k];
+    }
+    if (end == a.n) a.image_offsets[a.n / a.N] = (int32_t)rows;
+  }
 #pragma unroll
   for (int k = 0; k < kScanItems; ++k) {
     if (!f[k]) continue;
@@ -1920,11 +1933,24 @@ extern "C" int gs_pack_visible(int64_t n_elements, int32_t N, const int32_t* rad
                                float* p_depths, float* p_conics, float* p_compensations,
                                int64_t* nnz_device, void* workspace, size_t workspace_bytes,
                                gs_stream_t stream) {
+  return gs_pack_visible_images(n_elements, N, radii, means2d, depths, conics, compensations,
+                                capacity, image_ids, gaussian_ids, p_radii, p_means2d, p_depths,
+                                p_conics, p_compensations, nullptr, nnz_device, workspace,
+                                workspace_bytes, stream);
+}
+
+extern "C" int gs_pack_visible_images(
+    int64_t n_elements, int32_t N, const int32_t* radii, const float* means2d,
+    const float* depths, const float* conics, const float* compensations, int64_t capacity,
+    int32_t* image_ids, int32_t* gaussian_ids, int32_t* p_radii, float* p_means2d,
+    float* p_depths, float* p_conics, float* p_compensations, int32_t* image_offsets,
+    int64_t* nnz_device, void* workspace, size_t workspace_bytes, gs_stream_t stream) {
   if (n_elements < 0 || N <= 0 || (n_elements % N) != 0 || capacity < 0 || !nnz_device)
     return invalid("pack_visible: bad sizes");
   cudaStream_t s = as_stream(stream);
   if (n_elements == 0) {
-    if (cudaMemsetAsync(nnz_device, 0, sizeof(int64_t), s) != cudaSuccess)
+    if (cudaMemsetAsync(nnz_device, 0, sizeof(int64_t), s) != cudaSuccess ||
+        (image_offsets && cudaMemsetAsync(image_offsets, 0, sizeof(int32_t), s) != cudaSuccess))
       return launch_status("pack_visible");
     return GS_OK;
   }
@@ -1943,8 +1969,9 @@ extern "C" int gs_pack_visible(int64_t n_elements, int32_t N, const int32_t* rad
   scan_sums_kernel<<<1, 1024, 0, s>>>(nb, sums, nnz_device);
   const PackArgs a{n_elements, capacity, N, radii, means2d, depths, conics,
                    compensations, image_ids, gaussian_ids, p_radii, p_means2d, p_depths,
-                   p_conics, compensations ? p_compensations : nullptr};
-  pack_rows_kernel<<<(unsigned)nb, kScanThreads, 0, s>>>(a, sums);
+                   p_conics, compensations ? p_compensations : nullptr, image_offsets};
+  if (capacity > 0 || image_offsets)  // else only the count is wanted
+    pack_rows_kernel<<<(unsigned)nb, kScanThreads, 0, s>>>(a, sums);
   return launch_status("pack_visible");
 }
 

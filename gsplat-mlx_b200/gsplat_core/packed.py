@@ -28,7 +28,7 @@ import torch
 
 from . import _lib
 from ._lib import IsectParams, RasterParams, check
-from .grouped import group_offsets, grouped_linear_backward, grouped_linear_forward
+from .grouped import grouped_linear_backward, grouped_linear_forward
 
 
 def _p(t):
@@ -57,11 +57,13 @@ def pack_projection(proj):
     nnz_dev = torch.zeros((1,), dtype=torch.int64, device=dev)
 
     def call(cap, o):
-        check(lib.gs_pack_visible(n, max(N, 1), _p(radii), _p(m2), _p(dep), _p(con), _p(comps),
-                                  cap, *(_p(o.get(k)) for k in (
-                                      "image_ids", "gaussian_ids", "radii", "means2d", "depths",
-                                      "conics", "compensations")),
-                                  _p(nnz_dev), _p(ws), ws.numel(), _s()), "pack_projection")
+        check(lib.gs_pack_visible_images(n, max(N, 1), _p(radii), _p(m2), _p(dep), _p(con),
+                                         _p(comps), cap, *(_p(o.get(k)) for k in (
+                                             "image_ids", "gaussian_ids", "radii", "means2d",
+                                             "depths", "conics", "compensations",
+                                             "image_offsets")),
+                                         _p(nnz_dev), _p(ws), ws.numel(), _s()),
+              "pack_projection")
 
     call(0, {})
     nnz = int(nnz_dev.item())
@@ -70,8 +72,11 @@ def pack_projection(proj):
     out = {"image_ids": i32(nnz), "gaussian_ids": i32(nnz), "radii": i32(nnz, 2),
            "means2d": f32(nnz, 2), "depths": f32(nnz), "conics": f32(nnz, 3),
            "compensations": f32(nnz) if comps is not None else None}
+    images = math.prod(radii.shape[:-2])
+    # (without elements nothing runs that would write them)
+    out["image_offsets"] = i32(images + 1) if n else torch.zeros(images + 1, dtype=torch.int32,
+                                                                 device=dev)
     call(nnz, out)
-    out["image_offsets"] = group_offsets(out["image_ids"], math.prod(radii.shape[:-2]))
     return out
 
 

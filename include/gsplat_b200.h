@@ -307,7 +307,9 @@ int gs_isect_tile_encode_binned_culled(const gs_isect_params* p, const float* me
  * [nnz], conics [nnz,3], compensations [nnz] (when given).  *nnz_device gets
  * the row count; rows past `capacity` are not written (size the outputs
  * with a first call of capacity 0, or with an upper bound).  Workspace:
- * gs_pack_visible_workspace_size(n_elements) bytes.
+ * gs_pack_visible_workspace_size(n_elements) bytes.  gs_pack_visible_images is
+ * the same with image_offsets [I+1] (or NULL): image i's rows are those from
+ * image_offsets[i] up to image_offsets[i+1], capacity or not; nnz below 2^31.
  *
  * gs_isect_tile_encode_binned_packed: the binned encode over nnz packed
  * rows (p->N = nnz, p->I = images): element i's image is image_ids[i],
@@ -325,6 +327,14 @@ int gs_pack_visible(int64_t n_elements, int32_t N, const int32_t* radii,
                     float* p_conics, float* p_compensations,
                     int64_t* nnz_device, void* workspace, size_t workspace_bytes,
                     gs_stream_t stream);
+int gs_pack_visible_images(int64_t n_elements, int32_t N, const int32_t* radii,
+                           const float* means2d, const float* depths,
+                           const float* conics, const float* compensations,
+                           int64_t capacity, int32_t* image_ids, int32_t* gaussian_ids,
+                           int32_t* p_radii, float* p_means2d, float* p_depths,
+                           float* p_conics, float* p_compensations,
+                           int32_t* image_offsets, int64_t* nnz_device, void* workspace,
+                           size_t workspace_bytes, gs_stream_t stream);
 size_t gs_isect_tile_encode_binned_packed_workspace_size(const gs_isect_params* p,
                                                          int64_t n_bin_entries);
 int gs_isect_tile_encode_binned_packed(const gs_isect_params* p,
