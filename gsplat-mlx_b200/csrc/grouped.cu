@@ -98,7 +98,7 @@ __device__ __forceinline__ float through(float v, float y) {
 // which other warps meet it.  Whoever sent bulk copies or MMAs waits for those
 // (with a limit of its own) before the CTA gives its memory back.  The results
 // are void.
-constexpr uint32_t kWaitLimit = 1u << 16;   // polls of 20 us: a second or more
+constexpr uint32_t kWaitLimit = 1u << 18;   // polls of 4 us: a second
 constexpr uint32_t kDrainLimit = 1u << 12;  // for what takes microseconds
 
 struct WaitArgs {

@@ -695,7 +695,7 @@ typedef struct {
   int32_t activation;   /* gs_activation                                    */
   int32_t use_row_ids;  /* 1: row_ids is given; 0: id(r) = r                */
   uint32_t wait_limit;  /* 0, or n: a wait inside a kernel gives up after n - 1
-                           polls of 20 us (see gs_grouped_linear_check)     */
+                           polls of 4 us (see gs_grouped_linear_check)      */
   int32_t wanted;       /* the backward: gs_grouped_wanted bits of the gradients
                            that may be asked for (less scratch), or 0: any  */
   uint32_t* status;     /* a word that kernels can write (device or pinned
@@ -740,7 +740,7 @@ int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
                           gs_stream_t stream);
 
 /* The grouped_linear kernels wait for their own copies and tensor-core tiles,
- * for a second or more at most.  One that gives up (a defect, not a workload
+ * for a second at most.  One that gives up (a defect, not a workload
  * condition) leaves its call's results void, sets the call's status word, and
  * returns.  The word of calls without one of their own is the device's: from
  * then on such calls are refused on that device (GS_ERR_DEVICE, before they
