@@ -102,7 +102,7 @@ int gave_up() {
 
 // Where a call's waits report to, and how long they are.
 int waits_of(const gs_grouped_params* p, WaitArgs* w) {
-  w->limit = p->wait_limit ? p->wait_limit - 1 : kWaitLimit;
+  w->limit = p->wait_selftest ? 0 : kWaitLimit;
   w->status = p->status;
   if (p->status) return GS_OK;
   if (int rc = device_word(&w->status)) return rc;

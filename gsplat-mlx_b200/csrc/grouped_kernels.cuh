@@ -93,7 +93,8 @@ __device__ __forceinline__ float through(float v, float y) {
 // what was not done: it leaves its loops, or walks on to the named barriers at
 // which other warps meet it.  Whoever sent bulk copies or MMAs waits for those
 // (with a limit of its own) before the CTA gives its memory back.  The results
-// are void.
+// are void.  A test sets the limit to 0: then the barriers of what arrives expect
+// one arrival that nobody makes.
 constexpr uint32_t kDrainLimit = 1u << 12;  // for what takes microseconds
 
 // False for the whole warp where the wait gave up.
@@ -550,10 +551,11 @@ __global__ void __launch_bounds__(LOAD == kGather ? kCta : kCta - kLoaders, 1)
 
   if (warp == 0) tc::alloc(&s_tmem, columns);
   if (threadIdx.x == 32) {
+    const int none = p.waits.limit == 0;
     for (int i = 0; i < p.slots; ++i) {
-      tc::bar_init(full(i), LOAD == kGather ? kLoaders : 1);
+      tc::bar_init(full(i), (LOAD == kGather ? kLoaders : 1) + none);
       tc::bar_init(free_(i), 1);
-      tc::bar_init(ready(i), 8);
+      tc::bar_init(ready(i), 8 + none);
     }
     tc::bar_init(weighed, 8);
     tc::bar_init(drained, 1);
@@ -1004,7 +1006,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (warp == 0) tc::alloc(&s_tmem, columns);
   if (tid == 0) {
-    tc::bar_init(tc::smem_addr(s_bars), 1);
+    tc::bar_init(tc::smem_addr(s_bars), p.waits.limit == 0 ? 2 : 1);
     tc::bar_init(tc::smem_addr(s_bars + 1), 1);
     s_stop = 0;
     tc::bar_init_done();
@@ -1262,12 +1264,14 @@ __global__ void __launch_bounds__(kCta, 1)
   const bool sent = tma_boxes > 0 || p.x_mode == 1;  // by other than the front warps
   if (warp == 0) tc::alloc(&s_tmem, 4 * NT);
   if (threadIdx.x == 32) {
+    const int none = p.waits.limit == 0;
     for (int i = 0; i < 8; ++i) {
-      tc::bar_init(full(i), max((tma_boxes > 0 ? 1 : 0) + (p.x_mode == 1 ? kLoaders : 0), 1));
+      tc::bar_init(full(i),
+                   max((tma_boxes > 0 ? 1 : 0) + (p.x_mode == 1 ? kLoaders : 0), 1) + none);
       tc::bar_init(free_(i), 4);
     }
     for (int i = 0; i < 4; ++i) {
-      tc::bar_init(ready(i), 4);
+      tc::bar_init(ready(i), 4 + none);
       tc::bar_init(spent(i), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -1710,7 +1714,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   if (warp == 0) tc::alloc(&s_tmem, columns);
   if (threadIdx.x == 32) {
     for (int i = 0; i < 4; ++i) {
-      tc::bar_init(full(i), 1);
+      tc::bar_init(full(i), p.waits.limit == 0 ? 2 : 1);
       tc::bar_init(free_(i), 1);
       tc::bar_init(ready(i), 8);
       tc::bar_init(y_full(i), 1);

@@ -152,23 +152,21 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// A whole warp waits for the phase to end, for up to `limit` polls, which are the
-// hardware's own waits (4 us each on a B200, whatever the hint), and not past the
-// first one behind which *stop (where given) is set; false, for every lane, when it
-// gave up.
+// A whole warp waits for the phase to end, for a poll and up to `limit` more, which
+// are the hardware's own waits (4 us each on a B200, whatever the hint), and not past
+// the first one behind which *stop (where given) is set; false, for every lane, when
+// it gave up.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t limit,
                                          const volatile uint32_t* stop) {
-  while (limit > 0) {
+  while (true) {
     uint32_t done;
     asm volatile(
         "{\n .reg .pred p;\n"
         " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
         : "=r"(done) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
     if (__all_sync(0xffffffffu, done)) return true;
-    if (__any_sync(0xffffffffu, stop && *stop)) return false;
-    --limit;
+    if (limit-- == 0 || __any_sync(0xffffffffu, stop && *stop)) return false;
   }
-  return false;
 }
 
 }  // namespace tc

@@ -95,7 +95,7 @@ class DropoutParams(ct.Structure):
 class GroupedParams(ct.Structure):
     _fields_ = [("rows", _i64), ("n", _i64), ("groups", _i32), ("in_features", _i32),
                 ("out_features", _i32), ("dtype", _i32), ("activation", _i32), ("use_row_ids", _i32),
-                ("wait_limit", ct.c_uint32), ("wanted", _i32), ("status", _vp)]
+                ("wait_selftest", _i32), ("wanted", _i32), ("status", _vp)]
 
 
 _P = ct.POINTER

@@ -694,8 +694,9 @@ typedef struct {
   int32_t dtype;        /* gs_dtype of x, weights, biases, y and gradients  */
   int32_t activation;   /* gs_activation                                    */
   int32_t use_row_ids;  /* 1: row_ids is given; 0: id(r) = r                */
-  uint32_t wait_limit;  /* 0, or n: a wait inside a kernel gives up after n - 1
-                           polls of 4 us (see gs_grouped_linear_check)      */
+  int32_t wait_selftest;/* 1: the kernels' first waits run out, after 4 us, as
+                           if what they wait for never came (a test of the
+                           report: see gs_grouped_linear_check); else 0     */
   int32_t wanted;       /* the backward: gs_grouped_wanted bits of the gradients
                            that may be asked for (less scratch), or 0: any  */
   uint32_t* status;     /* a word that kernels can write (device or pinned

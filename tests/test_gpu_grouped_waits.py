@@ -1,6 +1,6 @@
-"""Waits inside the grouped_linear kernels that give up: without a poll every
-role's first wait ends at once, while the copies that were sent are still
-under way.  The call says so and returns, and the device goes on."""
+"""Waits inside the grouped_linear kernels that run out: of copies that never
+count as arrived, or a tensor-core tile that never counts as done.  The call
+says so and returns, and the device goes on."""
 from __future__ import annotations
 
 import ctypes as ct
@@ -50,17 +50,17 @@ class Call:
         self.y, self.v = rand(R, M).sigmoid(), rand(R, M)
         self.sizes = (R, n, 3, K, M, list(TYPES).index(dtype), ACTS[act], int(bool(N)))
 
-    def params(self, limit, status):
-        return self.L.GroupedParams(*self.sizes, limit, 0, None if status is None else status.data_ptr())
+    def params(self, selftest, status):
+        return self.L.GroupedParams(*self.sizes, selftest, 0, None if status is None else status.data_ptr())
 
-    def forward(self, limit=0, status=None):
-        y, p = torch.empty_like(self.y), self.params(limit, status)
+    def forward(self, selftest=0, status=None):
+        y, p = torch.empty_like(self.y), self.params(selftest, status)
         rc = self.lib.gs_grouped_linear_fwd(ct.byref(p), P(self.x), P(self.ids), P(self.off), P(self.w),
                                             P(self.b), P(y), None)
         return rc, [y]
 
-    def backward(self, limit=0, status=None):
-        p = self.params(limit, status)
+    def backward(self, selftest=0, status=None):
+        p = self.params(selftest, status)
         need = self.lib.gs_grouped_linear_bwd_workspace_size(ct.byref(p))
         ws = torch.empty((need + 3) // 4, dtype=torch.int32, device="cuda")
         out = [torch.zeros_like(t) for t in (self.w, self.b, self.x)]
@@ -82,7 +82,7 @@ def test_a_wait_that_gives_up_is_reported(gs, cuda, direction, dtype, K, M, N, o
     torch.cuda.synchronize()
     rc, want = call(status=status)
     assert rc == 0 and int(status) == 0
-    assert call(limit=1, status=status)[0] == 0
+    assert call(selftest=1, status=status)[0] == 0
     torch.cuda.synchronize()
     assert int(status) == 1
     status.zero_()
@@ -105,7 +105,7 @@ def test_calls_behind_one_that_gave_up_raise(gs, cuda):
     x = c.x.clone().requires_grad_(True)
     y = A.grouped_linear(x, c.w, c.off, c.b)
     torch.cuda.synchronize()
-    assert c.forward(limit=1)[0] == 0
+    assert c.forward(selftest=1)[0] == 0
     torch.cuda.synchronize()
     ids = torch.arange(c.x.shape[0], dtype=torch.int32, device="cuda")
     for f in (lambda: grouped.grouped_linear_forward(inputs),
