@@ -1735,10 +1735,6 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = s_tmem, sum_acc = tmem + NBUF * TERMS * nk;
-  bool alive = true;  // no wait of this warp gave up
-  auto wait = [&](uint32_t bar, uint32_t parity) {
-    alive = alive && waited(bar, parity, p.waits, &s_stop);
-  };
 
   const int64_t tiles = (p.s.R + kTile - 1) / kTile;
   const int end = (int)min(p.s.R, first_tile(tiles, gridDim.x, blockIdx.x + 1) * kTile);
@@ -1885,24 +1881,25 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
     for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
     Ring ring(p.slots), y_ring(p.ys);
     int t = 0;
-    for (Run cur = after_live(none); cur.n > 0; cur = after_live(cur))
+    Run cur;
+    for (cur = after_live(none); cur.n > 0; cur = after_live(cur))
     for (int left = cur.n; left > 0; left -= kTile, ++t, ring.next()) {
       const int slot = ring.slot;
       if (p.vx && left == cur.n) {
-        if (t > 0) wait(free_(ring.slot_before(1)), ring.turn_before(1));
+        if (t > 0) WAIT_OR(walk, free_(ring.slot_before(1)), ring.turn_before(1));
         stage_weights(cur.g);
         tc::fence_smem();
         __syncwarp();
-        if (lane == 0 && alive) tc::arrive(weighed);
+        if (lane == 0) tc::arrive(weighed);
       }
-      wait(full(slot), ring.turn);
+      WAIT_OR(walk, full(slot), ring.turn);
       char* const vz = s_tiles + slot * tile_bytes;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (j >= p.pm) break;
         const int ys = y_ring.slot;
         char* const yt = s_y + ys * kPanel - j * kPanel;
-        if (HAS_Y) wait(y_full(ys), y_ring.turn);
+        if (HAS_Y) WAIT_OR(walk, y_full(ys), y_ring.turn);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t o = j * kPanel + o16 + 4096 * i;
@@ -1926,7 +1923,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
           if (TERMS == 1) {
             tc::fence_smem();  // read before TMA writes there again
             __syncwarp();
-            if (lane == 0 && alive) tc::arrive(y_free(ys));
+            if (lane == 0) tc::arrive(y_free(ys));
           }
           y_ring.next();
         }
@@ -1940,7 +1937,7 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
       }
       tc::fence_smem();
       __syncwarp();
-      if (lane == 0 && alive) tc::arrive(ready(slot));
+      if (lane == 0) tc::arrive(ready(slot));
       if (left <= kTile) {  // the group's v_b, summed in a fixed order
         if (p.biases) {
           float* const to = p.part + (int64_t)(blockIdx.x + cur.g) * ((int64_t)M * (K + 1)) +
@@ -1968,6 +1965,10 @@ __global__ void __launch_bounds__(2 * kThreads + 64, 1)
         for (int i = 0; i < 16; ++i) db[i >> 3][i & 7] = 0.0f;
       }
     }
+  walk:
+    // behind a wait that gave up: the other front warps still meet this one
+    for (; p.biases && cur.n > 0; cur = after_live(cur))
+      for (int i = 0; i < 4; ++i) tc::bar_sync(1, kThreads);
   } else {
     // ------------------------------------------------------------- back warps
     constexpr int MODE = SHARED ? kScatter : kBackward;
