@@ -75,12 +75,12 @@ __device__ __forceinline__ float through(float v, float y) {
 // Operands in 16 bits go to the tensor core as they are.  An fp32 value goes
 // as two tf32 parts, x = hi + lo to 2^-22 |x|; the products hi hi are summed
 // in one accumulator and the three others in a second, which are added in
-// fp32 when the sum is read: about the accuracy of fp32 multiply-adds.
-// (A NaN all of whose payload lies in the 13 low bits counts as an infinity.)
-// Where the first accumulator is not finite it is the
-// result: the second has inf - inf and inf * 0 there, and is not finite only
-// where the first is not.  v_z of the
-// sigmoid in 16 bits goes as two parts in the same manner, so that it is not
+// fp32 when the sum is read.  A product is off by up to 3 2^-22: sums of a few are
+// off by two to three times what fp32 multiply-adds would be, longer ones by
+// no more.  (A NaN all of whose payload lies in the 13 low bits counts as an
+// infinity.)  Where the first accumulator is not finite it is the result: the
+// second has inf - inf and inf * 0 there, and is not finite only where the first is
+// not.  v_z of the sigmoid in 16 bits goes as two parts in the same manner, so that it is not
 // rounded to 16 bits on its way.  fp16 ends at 2^-24, next to the gradients of a
 // mean over an image, so its second part is held times 2^11 (it is at most 2^4:
 // half a step of the first) and what it gives is scaled back where the sums are
@@ -496,12 +496,13 @@ __device__ __forceinline__ void take_results(bool live, uint32_t acc, int second
 // the backward through an activation rewrites the panel as v_z.  The group's
 // weights are staged once per group, and stay.
 //
-// Bound by HBM where the MMAs keep up: 2 M rows 128-128 bf16 forward 180 us,
-// 5.7 TB/s of a copy's 6.5; v_x of 1.2 M rows 64-64 fp32, gathered, 180 us, 6.2
-// TB/s of DRAM traffic (the sums' lines are read and written).  fp32 at 128
-// features is bound by its four MMAs a step (600 k rows forward 204 us, twice
-// the floor).  A form that ran a tile's loads, MMAs and results one after the
-// other, two CTAs an SM, took 284 us of the first.
+// Bound by HBM for 16-bit rows: 2 M rows 128-128 bf16 forward 182 us, 5.6 TB/s of
+// a copy's 6.5; v_x of 1.2 M rows 64-64 fp32, gathered, 6.1 TB/s of DRAM traffic
+// (the sums' lines are read and written).  fp32 forwards wait: 600 k rows 128-128
+// take 203 us, where HBM needs 94 and the four MMAs a step 66 (with the copies and
+// low parts shared memory is busy for 89): only two panels of low parts are in
+// flight.  A form that ran a tile's loads, MMAs and results one after the other,
+// two CTAs an SM, took 284 us of the first.
 //
 // How rows arrive: by TMA; gathered, by two warps' copies; by copies of the
 // front warps.  (TMA's four-row gathers took 19 cycles a 128-byte row, 49 us
@@ -1204,9 +1205,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 // change accumulators, and the back warps add the finished one to sums that
 // they hold in registers.
 //
-// 1.2 M gathered rows 64-64: 200 us, 4.6 TB/s.  The MMAs (16 a panel, 48 cycles
-// each), the transposition and the copies share the shared memory's 128 bytes
-// a cycle: about 1400 of the 1500 cycles that a panel takes.
+// 1.2 M gathered rows 64-64: 212 us with the join, 4.4 TB/s.  The MMAs (16 a panel,
+// 48 cycles each), the transposition and the copies share the shared memory's 128
+// bytes a cycle: about 1400 of the 1500 cycles that a panel takes.  More than 64
+// outputs spill: the back warps' sums do not all fit a thread's 96 registers.
 constexpr int kFlush = 4;
 constexpr int kRows32 = 32;
 constexpr int kBox = kRows32 * 128;
@@ -1666,13 +1668,15 @@ struct BothArgs {
 // rows as lanes and the weights (v_x), and with rows as depth and x (v_W: both
 // operands are "MN-major" then, as the weights are in the first product), so
 // nothing is transposed.  The roles of the warps are those of the rows kernel.
-// HBM-bound: 2 M rows 128-128 bf16, relu, 319 us, 6.4 TB/s; v_x and v_W by kernels
-// of their own took 1107 us.
+// HBM-bound: 2 M rows 128-128 bf16, relu, 340 us with the join, 6.0 TB/s; v_x and
+// v_W by kernels of their own took 1107 us.
 //
 // v_W's accumulator is added to the CTA's place in `part` at the end of a
 // group, and every kPiece tiles: the tensor core cuts sums to fp32 instead of
-// rounding them, 2^-24 of the sum on average at each of a tile's 8 additions
-// (32 tiles: 2 M rows 128-128 were 2e-6 low).
+// rounding them, by 3 2^-25 of a growing sum at each of a tile's 8 steps.  With 32
+// tiles sums of one sign were 2.5e-5 low, with 4 they are 3e-6; the 2 M rows take
+// 340 us instead of 336 (in a long run, which power bounds, 361 instead of 350).
+// Another accumulator is filled meanwhile where v_z has one part.
 constexpr int kPiece = 4;
 constexpr int kBothBars = 30;
 
@@ -2095,9 +2099,10 @@ __global__ void __launch_bounds__(256) join_kernel(Shape s, int kp, int mp, int 
 // in registers, and of v_W's sums in the backward, which does all of its parts
 // in the one pass.  A warp has 16 / MP rows per lane in flight.
 //
-// 4 M gathered rows 32-3 fp32: 125 us (as tensor-core tiles 278), 4.1 TB/s of
-// scattered 128-byte row reads, which is what bounds it: 7% fewer instructions
-// changed nothing.  Its backward, 1.2 M rows: 125 us.
+// 4 M gathered rows 32-3 fp32: 127 us (as tensor-core tiles 278).  The 128-byte row
+// reads alone take 94 us, 5.4 TB/s; the rest is that a warp loads and uses its
+// rows in the same turn, with nothing under way while it adds up (7% fewer
+// instructions changed nothing).  Its backward, 1.2 M rows: 163 us.
 struct NarrowArgs {
   Shape s;
   const void* x;

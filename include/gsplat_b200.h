@@ -694,7 +694,7 @@ typedef struct {
   int32_t dtype;        /* gs_dtype of x, weights, biases, y and gradients  */
   int32_t activation;   /* gs_activation                                    */
   int32_t use_row_ids;  /* 1: row_ids is given; 0: id(r) = r                */
-  int32_t wait_selftest;/* 1: the kernels' first waits run out, after 4 us, as
+  int32_t wait_selftest; /* 1: the kernels' first waits run out, after 4 us, as
                            if what they wait for never came (a test of the
                            report: see gs_grouped_linear_check); else 0     */
   int32_t wanted;       /* the backward: gs_grouped_wanted bits of the gradients
@@ -708,12 +708,13 @@ typedef struct {
  * offsets[g + 1]: x [n,K], weights [G,M,K], biases [G,M] or NULL, offsets
  * [G+1] int32 ascending, row_ids [R] int32 (with use_row_ids), y [R,M].
  * Sums are in fp32 and rounded once; fp32 factors are carried to 2^-22 of
- * themselves (and to 2^-126).  The tensor core cuts sums instead of rounding
- * them, so that one of equal signs comes out low, by 3e-6 of itself at most; in
- * the 16-bit y and v_x, which are summed in one go, by 1e-7 for each 16 features
- * where that is more.  Rows outside every group are written
- * as zeros; an id outside [0, n) reads a row of zeros.  Offsets that do not
- * ascend give unspecified values and no access out of bounds. */
+ * themselves (and to 2^-126; a NaN with nothing but zeros in its upper 10
+ * fraction bits counts as an infinity).  The tensor core cuts sums instead of
+ * rounding them, so that one of equal signs comes out low, by some 3e-6 of
+ * itself; in the 16-bit y and v_x, which are summed in one go, by 1e-7 for each
+ * 16 features where that is more.  Rows outside every group are written as
+ * zeros; an id outside [0, n) reads a row of zeros.  Offsets that do not ascend
+ * give unspecified values and no access out of bounds. */
 int gs_grouped_linear_fwd(const gs_grouped_params* p, const void* x,
                           const int32_t* row_ids, const int32_t* offsets,
                           const void* weights, const void* biases, void* y,
@@ -729,10 +730,9 @@ size_t gs_grouped_linear_bwd_workspace_size(const gs_grouped_params* p);
  * read it of v_z[r] weights[g] (zeros where none does), v_weights [G,M,K] =
  * the sum over g's rows of v_z[r]^T x[id(r)], v_biases [G,M] = the sum of
  * v_z[r]; each may be NULL (not wanted).  Behind a sigmoid v_z is carried to
- * 2^-22 of itself and to 2^-36 in fp16, and to 2^-16 in bf16.  v_weights and
- * v_biases are summed
- * in a fixed order; v_x is too, except that with row_ids the rows of one id
- * are added atomically in fp32. */
+ * 2^-22 of itself and to 2^-36 in fp16, and to 2^-16 of itself in bf16.
+ * v_weights and v_biases are summed in a fixed order; v_x is too, except that
+ * with row_ids the rows of one id are added atomically in fp32. */
 int gs_grouped_linear_bwd(const gs_grouped_params* p, const void* x,
                           const int32_t* row_ids, const int32_t* offsets,
                           const void* weights, const void* y, const void* v_y,
