@@ -95,8 +95,8 @@ int device_word(uint32_t** word) {
   return GS_OK;
 }
 
-int gave_up() {
-  set_error("grouped_linear: a wait inside a kernel gave up: its call's results are void");
+int gave_up(const char* more) {
+  set_error("grouped_linear: a wait inside a kernel gave up: its call's results are void%s", more);
   return GS_ERR_DEVICE;
 }
 
@@ -106,7 +106,8 @@ int waits_of(const gs_grouped_params* p, WaitArgs* w) {
   w->status = p->status;
   if (p->status) return GS_OK;
   if (int rc = device_word(&w->status)) return rc;
-  return __atomic_load_n(w->status, __ATOMIC_ACQUIRE) ? gave_up() : GS_OK;
+  return __atomic_load_n(w->status, __ATOMIC_ACQUIRE)
+             ? gave_up("; refused until gs_grouped_linear_check has reported it") : GS_OK;
 }
 
 // Rows are counted in 32 bits, some tiles past the last.
@@ -212,5 +213,5 @@ extern "C" int gs_grouped_linear_check(gs_stream_t stream) {
   uint32_t* word = nullptr;
   if (int rc = device_word(&word)) return rc;
   if (!__atomic_exchange_n(word, 0u, __ATOMIC_ACQ_REL)) return GS_OK;
-  return gave_up();
+  return gave_up("");
 }
